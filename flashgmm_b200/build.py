@@ -15,7 +15,9 @@ def build_torch_ext(verbose=False):
     """Compile csrc/fgmm_torch.cpp against torch and libflashgmm_b200.so (found next to
     the extension at run time through its rpath)."""
     if os.path.exists("/usr/bin/g++"):
-        os.environ.setdefault("CXX", "/usr/bin/g++")
+        # the compiler that belongs to the libstdc++ of the process: one of another toolchain ($CXX)
+        # brings its own copies of the stream facets, and formatting a number in a message crashes
+        os.environ["CXX"] = "/usr/bin/g++"
     from torch.utils.cpp_extension import CUDA_HOME, load
     bdir = os.path.join(HERE, "csrc", "_build", "torch_ext")
     os.makedirs(bdir, exist_ok=True)
