@@ -6,10 +6,15 @@ import resolves here.  The reference's four ops (``flash_em_fused``, ``standard_
 ``flash_e_step``, ``standard_m_step``; ``flash_gmm/csrc/binding.cpp:94-108``) come from
 the compiled PyTorch extension ``flashgmm_b200/_fgmm_torch.so`` (pybind11 over this
 package's C ABI). The statistics / update building blocks of sharded and out-of-core fits
-come from :mod:`flashgmm_b200.flash_gmm_native`.  The reference's wrapper therefore runs
+come from :mod:`flashgmm_b200.flash_gmm_native`, the operators of a mixture of experts from
+:mod:`flashgmm_b200.experts`.  The reference's wrapper therefore runs
 unmodified on the CUDA kernels.
 """
 from flashgmm_b200._ext import load as _load_ext
+from flashgmm_b200 import experts as _experts
+from flashgmm_b200.experts import (  # noqa: F401
+    Routes, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
+    group_routes, route_experts, route_experts_backward)
 from flashgmm_b200.flash_gmm_native import (  # noqa: F401
     StatsWorkspace, em_stats, em_step, em_update, em_update_prepared, family_for,
     prepare_points, set_family, stats_len)
@@ -22,4 +27,4 @@ standard_m_step = _C.standard_m_step
 
 __all__ = ["flash_em_fused", "standard_e_step", "flash_e_step", "standard_m_step", "em_stats",
            "em_step", "em_update", "em_update_prepared", "prepare_points", "stats_len",
-           "family_for", "set_family", "StatsWorkspace"]
+           "family_for", "set_family", "StatsWorkspace", *_experts.__all__]

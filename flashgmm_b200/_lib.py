@@ -18,9 +18,13 @@ FGMM_ERR_WORKSPACE = 3
 FGMM_ERR_CUDA = 4
 FAMILY_AUTO, FAMILY_SIMT, FAMILY_TC, FAMILY_LOWK = 0, 1, 2, 3
 UPDATE_NO_FLOORS = 1
+F32, BF16, F16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID, SCORE_GIVEN = 0, 1, 2
+MAX_EXPERTS, MAX_TOP_K, MAX_SCORE_GROUPS = 4096, 32, 32
 
 # (name, restype, argtypes) for every symbol the header declares.
 _vp, _i64, _i32, _sz, _d = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t, ctypes.c_double
+_f = ctypes.c_float
 SIGNATURES = {
     "fgmm_last_error": (ctypes.c_char_p, []),
     "fgmm_version": (ctypes.c_int, []),
@@ -48,6 +52,21 @@ SIGNATURES = {
     "fgmm_e_step": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
     "fgmm_m_step_workspace_bytes": (ctypes.c_size_t, [_i64, _i32, _i32]),
     "fgmm_m_step": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgmm_route_experts": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _f,
+                                          _vp, _vp, _vp]),
+    "fgmm_route_experts_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _i64, _vp, _i32, _i32, _i32, _f,
+                                                   _vp, _vp]),
+    "fgmm_group_routes_workspace_bytes": (_sz, [_i64, _i32]),
+    "fgmm_group_routes": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgmm_expert_products_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "fgmm_expert_products": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _sz,
+                                            _vp]),
+    "fgmm_expert_products_backward_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "fgmm_expert_products_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp,
+                                                     _i32, _vp, _vp, _vp, _sz, _vp]),
+    "fgmm_combine_experts": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "fgmm_combine_experts_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp,
+                                                     _vp, _vp]),
 }
 
 _lib = None

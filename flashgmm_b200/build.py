@@ -1,6 +1,6 @@
 """Build the in-tree CUDA library (sm_100a) with ``make -C flashgmm_b200/csrc`` and the
 PyTorch op module ``flashgmm_b200/_fgmm_torch.so`` (pybind11 bindings over the library's
-C ABI, ``csrc/fgmm_torch.cpp``)."""
+C ABI, ``csrc/fgmm_torch.cpp`` and ``csrc/fgmm_torch_experts.cpp``)."""
 import os
 import shutil
 import subprocess
@@ -9,10 +9,11 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 EXT_NAME = "_fgmm_torch"
 EXT_PATH = os.path.join(HERE, EXT_NAME + ".so")
+TORCH_SOURCES = ("fgmm_torch.cpp", "fgmm_torch_experts.cpp")
 
 
 def build_torch_ext(verbose=False):
-    """Compile csrc/fgmm_torch.cpp against torch and libflashgmm_b200.so (found next to
+    """Compile the extension's sources against torch and libflashgmm_b200.so (found next to
     the extension at run time through its rpath)."""
     if os.path.exists("/usr/bin/g++"):
         # the compiler that belongs to the libstdc++ of the process: one of another toolchain ($CXX)
@@ -21,7 +22,7 @@ def build_torch_ext(verbose=False):
     from torch.utils.cpp_extension import CUDA_HOME, load
     bdir = os.path.join(HERE, "csrc", "_build", "torch_ext")
     os.makedirs(bdir, exist_ok=True)
-    load(name=EXT_NAME, sources=[os.path.join(HERE, "csrc", "fgmm_torch.cpp")],
+    load(name=EXT_NAME, sources=[os.path.join(HERE, "csrc", f) for f in TORCH_SOURCES],
          extra_cflags=["-O2", "-std=c++17"],
          extra_include_paths=[os.path.join(CUDA_HOME or "/usr/local/cuda", "include")],
          extra_ldflags=[f"-L{HERE}", "-lflashgmm_b200", r"-Wl,-rpath,\$$ORIGIN:\$$ORIGIN/../../.."],

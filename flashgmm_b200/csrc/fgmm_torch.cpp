@@ -122,6 +122,8 @@ std::vector<torch::Tensor> standard_m_step(torch::Tensor X, torch::Tensor gamma)
 
 }  // namespace
 
+void bind_experts(pybind11::module_ &m);  // fgmm_torch_experts.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "flashgmm_b200 CUDA ops with the reference's op-module interface";
   m.def("flash_em_fused", &flash_em_fused, "One fused EM iteration (CUDA)", py::arg("X"),
@@ -132,4 +134,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("X"), py::arg("mu"), py::arg("var"), py::arg("log_pi"), py::arg("BK") = 4);
   m.def("standard_m_step", &standard_m_step, "M-step from responsibilities (CUDA)", py::arg("X"),
         py::arg("gamma"));
+  bind_experts(m);
 }

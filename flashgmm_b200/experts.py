@@ -1,0 +1,180 @@
+"""Operators of a mixture of experts: a mixture whose K components each hold a linear map.
+
+The gate picks a few experts for every point (:func:`route_experts`: the E-step's softmax cut to
+its leading components, or a learned router's scores), the routes are grouped by expert
+(:func:`group_routes`), the experts' products run over the grouped rows
+(:func:`expert_products`), and a point's results are joined by its weights
+(:func:`combine_experts`)::
+
+    weights, indices = route_experts(scores, top_k=2)
+    routes = group_routes(indices, K)
+    y = expert_products(x, weight, routes)        # [N top_k, d_out], grouped by expert
+    out = combine_experts(y, weights, routes)     # [N, d_out]
+
+They take float32, bfloat16 or float16 CUDA tensors (weights, their gradients and the bias are float32,
+indices int32), run on the current stream of the tensors' device and hold their sums in 32 bits.  Where a tensor
+input requires a gradient, the functions record one; the ``*_backward`` functions are the same
+gradients without autograd; a step that is captured into a CUDA graph while an eager autograd graph of the
+same leaves is alive takes those (autograd then joins the eager graph's stream to the capture, which CUDA
+refuses).  The reference has no counterpart; its E-step
+(``flash_gmm/csrc/binding.cpp:35-49``) gives the scores of a fitted mixture's gate.
+"""
+from typing import NamedTuple
+
+import torch
+
+from . import _ext
+
+__all__ = ["Routes", "route_experts", "route_experts_backward", "group_routes", "expert_products",
+           "expert_products_backward", "combine_experts", "combine_experts_backward"]
+
+
+class Routes(NamedTuple):
+    """The N top_k routes of N points, grouped by expert (int32 CUDA tensors).
+
+    ``order[R]``: the routes sorted by expert (route ``n * top_k + j`` is slot j of point n), those
+    without an expert last; ``offsets[K + 1]``: where each expert's begin; ``position[N, top_k]``:
+    each route's place in ``order``, -1 for those without an expert."""
+    order: torch.Tensor
+    offsets: torch.Tensor
+    position: torch.Tensor
+
+
+def _check_tensors(**tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{name} must be a torch.Tensor")
+
+
+def _check_routes(routes):
+    if not isinstance(routes, Routes):
+        raise RuntimeError("routes must be a Routes (of group_routes)")
+    _check_tensors(order=routes.order, offsets=routes.offsets, position=routes.position)
+
+
+def _records(*tensors):
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale):
+        weights, indices = _ext.load().route_experts(scores, top_k, score_func, bias, n_groups, top_groups,
+                                                     renormalize, scale)
+        ctx.save_for_backward(scores, indices)
+        ctx.args = (score_func, renormalize, scale)
+        ctx.mark_non_differentiable(indices)
+        ctx.set_materialize_grads(False)
+        return weights, indices
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_weights, _):
+        if d_weights is None:
+            return (None,) * 8
+        scores, indices = ctx.saved_tensors
+        return (_ext.load().route_experts_backward(d_weights, scores, indices, *ctx.args),) + (None,) * 7
+
+
+def route_experts(scores, top_k, score_func="softmax", bias=None, n_groups=1, top_groups=None,
+                  renormalize=True, scale=1.0):
+    """The ``top_k`` experts of every point and their weights -> ``(weights[N, top_k] float32,
+    indices[N, top_k] int32)``, best first.
+
+    ``scores[N, K]``; ``score_func``: ``"softmax"`` over a row, ``"sigmoid"``, or ``"given"`` (the
+    scores are values already, responsibilities for example).  ``bias[K]`` (float32) is added for the
+    choice only, to keep the experts' loads balanced.  With ``n_groups > 1`` the experts form equal
+    consecutive groups and only the ``top_groups`` groups (default: all) with the largest sums of
+    their two best biased values are chosen from.  Ties go to the lowest index; the order is decided on
+    64-bit values, without bias and groups on the scores themselves.  ``renormalize`` divides a
+    point's weights by their sum, ``scale`` multiplies them.
+
+    A score of -inf or NaN is masked and +inf counts as the largest finite value; slots that no
+    unmasked expert is left for hold index -1 and weight 0.  K <= 4096, top_k <= 32, n_groups <= 32.
+    The weights carry a gradient to ``scores``; the choice and ``bias`` have none."""
+    _check_tensors(scores=scores)
+    if bias is not None:
+        _check_tensors(bias=bias)
+    if _records(scores):
+        return _Route.apply(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
+    return _ext.load().route_experts(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
+
+
+def route_experts_backward(d_weights, scores, indices, score_func="softmax", renormalize=True, scale=1.0):
+    """``d_scores[N, K]`` (of the scores' type) from the weights' gradient, for the ``indices`` that
+    :func:`route_experts` gave with the same ``score_func``, ``renormalize`` and ``scale``."""
+    _check_tensors(d_weights=d_weights, scores=scores, indices=indices)
+    return _ext.load().route_experts_backward(d_weights, scores, indices, score_func, renormalize, scale)
+
+
+def group_routes(indices, K):
+    """Groups the routes of ``indices[N, top_k]`` (int32) by expert -> :class:`Routes`, stable: an
+    expert's routes keep their order.  Indices outside [0, K) are routes without an expert."""
+    _check_tensors(indices=indices)
+    return Routes(*_ext.load().group_routes(indices, K))
+
+
+class _Products(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, order, offsets, position):
+        ctx.save_for_backward(x, weight, order, offsets, position)
+        return _ext.load().expert_products(x, weight, order, offsets, position)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, *plan = ctx.saved_tensors
+        dx, dw = _ext.load().expert_products_backward(dy, x, weight, *plan, ctx.needs_input_grad[0],
+                                                      ctx.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+def expert_products(x, weight, routes):
+    """``y[r] = weight[e] @ x[n]`` for every grouped row r of ``routes`` (point n, expert e) ->
+    ``y[N top_k, d_out]``; rows behind ``offsets[K]`` (routes without an expert) are 0.
+
+    ``x[N, d_in]`` and ``weight[K, d_out, d_in]`` of one type; gradients to both."""
+    _check_tensors(x=x, weight=weight)
+    _check_routes(routes)
+    if _records(x, weight):
+        return _Products.apply(x, weight, *routes)
+    return _ext.load().expert_products(x, weight, *routes)
+
+
+def expert_products_backward(dy, x, weight, routes, need_dx=True, need_dweight=True):
+    """``[dx, dweight]`` from ``dy[N top_k, d_out]`` (``None`` where not needed): dx sums a point's
+    rows in slot order, each row rounded to the inputs' type before; dweight sums an expert's rows."""
+    _check_tensors(dy=dy, x=x, weight=weight)
+    _check_routes(routes)
+    return list(_ext.load().expert_products_backward(dy, x, weight, *routes, need_dx, need_dweight))
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, order, offsets, position):
+        ctx.save_for_backward(y, weights, order, offsets, position)
+        return _ext.load().combine_experts(y, weights, order, offsets, position)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        dy, dw = _ext.load().combine_experts_backward(d_out, *ctx.saved_tensors)
+        return dy if ctx.needs_input_grad[0] else None, dw if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def combine_experts(y, weights, routes):
+    """``out[n] = sum_j weights[n, j] y[position[n, j]]`` -> ``out[N, d]``, slots without an expert
+    left out.  ``y[N top_k, d]`` as :func:`expert_products` gives it, ``weights[N, top_k]`` float32;
+    gradients to both."""
+    _check_tensors(y=y, weights=weights)
+    _check_routes(routes)
+    if _records(y, weights):
+        return _Combine.apply(y, weights, *routes)
+    return _ext.load().combine_experts(y, weights, *routes)
+
+
+def combine_experts_backward(d_out, y, weights, routes):
+    """``[dy, d_weights]`` from ``d_out[N, d]``; rows and slots of no expert get 0."""
+    _check_tensors(d_out=d_out, y=y, weights=weights)
+    _check_routes(routes)
+    return list(_ext.load().combine_experts_backward(d_out, y, weights, *routes))

@@ -20,10 +20,15 @@ Differences from the reference, all deliberate:
 import torch
 
 from . import _lib
+from . import experts as _experts
+from .experts import (  # noqa: F401
+    Routes, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
+    group_routes, route_experts, route_experts_backward)
 
 __all__ = ["flash_em_fused", "standard_e_step", "flash_e_step", "standard_m_step", "em_stats", "em_step",
            "StatsWorkspace",
-           "em_update", "em_update_prepared", "prepare_points", "stats_len", "family_for", "set_family"]
+           "em_update", "em_update_prepared", "prepare_points", "stats_len", "family_for", "set_family",
+           *_experts.__all__]
 
 
 def _stream_ptr(device):

@@ -52,6 +52,21 @@ class _EMModel:
     def predict(self, X: torch.Tensor) -> torch.Tensor:
         return self.predict_proba(X).argmax(dim=1)
 
+    def route(self, X: torch.Tensor, top_k: int, renormalize: bool = True):
+        """The ``top_k`` leading components of every point, best first, and their
+        responsibilities (divided by their sum unless ``renormalize`` is off) ->
+        ``(weights[N, top_k], indices[N, top_k])``: the E-step as a sparse gate."""
+        return _C.route_experts(self.predict_proba(X), top_k, score_func="given", renormalize=renormalize)
+
+    def mix_experts(self, X: torch.Tensor, weight: torch.Tensor, top_k: int) -> torch.Tensor:
+        """A mixture of linear experts ``weight[K, d_out, d]`` with the fitted mixture as its gate:
+        ``out[n] = sum_j w[n, j] weight[indices[n, j]] @ X[n]`` over :meth:`route`'s leading
+        components.  Gradients flow to ``weight`` and ``X`` through the experts, not the gate."""
+        X = self._to_device(X)
+        weights, indices = self.route(X.detach(), top_k)
+        routes = _C.group_routes(indices, self.K)
+        return _C.combine_experts(_C.expert_products(X, weight, routes), weights, routes)
+
 
 class NativeStandardGMM(_EMModel):
     """Standard EM (materialised L and gamma) on this package's CUDA kernels.

@@ -190,6 +190,84 @@ int fgmm_em_stats_profiled(const float *X, const void *points, int64_t N, int32_
                            void *workspace, size_t workspace_bytes, void *stream,
                            float *launch_ms, const char **names, int32_t n);
 
+/* ---- Mixture of experts ----
+ *
+ * The operators of a mixture whose K components each hold an expert (a linear map): the gate picks a few
+ * experts for every point, the points are grouped by expert, the experts' products run over the
+ * grouped rows, and a point's results are joined by its weights.  They have no counterpart in the
+ * reference; the gate is its E-step (flash_gmm/csrc/flash_gmm_cuda.cu:328-374) cut to the leading components.
+ *
+ * Element types of scores, x, weight, y and their gradients: FGMM_F32, FGMM_BF16, FGMM_F16, one type in a
+ * call; sums are held in fp32.  Weights, their gradients and the bias are fp32, indices int32.
+ * K <= FGMM_MAX_EXPERTS, top_k <= FGMM_MAX_TOP_K, N top_k < 2^31.  N = 0 is allowed. */
+#define FGMM_F32 0
+#define FGMM_BF16 1
+#define FGMM_F16 2
+#define FGMM_SCORE_SOFTMAX 0
+#define FGMM_SCORE_SIGMOID 1
+#define FGMM_SCORE_GIVEN 2
+#define FGMM_MAX_EXPERTS 4096
+#define FGMM_MAX_TOP_K 32
+#define FGMM_MAX_SCORE_GROUPS 32
+
+/* Routes every point to its top_k experts.  scores[n * row_stride + e]; s = softmax over the row,
+ * sigmoid, or the score as given (responsibilities, say); c = s + bias[e] (bias may be NULL; it
+ * moves the choice, not the weights).  With n_groups > 1 the K experts form equal consecutive
+ * groups, and only the top_groups groups with the largest sums of their two best c stay.  Chosen
+ * are the top_k largest c, best first, ties to the lowest index, the order decided on 64-bit
+ * values (without bias and groups on the scores themselves).  weights[n][j] = scale * s, divided by the
+ * chosen ones' sum if `renormalize` (0 where that is 0).  A score of -inf or NaN is masked, +inf
+ * counts as the largest finite fp32 value; a slot that no unmasked expert is left for has index -1
+ * and weight 0. */
+int fgmm_route_experts(const void *scores, int32_t dtype, int64_t N, int32_t K, int64_t row_stride,
+                       const float *bias, int32_t top_k, int32_t score_func, int32_t n_groups,
+                       int32_t top_groups, int32_t renormalize, float scale, float *weights,
+                       int32_t *indices, void *stream);
+
+/* d_scores[N][K] (of the scores' type) from d_weights[N][top_k] for the indices of
+ * fgmm_route_experts; indices outside [0, K) get nothing and pass nothing on.  The choice itself and
+ * the bias have no gradient. */
+int fgmm_route_experts_backward(const float *d_weights, const void *scores, int32_t dtype, int64_t N,
+                                int32_t K, int64_t row_stride, const int32_t *indices, int32_t top_k,
+                                int32_t score_func, int32_t renormalize, float scale, void *d_scores,
+                                void *stream);
+
+/* Groups the R = N top_k routes of indices[N][top_k] by expert, in their order: order[R] holds the
+ * routes sorted by expert (route n top_k + j is slot j of point n), those with an index outside
+ * [0, K) last; offsets[K + 1] where each expert's begin; position[R] each route's place in `order`,
+ * -1 for those without an expert. */
+size_t fgmm_group_routes_workspace_bytes(int64_t R, int32_t K);
+int fgmm_group_routes(const int32_t *indices, int64_t R, int32_t K, int32_t *order, int32_t *offsets,
+                      int32_t *position, void *workspace, size_t workspace_bytes, void *stream);
+
+/* y[r] = weight[e] x[n] for every grouped row r (route order[r] of point n, expert e), x[N][d_in],
+ * weight[K][d_out][d_in], y[N top_k][d_out]; rows of no expert are 0.  `order` and `offsets` are those of
+ * fgmm_group_routes: entries out of range are treated as rows of no expert, never read through. */
+size_t fgmm_expert_products_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
+                                            int32_t d_out, int32_t top_k);
+int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, const void *weight,
+                         int32_t K, int32_t d_out, const int32_t *order, const int32_t *offsets,
+                         int32_t top_k, void *y, void *workspace, size_t workspace_bytes, void *stream);
+
+/* dx[N][d_in] and d_weight[K][d_out][d_in] (either may be NULL) from dy[N top_k][d_out]. */
+size_t fgmm_expert_products_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
+                                                     int32_t d_out, int32_t top_k);
+int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, int64_t N, int32_t d_in,
+                                  const void *weight, int32_t K, int32_t d_out, const int32_t *order,
+                                  const int32_t *offsets, const int32_t *position, int32_t top_k,
+                                  void *dx, void *d_weight, void *workspace, size_t workspace_bytes,
+                                  void *stream);
+
+/* out[n] = sum_j weights[n][j] y[position[n][j]], y[N top_k][d], places outside [0, N top_k)
+ * skipped. */
+int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,
+                         const int32_t *position, int32_t top_k, void *out, void *stream);
+
+/* dy[N top_k][d] and d_weights[N][top_k] from d_out[N][d]; rows and slots of no expert get 0. */
+int fgmm_combine_experts_backward(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
+                                  const float *weights, const int32_t *order, const int32_t *offsets,
+                                  int32_t K, int32_t top_k, void *dy, float *d_weights, void *stream);
+
 /* Size of the fixed device scratch array behind fgmm_em_fused_static. */
 #define FGMM_STATIC_SCRATCH_BYTES (16u << 20)
 
