@@ -299,7 +299,10 @@ int fgmm_m_step(const float *X, int64_t N, int32_t d, const float *gamma, int32_
   return em_update(stats, (double)N, K, d, new_mu, new_var, new_log_pi, st, /*floors=*/false);
 }
 
-int fgmm_device_error(int reset) { return tc_device_error(reset != 0); }
+int fgmm_device_error(int reset) {
+  const int a = tc_device_error(reset != 0), b = experts_device_error(reset != 0);
+  return a ? a : b;
+}
 
 int fgmm_em_stats_launches(int64_t N, int32_t d, int32_t K) {
   const int fam = resolve_family(N, d, K);

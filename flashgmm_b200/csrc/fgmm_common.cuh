@@ -130,6 +130,7 @@ size_t tc_workspace_bytes(int64_t N, int d, int K);
 int tc_prepare_points(const float *X, int64_t N, int d, void *points, cudaStream_t stream);
 // Code of the first bounded-wait failure recorded by a tensor-core kernel (0 = none).
 int tc_device_error(bool reset);
+int experts_device_error(bool reset);  // the same of the experts' products (fgmm_experts_tc.cu)
 int tc_em_stats(const float *X, const void *points, int64_t N, int d, const float *mu,
                 const float *var, const float *log_pi, int K, double *stats,
                 float *log_norm, void *ws, cudaStream_t stream, const UpdateOut *update = nullptr,

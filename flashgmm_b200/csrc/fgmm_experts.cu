@@ -542,8 +542,13 @@ __global__ void __launch_bounds__(kSortWarps * 32) group_place_kernel(const int3
 template <typename T, int V>
 __device__ __forceinline__ void load_pack(const T *p, float (&f)[V]) {
   T raw[V];
-  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4 *>(raw) = __ldg(reinterpret_cast<const uint4 *>(p));
-  else raw[0] = __ldg(p);
+  if constexpr (V * sizeof(T) >= 16) {
+#pragma unroll
+    for (int i = 0; i < V * (int)sizeof(T) / 16; ++i)
+      reinterpret_cast<uint4 *>(raw)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+  } else {
+    raw[0] = __ldg(p);
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f32(raw[i]);
 }
@@ -557,8 +562,8 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
 }
 
 // tpr threads share a point; each owns packs of columns.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
+template <typename TY, typename T, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
                                                       const int32_t *__restrict__ position, int64_t N, int top_k, int tpr,
                                                       T *__restrict__ out) {
   const int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
@@ -570,7 +575,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ y, i
       if (p < 0 || p >= R) continue;
       const float w = weights ? __ldg(weights + n * top_k + j) : 1.0f;
       float f[V];
-      load_pack<T, V>(y + (int64_t)p * d + c, f);
+      load_pack<TY, V>(y + (int64_t)p * d + c, f);
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
     }
@@ -608,15 +613,15 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
   if (lane == 0 && known) d_weights[id] = dot;
 }
 
-template <typename T>
-int combine_forward_t(const T *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st) {
+template <typename TY, typename T>
+int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   int tpr = 1;
   while (tpr < 256 && tpr * (vec ? V : 1) < d) tpr *= 2;
   const unsigned grid = (unsigned)cdiv(N, 256 / tpr);
-  if (vec) combine_kernel<T, V><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
-  else combine_kernel<T, 1><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
+  if (vec) combine_kernel<TY, T, V><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
+  else combine_kernel<TY, T, 1><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
   FGMM_LAUNCH_CHECK("combine_kernel");
   return FGMM_OK;
 }
@@ -689,6 +694,13 @@ int combine_forward(const void *y, int dtype, int64_t R, int d, const float *wei
   if (dtype == FGMM_F32) return combine_forward_t((const float *)y, R, d, weights, position, N, top_k, (float *)out, st);
   if (dtype == FGMM_BF16) return combine_forward_t((const __nv_bfloat16 *)y, R, d, weights, position, N, top_k, (__nv_bfloat16 *)out, st);
   return combine_forward_t((const __half *)y, R, d, weights, position, N, top_k, (__half *)out, st);
+}
+
+int sum_rows(const float *rows, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
+             cudaStream_t st) {
+  if (dtype == FGMM_F32) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (float *)out, st);
+  if (dtype == FGMM_BF16) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__nv_bfloat16 *)out, st);
+  return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__half *)out, st);
 }
 
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,

@@ -54,18 +54,21 @@ int route_backward(const float *dw, const void *scores, int dtype, int64_t N, in
 size_t group_workspace_bytes(int64_t R, int K);
 int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32_t *offsets,
                  int32_t *position, void *ws, cudaStream_t st);
-// out[n] = sum_j w[n][j] y[position[n][j]] (weights null: 1), positions outside [0, R) skipped.
+// out[n] = sum_j w[n][j] y[position[n][j]], positions outside [0, R) skipped.
 int combine_forward(const void *y, int dtype, int64_t R, int d, const float *weights,
                     const int32_t *position, int64_t N, int top_k, void *out, cudaStream_t st);
+// The same of fp32 rows with weights 1.
+int sum_rows(const float *rows, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
+             cudaStream_t st);
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,
                      const RoutePlan &plan, void *dy, float *d_weights, cudaStream_t st);
 
-// ---- fgmm_experts_simt.cu: CUDA-core products, any size and type ----
-int products_simt(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
-                  const RoutePlan &plan, void *y, cudaStream_t st);
-int products_simt_dx(const void *dy, const void *weight, int dtype, int d_in, int d_out,
-                     const RoutePlan &plan, void *dx_rows, cudaStream_t st);
-int products_simt_dw(const void *dy, const void *x, int dtype, int64_t N, int d_in, int d_out,
-                     const RoutePlan &plan, void *dweight, cudaStream_t st);
+// ---- fgmm_experts_tc.cu ----
+size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, bool backward);
+int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y,
+                void *ws, cudaStream_t st);
+// dx_rows[R][d_in] and d_weight, either may be null.
+int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
+                         const RoutePlan &p, float *dx_rows, void *d_weight, void *ws, cudaStream_t st);
 
 }  // namespace fgmm

@@ -98,7 +98,7 @@ int fgmm_group_routes(const int32_t *indices, int64_t R, int32_t K, int32_t *ord
 size_t fgmm_expert_products_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                             int32_t d_out, int32_t top_k) {
   if (check_experts(dtype, N, K, top_k) || check_widths(d_in, d_out)) return 0;
-  return 256;
+  return products_tc_workspace(dtype, N, K, d_in, d_out, top_k, false);
 }
 
 int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, const void *weight,
@@ -109,18 +109,18 @@ int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, 
   if (rc || N == 0) return rc;
   if (!x || !weight || !order || !offsets || !y || !workspace) return fail(FGMM_ERR_INVALID, "null pointer argument");
   const size_t es = elem_size(dtype);
-  if (!aligned(x, es) || !aligned(weight, es) || !aligned(y, es) || !aligned(workspace, 256))
-    return fail(FGMM_ERR_INVALID, "x, weight and y must be aligned to their elements, the workspace to 256 bytes");
+  if (!aligned(x, 16) || !aligned(weight, 16) || !aligned(y, es) || !aligned(workspace, 256))
+    return fail(FGMM_ERR_INVALID, "x and weight must be 16-byte aligned, y to its elements, the workspace to 256 bytes");
   if (workspace_bytes < fgmm_expert_products_workspace_bytes(dtype, N, K, d_in, d_out, top_k))
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
-  return products_simt(x, weight, dtype, N, d_in, d_out, plan, y, (cudaStream_t)stream);
+  return products_tc(x, weight, dtype, N, d_in, d_out, plan, y, workspace, (cudaStream_t)stream);
 }
 
 size_t fgmm_expert_products_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                                      int32_t d_out, int32_t top_k) {
   if (check_experts(dtype, N, K, top_k) || check_widths(d_in, d_out)) return 0;
-  return align_up((size_t)N * top_k * d_in * elem_size(dtype), 256) + 256;
+  return products_tc_workspace(dtype, N, K, d_in, d_out, top_k, true) + align_up((size_t)N * top_k * d_in * sizeof(float), 256);
 }
 
 int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, int64_t N, int32_t d_in,
@@ -139,18 +139,18 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
   }
   if (!dy || !order || !offsets || !workspace || (dx && (!weight || !position)) || (d_weight && !x))
     return fail(FGMM_ERR_INVALID, "null pointer argument");
-  if (!aligned(dy, es) || !aligned(x, es) || !aligned(weight, es) || !aligned(dx, es) || !aligned(d_weight, es) ||
+  if (!aligned(dy, 16) || !aligned(x, 16) || !aligned(weight, 16) || !aligned(dx, es) || !aligned(d_weight, es) ||
       !aligned(workspace, 256))
-    return fail(FGMM_ERR_INVALID, "matrices must be aligned to their elements, the workspace to 256 bytes");
+    return fail(FGMM_ERR_INVALID, "dy, x and weight must be 16-byte aligned, the results to their elements, the workspace to 256 bytes");
   if (workspace_bytes < fgmm_expert_products_backward_workspace_bytes(dtype, N, K, d_in, d_out, top_k))
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
-  if (dx) {
-    rc = products_simt_dx(dy, weight, dtype, d_in, d_out, plan, workspace, st);
-    if (!rc) rc = combine_forward(workspace, dtype, plan.R, d_in, nullptr, position, N, top_k, dx, st);
-    if (rc) return rc;
-  }
-  return d_weight ? products_simt_dw(dy, x, dtype, N, d_in, d_out, plan, d_weight, st) : FGMM_OK;
+  // the rows of dx first, in fp32: their sum over a point's slots rounds once
+  float *dx_rows = dx ? static_cast<float *>(workspace) : nullptr;
+  void *rest = static_cast<char *>(workspace) + align_up((size_t)plan.R * d_in * sizeof(float), 256);
+  rc = products_tc_backward(dy, x, weight, dtype, N, d_in, d_out, plan, dx_rows, d_weight, rest, st);
+  if (rc || !dx) return rc;
+  return sum_rows(dx_rows, dtype, plan.R, d_in, position, N, top_k, dx, st);
 }
 
 int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,

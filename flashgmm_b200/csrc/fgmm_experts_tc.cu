@@ -1,0 +1,637 @@
+// Products of experts on the tcgen05 tensor cores.
+//
+//   rows x weight    Y[r, o]     = sum_i X[point(r), i] W[e(r), o, i]
+//   rows x weight^T  DX[r, i]    = sum_o DY[r, o] W[e(r), o, i]
+//   sums over rows   DW[e, o, i] = sum_{r of e} DY[r, o] X[point(r), i]
+//
+// One persistent, warp-specialised kernel: a producer warp fills a ring of stages by TMA, one thread issues
+// tcgen05.mma into a double-buffered tensor-memory accumulator, four warps read it back and write the
+// results, and the next tile's products run meanwhile.  A tile has M = 128 rows of one expert (or, for
+// DW, 128 of its output dimensions) and NT columns; a stage holds 64 elements of the contraction.
+//   * A point's row of X is fetched by TMA gather4 straight from the points' matrix, four rows an
+//     instruction, so the grouped copy of X is never written.  Rows a tile does not have are not
+//     loaded: their accumulator rows hold leftovers that nobody reads.  Where the rows are the contraction (DW)
+//     they are fetched as rows outside the tensor, which are zeros in both operands.
+//   * W is fetched as a box of its 3-D tensor, K-major for Y, and MN-major, without a transposed copy, for DX.
+//   * float32 operands are three bf16 planes (x = b0 + b1 + b2, 24 bits together), laid out by
+//     split_planes_kernel, and the six products that matter (b0 b0 into one accumulator; b0 b1, b1 b0, b1 b1,
+//     b0 b2 and b2 b0, 2^-8 and less of it, into another).  Tensor-memory accumulation truncates, so the
+//     first is drained into fp32 registers every 256 elements of the contraction.
+//   * 16-bit operands whose rows are no multiple of 16 bytes are copied to padded rows first (TMA strides).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <algorithm>
+#include <mutex>
+
+#include "fgmm_experts.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fgmm {
+using namespace ptx;
+
+namespace {
+
+constexpr int BM = 128;       // tile rows (MMA M)
+constexpr int KCH = 64;       // contraction elements of a stage (128-byte rows)
+constexpr int kThreads = 256;  // warp 0 producer, warp 1 MMA, warps 2-3 rows of no expert, warps 4-7 epilogue
+constexpr int kSegment = 4;   // stages between drains of a float32 product (256 elements)
+
+enum { kForward = 0, kInputs = 1, kWeights = 2 };
+
+template <int NT, bool SPLIT>
+struct Shape {
+  static constexpr int kPlanes = SPLIT ? 3 : 1;
+  static constexpr int kA = BM * KCH * 2, kB = NT * KCH * 2;  // bytes of one plane's tile
+  static constexpr int kStage = kPlanes * (kA + kB);
+  static constexpr int kStages = (192 * 1024) / kStage;
+  static constexpr int kOut = 4 * 32 * 128;  // a 32-row, 128-byte staging tile for each epilogue warp
+  static constexpr int kBars = 256;
+  static constexpr int smem(int K) { return 1024 + kStages * kStage + kOut + kBars + (K + 1) * 4; }
+  static_assert(kStages >= 2, "shared-memory budget");
+  static_assert(smem(kMaxExperts) <= 227 * 1024, "shared-memory budget");
+};
+
+struct TcArgs {
+  RoutePlan plan;
+  int64_t N;
+  int d_in, d_out;
+  int a_plane, b_plane;  // columns between the planes of A's and B's rows (float32)
+  uint32_t idesc;
+  int vec;  // rows of the result start on 16-byte boundaries
+};
+
+// What one tile covers.  For Y and DX: expert e, rows [r0, r0 + rows), columns from n0.  For DW: expert e, output
+// dimensions from m0 (`rows` of them), columns from n0, contraction over the rows [r0, r1).
+struct Tile {
+  int e, r0, r1, rows, m0, n0, nk;
+};
+
+template <int MODE, int NT>
+struct Tiles {
+  const TcArgs &a;
+  const int *s_tile;  // first tile of rows of each expert (Y, DX)
+  int n_tiles, m_tiles, total, e = 0;
+
+  __device__ Tiles(const TcArgs &args, const int *st) : a(args), s_tile(st) {
+    const int width = MODE == kForward ? a.d_out : a.d_in;
+    n_tiles = (width + NT - 1) / NT;
+    m_tiles = (a.d_out + BM - 1) / BM;
+    total = MODE == kWeights ? a.plan.K * m_tiles * n_tiles : s_tile[a.plan.K] * n_tiles;
+  }
+  // t never decreases from call to call.
+  __device__ Tile at(int t) {
+    Tile x;
+    const int R = (int)a.plan.R;
+    x.n0 = t % n_tiles * NT;
+    const int m = t / n_tiles;
+    if (MODE == kWeights) {
+      x.e = m / m_tiles;
+      x.m0 = m % m_tiles * BM;
+      x.rows = min(BM, a.d_out - x.m0);
+      expert_rows(a.plan.offsets, x.e, R, x.r0, x.r1);
+      x.nk = (x.r1 - x.r0 + KCH - 1) / KCH;
+    } else {
+      while (e + 1 < a.plan.K && s_tile[e + 1] <= m) ++e;
+      x.e = e;
+      x.m0 = 0;
+      expert_rows(a.plan.offsets, e, R, x.r0, x.r1);
+      x.r0 += (m - s_tile[e]) * BM;
+      x.rows = max(0, min(BM, x.r1 - x.r0));
+      x.nk = ((MODE == kForward ? a.d_in : a.d_out) + KCH - 1) / KCH;
+    }
+    return x;
+  }
+};
+
+template <typename OUT>
+__device__ __forceinline__ uint4 pack16(const float *v) {
+  if constexpr (sizeof(OUT) == 4) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  } else {
+    OUT h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = from_f32<OUT>(v[i]);
+    return *reinterpret_cast<uint4 *>(h);
+  }
+}
+
+template <int MODE, int NT, bool SPLIT, typename OUT>
+__global__ void __launch_bounds__(kThreads, 1)
+experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                  const __grid_constant__ TcArgs a, OUT *__restrict__ out) {
+  using Sh = Shape<NT, SPLIT>;
+  constexpr int P = Sh::kPlanes, S = Sh::kStages;
+  constexpr int kCols = SPLIT ? 4 * NT : 2 * NT;  // tensor-memory columns
+  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "TMEM budget");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *s_out = smem + S * Sh::kStage;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(s_out + Sh::kOut);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_out + Sh::kOut + Sh::kBars - 64);
+  int *s_warp = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars - 48);  // [8]
+  int *s_tile = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars);        // [K + 1]
+  const uint32_t bar0 = smem_u32(bars);
+  auto FULL = [&](int s) { return bar0 + 8u * s; };
+  auto EMPTY = [&](int s) { return bar0 + 8u * (S + s); };
+  auto TFULL = [&](int b) { return bar0 + 8u * (2 * S + b); };
+  auto TEMPTY = [&](int b) { return bar0 + 8u * (2 * S + 2 + b); };
+  const uint32_t DONE = bar0 + 8u * (2 * S + 4);
+  static_assert(8 * (2 * S + 5) <= Sh::kBars - 64, "barrier space");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int R = (int)a.plan.R, K = a.plan.K;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) { mbar_init(FULL(i), 1); mbar_init(EMPTY(i), 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(TFULL(b), 1); mbar_init(TEMPTY(b), 4); }
+    mbar_init(DONE, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(tmem_slot), kCols);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  if (MODE != kWeights) {  // first tile of rows of each expert
+    const int per = (K + kThreads - 1) / kThreads;
+    const int e0 = min(K, (int)threadIdx.x * per), e1 = min(K, e0 + per);
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) {
+      int lo, hi;
+      expert_rows(a.plan.offsets, e, R, lo, hi);
+      mine += (hi - lo + BM - 1) / BM;
+    }
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) s_warp[warp] = sum;
+    __syncthreads();
+    int run = sum - mine;
+    for (int w = 0; w < warp; ++w) run += s_warp[w];
+    for (int e = e0; e < e1; ++e) {
+      int lo, hi;
+      expert_rows(a.plan.offsets, e, R, lo, hi);
+      s_tile[e] = run;
+      run += (hi - lo + BM - 1) / BM;
+    }
+    if (threadIdx.x == kThreads - 1) s_tile[K] = run;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_launch();
+  const uint32_t tmem = *tmem_slot;
+  Tiles<MODE, NT> tiles(a, s_tile);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    int stage = 0;
+    uint32_t phase = 0;
+    int filled = 0;  // stages ever armed, up to S
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x) {
+      const Tile x = tiles.at(t);
+      int src[4];  // Y: the points of this lane's four rows
+      if (MODE == kForward) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = lane * 4 + i;
+          const int p = r < x.rows ? row_point(a.plan.order, x.r0 + r, R, a.plan.top_k) : -1;
+          src[i] = p >= 0 ? p : (int)a.N;  // a row outside the tensor: zeros
+        }
+      }
+      for (int c = 0; c < x.nk; ++c) {
+        ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty) : 0, 0);
+        if (!ok) break;
+        const uint32_t base = smem_u32(smem + stage * Sh::kStage), base_b = base + P * Sh::kA;
+        if (MODE == kForward) {
+          const int quads = (x.rows + 3) / 4;
+          if (lane == 0) mbar_arrive_expect_tx(FULL(stage), P * (quads * 512 + Sh::kB));
+          __syncwarp();
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            if (lane < quads)
+              tma_gather4(base + p * Sh::kA + lane * 512, &tm_a, p * a.a_plane + c * KCH, src[0], src[1], src[2], src[3], FULL(stage));
+            if (lane == 0) tma_load_3d(base_b + p * Sh::kB, &tm_b, p * a.b_plane + c * KCH, x.n0, x.e, FULL(stage));
+          }
+        } else if (MODE == kInputs) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(FULL(stage), Sh::kStage);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+              tma_load_2d(base + p * Sh::kA, &tm_a, p * a.a_plane + c * KCH, x.r0, FULL(stage));
+#pragma unroll
+              for (int j = 0; j < NT / 64; ++j)
+                tma_load_3d(base_b + p * Sh::kB + j * 64 * 128, &tm_b, p * a.b_plane + x.n0 + j * 64, c * KCH, x.e, FULL(stage));
+            }
+          }
+        } else {
+          // 64 rows of the contraction: lanes 0-15 fetch four each of DY, lanes 16-31 of X
+          const int q = lane & 15, r = x.r0 + c * KCH + q * 4;
+          int row[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (lane < 16) {
+              row[i] = r + i < x.r1 ? r + i : R;
+            } else {
+              const int p = r + i < x.r1 ? row_point(a.plan.order, r + i, R, a.plan.top_k) : -1;
+              row[i] = p >= 0 ? p : (int)a.N;
+            }
+          }
+          if (lane == 0) mbar_arrive_expect_tx(FULL(stage), Sh::kStage);
+          __syncwarp();
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            if (lane < 16) {
+#pragma unroll
+              for (int j = 0; j < BM / 64; ++j)
+                tma_gather4(base + p * Sh::kA + j * 64 * 128 + q * 512, &tm_a, p * a.a_plane + x.m0 + j * 64, row[0], row[1], row[2], row[3], FULL(stage));
+            } else {
+#pragma unroll
+              for (int j = 0; j < NT / 64; ++j)
+                tma_gather4(base_b + p * Sh::kB + j * 64 * 128 + q * 512, &tm_b, p * a.b_plane + x.n0 + j * 64, row[0], row[1], row[2], row[3], FULL(stage));
+            }
+          }
+        }
+        __syncwarp();
+        filled = min(S, filled + 1);
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+    }
+    // no copy may land after the CTA ends: wait for the last fills of the ring
+    if (lane == 0) {
+      for (int i = 0; i < filled; ++i) {
+        stage = stage == 0 ? S - 1 : stage - 1;
+        if (stage == S - 1) phase ^= 1;
+        mbar_wait_drain(FULL(stage), phase);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA
+    if (lane == 0) {
+      // K-major tiles: 8-row groups 1 KB apart, a k-step of 16 elements is 32 bytes.  MN-major tiles: atoms of 64
+      // columns 8 KB apart, 8-row groups 1 KB apart, a k-step of 16 rows is 2 KB.
+      constexpr bool kAmn = MODE == kWeights, kBmn = MODE != kForward;
+      const uint64_t a0 = sdesc_sw128(smem_u32(smem), kAmn ? KCH * 128 : 16, 1024);
+      const uint64_t b0 = sdesc_sw128(smem_u32(smem) + P * Sh::kA, kBmn ? KCH * 128 : 16, 1024);
+      constexpr uint64_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;
+      constexpr uint64_t kPlA = Sh::kA >> 4, kPlB = Sh::kB >> 4;
+      int stage = 0, seg = 0, count = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, ++count) {
+        const int nk = tiles.at(t).nk;
+        const uint32_t low = tmem + (2 + (count & 1)) * NT;  // the smaller products of a float32 tile
+        int c = 0;
+        do {  // a segment: the whole tile, or kSegment stages of a float32 one
+          const int buf = seg & 1;
+          if (!mbar_wait(TEMPTY(buf), ((seg >> 1) & 1) ^ 1, kErrWaitTmemEmpty)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem + buf * NT;
+          const int first = c, end = SPLIT ? min(nk, c + kSegment) : nk;
+          for (; c < end; ++c) {
+            if (!mbar_wait(FULL(stage), phase, kErrWaitFull)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t ad = a0 + (uint64_t)((stage * Sh::kStage) >> 4), bd = b0 + (uint64_t)((stage * Sh::kStage) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < KCH / 16; ++kk) {
+              const uint64_t ak = ad + kk * kStepA, bk = bd + kk * kStepB;
+              if constexpr (SPLIT) {
+                mma_f16(low, ak + 2 * kPlA, bk, a.idesc, (c != 0 || kk != 0) ? 1u : 0u);
+                mma_f16(low, ak, bk + 2 * kPlB, a.idesc, 1u);
+                mma_f16(low, ak + kPlA, bk + kPlB, a.idesc, 1u);
+                mma_f16(low, ak + kPlA, bk, a.idesc, 1u);
+                mma_f16(low, ak, bk + kPlB, a.idesc, 1u);
+              }
+              mma_f16(d, ak, bk, a.idesc, (c != first || kk != 0) ? 1u : 0u);
+            }
+            mma_commit(EMPTY(stage));
+            if (++stage == S) { stage = 0; phase ^= 1; }
+          }
+          if (!ok) break;
+          mma_commit(TFULL(buf));
+          ++seg;
+        } while (c < nk);
+      }
+      mma_commit(DONE);
+      mbar_wait_drain(DONE, 0);
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ---------------------------------------------------------------- rows of no expert
+    if (MODE == kForward) {
+      const int64_t first = (int64_t)min(max(__ldg(a.plan.offsets + K), 0), R) * a.d_out, end = (int64_t)R * a.d_out;
+      for (int64_t i = first + blockIdx.x * 64 + threadIdx.x - 64; i < end; i += (int64_t)gridDim.x * 64) out[i] = from_f32<OUT>(0.0f);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    constexpr int CW = 128 / sizeof(OUT), EPV = 16 / sizeof(OUT);  // columns of a staging row, of 16 bytes
+    constexpr int W = SPLIT ? NT : CW;                             // columns held in registers
+    const int q = warp & 3;
+    const uint32_t lane_tmem = tmem + ((uint32_t)(q * 32) << 16);
+    uint8_t *stg = s_out + q * 32 * 128;
+    const int width = MODE == kForward ? a.d_out : a.d_in;
+    int seg = 0, count = 0;
+    bool ok = true;
+    // 32 rows x CW columns (from column c0 of the tile) through shared memory, so that the global writes are whole lines
+    auto write = [&](const float *v, const Tile &x, int c0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint4 *>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack16<OUT>(v + j * EPV);
+      __syncwarp();
+      const int64_t row0 = MODE == kWeights ? (int64_t)x.e * a.d_out + x.m0 : x.r0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3), j = lane & 7;
+        const int col = x.n0 + c0 + j * EPV;
+        if (q * 32 + r < x.rows && col < width) {
+          const uint4 u = *reinterpret_cast<const uint4 *>(stg + r * 128 + ((j ^ (r & 7)) << 4));
+          OUT *p = out + (row0 + q * 32 + r) * width + col;
+          if (a.vec) {  // then the width is a multiple of EPV
+            *reinterpret_cast<uint4 *>(p) = u;
+          } else {
+            OUT h[EPV];
+            *reinterpret_cast<uint4 *>(h) = u;
+#pragma unroll
+            for (int k = 0; k < EPV; ++k)
+              if (col + k < width) p[k] = h[k];
+          }
+        }
+      }
+      __syncwarp();
+    };
+    for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, ++count) {
+      const Tile x = tiles.at(t);
+      const bool live = q * 32 < x.rows;
+      float acc[W];
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[i] = 0.0f;
+      }
+      int c = 0;
+      do {
+        const int buf = seg & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(TFULL(buf), (seg >> 1) & 1, kErrWaitTmemFull));
+        if (!ok) break;
+        tc_fence_after();
+        c = SPLIT ? c + kSegment : x.nk;
+        if constexpr (SPLIT) {
+          if (live && x.nk > 0) {
+#pragma unroll
+            for (int i = 0; i < NT / 32; ++i) {
+              float v[32];
+              tmem_ld32(lane_tmem + buf * NT + i * 32, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) acc[i * 32 + k] += v[k];
+            }
+            if (c >= x.nk) {
+#pragma unroll
+              for (int i = 0; i < NT / 32; ++i) {
+                float v[32];
+                tmem_ld32(lane_tmem + (2 + (count & 1)) * NT + i * 32, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) acc[i * 32 + k] += v[k];
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(TEMPTY(buf));
+          if (c >= x.nk && live) {
+#pragma unroll
+            for (int i = 0; i < NT / CW; ++i) write(acc + i * CW, x, i * CW);
+          }
+        } else {
+          if (live) {
+            for (int i = 0; i < NT / CW; ++i) {
+              if (x.n0 + i * CW >= width) break;
+#pragma unroll
+              for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
+              tmem_wait_ld();
+              if (x.nk == 0) {  // an expert without a row
+#pragma unroll
+                for (int k = 0; k < CW; ++k) acc[k] = 0.0f;
+              }
+              write(acc, x, i * CW);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(TEMPTY(buf));
+        }
+        ++seg;
+      } while (c < x.nk);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+// Rows of `cols` elements to rows of PLANES planes of `colsp` (zeros behind cols): float32 in three bf16
+// planes whose sum it is (to 2^-24), 16-bit types as they are.  An infinite value keeps zeros in the lower planes.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) split_planes_kernel(const T *__restrict__ src, int64_t rows, int cols, int colsp,
+                                                           uint16_t *__restrict__ dst) {
+  griddep_launch();
+  griddep_wait();
+  const int per = colsp / 8;
+  const int64_t n = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    const T *p = src + r * cols + c;
+    uint16_t h[PLANES][8];
+    if constexpr (PLANES == 3) {
+      float v[8];
+      if (cols % 4 == 0 && c + 8 <= cols) {
+        *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(p));
+        *reinterpret_cast<float4 *>(v + 4) = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(p[k]) : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const __nv_bfloat16 b0 = __float2bfloat16_rn(v[k]);
+        float rest = v[k] - __bfloat162float(b0);
+        if (!isfinite(rest)) rest = 0.0f;
+        const __nv_bfloat16 b1 = __float2bfloat16_rn(rest);
+        const __nv_bfloat16 b2 = __float2bfloat16_rn(rest - __bfloat162float(b1));
+        h[0][k] = __bfloat16_as_ushort(b0);
+        h[1][k] = __bfloat16_as_ushort(b1);
+        h[2][k] = __bfloat16_as_ushort(b2);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[0][k] = c + k < cols ? reinterpret_cast<const uint16_t *>(p)[k] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q)
+      *reinterpret_cast<uint4 *>(dst + (r * PLANES + q) * colsp + c) = *reinterpret_cast<uint4 *>(h[q]);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// A matrix as the kernel reads it: rows of planes * plane 16-bit columns.
+struct Operand {
+  const void *p;
+  int64_t rows;
+  int cols;   // columns of a row in memory (all planes)
+  int plane;  // columns of a plane
+};
+
+// 2-D map with a box of 64 columns x box_rows, or, with depth > 0, a 3-D one of `depth` matrices.
+int make_map(CUtensorMap *m, const Operand &o, int bf16, int box_rows, int depth) {
+  auto fn = encode_fn();
+  if (!fn) return fail(FGMM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int rank = depth > 0 ? 3 : 2;
+  const int64_t rows = depth > 0 ? o.rows / depth : o.rows;
+  cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)rows, (cuuint64_t)depth};
+  cuuint64_t strides[2] = {(cuuint64_t)o.cols * 2, (cuuint64_t)o.cols * 2 * rows};
+  cuuint32_t box[3] = {KCH, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                        const_cast<void *>(o.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FGMM_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return FGMM_OK;
+}
+
+bool needs_copy(int dtype, int cols) { return dtype == FGMM_F32 || cols % 8 != 0; }
+int plane_cols(int dtype, int cols) { return (int)align_up(cols, dtype == FGMM_F32 ? KCH : 8); }
+size_t copy_elems(int dtype, int64_t rows, int cols) {
+  return needs_copy(dtype, cols) ? (size_t)rows * plane_cols(dtype, cols) * (dtype == FGMM_F32 ? 3 : 1) : 0;
+}
+
+// The operand of `src` [rows][cols], copied into `dst` where TMA cannot read it as it is.
+int operand(Operand *o, const void *src, int dtype, int64_t rows, int cols, uint16_t *dst, cudaStream_t st) {
+  if (!needs_copy(dtype, cols)) {
+    *o = {src, rows, cols, cols};
+    return FGMM_OK;
+  }
+  const int colsp = plane_cols(dtype, cols);
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(rows * (colsp / 8), 256), 8 * num_sms());
+  if (dtype == FGMM_F32)
+    FGMM_CUDA_TRY(launch_pdl(split_planes_kernel<float, 3>, dim3(grid), dim3(256), 0, st, (const float *)src, rows, cols, colsp, dst));
+  else
+    FGMM_CUDA_TRY(launch_pdl(split_planes_kernel<__half, 1>, dim3(grid), dim3(256), 0, st, (const __half *)src, rows, cols, colsp, dst));
+  const int planes = dtype == FGMM_F32 ? 3 : 1;
+  *o = {dst, rows, colsp * planes, colsp};
+  return FGMM_OK;
+}
+
+template <int MODE, int NT, bool SPLIT, typename OUT>
+int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
+           cudaStream_t st) {
+  using Sh = Shape<NT, SPLIT>;
+  const int bf16 = dtype != FGMM_F16, width = MODE == kForward ? d_out : d_in;
+  CUtensorMap ma, mb;
+  int rc = make_map(&ma, oa, bf16, MODE == kInputs ? BM : 1, 0);
+  if (!rc) rc = MODE == kWeights ? make_map(&mb, ob, bf16, 1, 0) : make_map(&mb, ob, bf16, MODE == kForward ? NT : KCH, p.K);
+  if (rc) return rc;
+  TcArgs a{};
+  a.plan = p;
+  a.N = N;
+  a.d_in = d_in;
+  a.d_out = d_out;
+  a.a_plane = oa.plane;
+  a.b_plane = ob.plane;
+  a.idesc = idesc_f16(BM, NT, MODE == kWeights, MODE != kForward, bf16);
+  a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
+  static std::atomic<bool> done[64];  // per device
+  int dev = 0;
+  FGMM_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(kMaxExperts)));
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+  }
+  const int64_t m_tiles = MODE == kWeights ? (int64_t)p.K * cdiv(d_out, BM) : cdiv(p.R, BM) + std::min<int64_t>(p.K, p.R);
+  const int64_t tiles = m_tiles * cdiv(width, NT);
+  if (tiles > INT32_MAX / 2) return fail(FGMM_ERR_UNSUPPORTED, "more than 2^30 tiles");
+  FGMM_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(tiles, num_sms())), dim3(kThreads), Sh::smem(p.K), st, ma, mb, a, out));
+  return FGMM_OK;
+}
+
+// Columns of a tile: 256 where every SM gets two such tiles, else 128.
+template <int MODE, typename OUT>
+int launch16(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
+             cudaStream_t st) {
+  const int width = MODE == kForward ? d_out : d_in;
+  const int64_t m_tiles = MODE == kWeights ? (int64_t)p.K * cdiv(d_out, BM) : cdiv(p.R, BM);
+  if (width > 128 && m_tiles * cdiv(width, 256) >= 2 * num_sms()) return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, st);
+  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, st);
+}
+
+}  // namespace
+
+int experts_device_error(bool reset) { return read_dev_error(reset); }
+
+size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, bool backward) {
+  Carve c(nullptr);
+  c.take<uint16_t>(copy_elems(dtype, N, d_in));
+  c.take<uint16_t>(copy_elems(dtype, (int64_t)K * d_out, d_in));
+  if (backward) c.take<uint16_t>(copy_elems(dtype, N * top_k, d_out));
+  return c.bytes() + 256;
+}
+
+int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y,
+                void *ws, cudaStream_t st) {
+  Carve c(ws);
+  uint16_t *cx = c.take<uint16_t>(copy_elems(dtype, N, d_in)), *cw = c.take<uint16_t>(copy_elems(dtype, (int64_t)p.K * d_out, d_in));
+  Operand ox, ow;
+  int rc = operand(&ox, x, dtype, N, d_in, cx, st);
+  if (!rc) rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
+  if (rc) return rc;
+  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, st);
+  if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, st);
+  return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, st);
+}
+
+int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
+                         const RoutePlan &p, float *dx_rows, void *d_weight, void *ws, cudaStream_t st) {
+  Carve c(ws);
+  uint16_t *cx = c.take<uint16_t>(copy_elems(dtype, N, d_in)), *cw = c.take<uint16_t>(copy_elems(dtype, (int64_t)p.K * d_out, d_in));
+  uint16_t *cg = c.take<uint16_t>(copy_elems(dtype, p.R, d_out));
+  Operand og;
+  int rc = operand(&og, dy, dtype, p.R, d_out, cg, st);
+  if (rc) return rc;
+  if (dx_rows) {
+    Operand ow;
+    rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
+    if (!rc) rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, st)
+                                    : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, st);
+    if (rc) return rc;
+  }
+  if (!d_weight) return FGMM_OK;
+  Operand ox;
+  rc = operand(&ox, x, dtype, N, d_in, cx, st);
+  if (rc) return rc;
+  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, st);
+  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, st);
+  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, st);
+}
+
+}  // namespace fgmm

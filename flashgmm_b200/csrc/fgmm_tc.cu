@@ -1673,15 +1673,6 @@ int tc_update_prepare(const double *stats, double n_total, const void *points, i
                         param_ops(w, p, points), st);
 }
 
-int tc_device_error(bool reset) {
-  int v = 0;
-  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  if (cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(int)) != cudaSuccess) return -1;
-  if (reset && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_dev_error, &z, sizeof(int));
-  }
-  return v;
-}
+int tc_device_error(bool reset) { return read_dev_error(reset); }
 
 }  // namespace fgmm

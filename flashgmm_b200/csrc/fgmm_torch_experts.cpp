@@ -44,6 +44,12 @@ Tensor with_rows(const Tensor &t) {
 }
 int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
+// Contiguous and on a 16-byte boundary, as the products read their matrices.
+Tensor for_products(const Tensor &t) {
+  Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
 Tensor scratch(size_t bytes, const torch::Device &dev) {
   return torch::empty({(int64_t)std::max<size_t>(bytes, 256)}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
 }
@@ -165,7 +171,7 @@ Tensor expert_products(const Tensor &x, const Tensor &weight, const Tensor &orde
   check_shape(x, "x", {p.N, d_in});
   check_shape(weight, "weight", {p.K, d_out, d_in});
   TORCH_CHECK(d_in >= 1 && d_out >= 1, "x and weight must have at least one column");
-  const Tensor xc = x.contiguous(), wc = weight.contiguous();
+  const Tensor xc = for_products(x), wc = for_products(weight);
   Tensor y = torch::empty({p.R, d_out}, x.options());
   const int di = narrow(d_in, "d_in"), dn = narrow(d_out, "d_out");
   const size_t nb = fgmm_expert_products_workspace_bytes(dtype, p.N, p.K, di, dn, p.top_k);
@@ -194,7 +200,7 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>> expert_products_backwar
   check_shape(weight, "weight", {p.K, d_out, d_in});
   check_shape(dy, "dy", {p.R, d_out});
   TORCH_CHECK(d_in >= 1 && d_out >= 1, "x and weight must have at least one column");
-  const Tensor xc = x.contiguous(), wc = weight.contiguous(), gc = dy.contiguous();
+  const Tensor xc = for_products(x), wc = for_products(weight), gc = for_products(dy);
   c10::optional<Tensor> dx, dw;
   if (need_dx) dx = torch::empty({p.N, d_in}, x.options());
   if (need_dweight) dw = torch::empty({p.K, d_out, d_in}, x.options());

@@ -12,9 +12,21 @@
 namespace fgmm {
 namespace ptx {
 
-// Device-wide error word: 0 = fine; otherwise the code of the first failure.
-// (This header is included by exactly one translation unit, fgmm_tc.cu.)
-__device__ int g_dev_error = 0;
+// Error word of the including translation unit on each device: 0 = fine; otherwise the code of the first
+// failure.  fgmm_device_error reads those of all units.
+static __device__ int g_dev_error = 0;
+
+// Host side of the word: synchronises the device; -1 on a CUDA error.
+static inline int read_dev_error(bool reset) {
+  int v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+  if (cudaMemcpyFromSymbol(&v, g_dev_error, sizeof(int)) != cudaSuccess) return -1;
+  if (reset && v) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_dev_error, &z, sizeof(int));
+  }
+  return v;
+}
 
 constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s
 
@@ -144,6 +156,17 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
+// Four rows of a 2-D tensor (map box one row high), any rows in any order, into consecutive 128-byte rows
+// of a tile; rows outside the tensor are zeros.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t r0, int32_t r1,
+                                            int32_t r2, int32_t r3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+      : "memory");
+}
+
 // L2 eviction policies for the cache-hinted loads and stores below.
 __device__ __forceinline__ uint64_t policy_evict_first() {
   uint64_t p;
@@ -230,7 +253,7 @@ __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
-// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f16 (A and B both fp16), fp32 accumulate.
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f16 (A and B of one 16-bit type), fp32 accumulate.
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                         uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -363,11 +386,11 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t lbo, ui
   return sdesc(saddr, lbo, sbo, kSw128);
 }
 
-// Instruction descriptor, kind::f16 with fp16 A and B and fp32 accumulate.
-__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn, int b_mn) {
+// Instruction descriptor, kind::f16 with A and B both fp16 (or both bf16) and fp32 accumulate.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn, int b_mn, int bf16 = 0) {
   return (1u << 4)                          // D format f32
-         | (0u << 7)                        // A format f16
-         | (0u << 10)                       // B format f16
+         | ((uint32_t)bf16 << 7)            // A format: f16 0, bf16 1
+         | ((uint32_t)bf16 << 10)           // B format
          | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }

@@ -133,7 +133,8 @@ def expert_products(x, weight, routes):
     """``y[r] = weight[e] @ x[n]`` for every grouped row r of ``routes`` (point n, expert e) ->
     ``y[N top_k, d_out]``; rows behind ``offsets[K]`` (routes without an expert) are 0.
 
-    ``x[N, d_in]`` and ``weight[K, d_out, d_in]`` of one type; gradients to both."""
+    ``x[N, d_in]`` and ``weight[K, d_out, d_in]`` of one type; gradients to both.  float32 operands run
+    on the tensor cores as three bf16 planes (24 bits together); an infinite entry gives NaN there."""
     _check_tensors(x=x, weight=weight)
     _check_routes(routes)
     if _records(x, weight):
@@ -143,7 +144,7 @@ def expert_products(x, weight, routes):
 
 def expert_products_backward(dy, x, weight, routes, need_dx=True, need_dweight=True):
     """``[dx, dweight]`` from ``dy[N top_k, d_out]`` (``None`` where not needed): dx sums a point's
-    rows in slot order, each row rounded to the inputs' type before; dweight sums an expert's rows."""
+    rows in slot order, dweight an expert's rows; both round once."""
     _check_tensors(dy=dy, x=x, weight=weight)
     _check_routes(routes)
     return list(_ext.load().expert_products_backward(dy, x, weight, *routes, need_dx, need_dweight))

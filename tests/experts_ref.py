@@ -89,7 +89,7 @@ def products(x, weight, order, offsets, top_k, dy=None):
     """y, and with dy also dx and dweight; float64 results and the sums of the products' magnitudes."""
     x, weight = x.double(), weight.double()
     R, (K, d_out, d_in) = order.numel(), weight.shape
-    y, ya = torch.zeros(R, d_out).double(), torch.zeros(R, d_out).double()
+    y, ya = (torch.zeros(R, d_out, dtype=torch.float64, device=x.device) for _ in range(2))
     dx, dxa = torch.zeros_like(x), torch.zeros_like(x)
     dw, dwa = torch.zeros_like(weight), torch.zeros_like(weight)
     off = offsets.tolist()

@@ -593,3 +593,19 @@ def test_models_route_by_their_responsibilities(model):
     assert float((out.detach().double() - exact).abs().max()) <= 1e-5 * float(exact.abs().max())
     out.sum().backward()
     assert weight.grad.shape == weight.shape and torch.isfinite(weight.grad).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_products_of_many_rows(dtype):
+    """Enough rows and columns for the widest tiles in each direction (results in 64 bits on the GPU)."""
+    N, k, K, d_in, d_out = 3000, 4, 8, 1032, 1040
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, w = torch.randn(N, d_in, generator=g, device=DEV).to(dtype), (torch.randn(K, d_out, d_in, generator=g, device=DEV) / 32).to(dtype)
+    dy = torch.randn(N * k, d_out, generator=g, device=DEV).to(dtype)
+    routes = C().group_routes(plan(N, k, K, 2).to(DEV), K)
+    y, ya, dx, dxa, dw, dwa = ref.products(x, w, routes.order, routes.offsets, k, dy)
+    close(C().expert_products(x, w, routes), y.cpu(), ya.cpu(), d_in, dtype, "y")
+    gx, gw = C().expert_products_backward(dy, x, w, routes)
+    close(gx, dx.cpu(), dxa.cpu(), d_out + k, dtype, "dx")
+    counts = routes.offsets[1:] - routes.offsets[:-1]
+    close(gw, dw.cpu(), dwa.cpu(), int(counts.max()), dtype, "dw")
