@@ -4,14 +4,16 @@
 //   rows x weight^T  DX[r, i]    = sum_o DY[r, o] W[e(r), o, i]
 //   sums over rows   DW[e, o, i] = sum_{r of e} DY[r, o] X[point(r), i]
 //
-// One persistent, warp-specialised kernel: a producer warp fills a ring of stages by TMA, one thread issues
-// tcgen05.mma into a double-buffered tensor-memory accumulator, four warps read it back and write the
-// results, and the next tile's products run meanwhile.  A tile has M = 128 rows of one expert (or, for
+// One persistent, warp-specialised kernel: a TMA warp and four gathering warps fill a ring of stages, one thread
+// issues tcgen05.mma into a double-buffered tensor-memory accumulator, eight warps read it back and write
+// the results, and the next tile's products run meanwhile.  A tile has M = 128 rows of one expert (or, for
 // DW, 128 of its output dimensions) and NT columns; a stage holds 64 elements of the contraction.
-//   * A point's row of X is fetched by TMA gather4 straight from the points' matrix, four rows an
-//     instruction, so the grouped copy of X is never written.  Rows a tile does not have are not
-//     loaded: their accumulator rows hold leftovers that nobody reads.  Where the rows are the contraction (DW)
-//     they are fetched as rows outside the tensor, which are zeros in both operands.
+//   * The points' rows of X are gathered straight from the points' matrix by 16-byte cp.async, in the
+//     swizzled layout that TMA writes, so a grouped copy of X is never made.  (TMA gather4 measured 80
+//     cycles for four 128-byte rows, a third of what the products consume: 326 us against 39 us of the same
+//     products with contiguous rows at 8,186 rows, 1,000 x 1,016.)  Rows a tile does not have are not loaded: their
+//     accumulator rows hold leftovers that nobody reads.  Where the rows are the contraction (DW), those behind
+//     the expert's last one are zeros in both operands.
 //   * W is fetched as a box of its 3-D tensor, K-major for Y, and MN-major, without a transposed copy, for DX.
 //   * float32 operands are three bf16 planes (x = b0 + b1 + b2, 24 bits together), laid out by
 //     split_planes_kernel, and the six products that matter (b0 b0 into one accumulator; b0 b1, b1 b0, b1 b1,
@@ -33,8 +35,17 @@ namespace {
 
 constexpr int BM = 128;       // tile rows (MMA M)
 constexpr int KCH = 64;       // contraction elements of a stage (128-byte rows)
-constexpr int kThreads = 256;  // warp 0 producer, warp 1 MMA, warps 2-3 rows of no expert, warps 4-7 epilogue
+constexpr int kGather = 128;   // gathering threads: warps 2-5
+constexpr int kEpiWarps = 8;   // warps 6-13: two per tensor-memory lane quarter, half of the columns each
+constexpr int kThreads = 64 + kGather + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA
 constexpr int kSegment = 4;   // stages between drains of a float32 product (256 elements)
+
+// A load that stays where it is written (a plan's entry fetched a stage ahead of its use).
+__device__ __forceinline__ int ld_now(const int32_t *p) {
+  int v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
 
 enum { kForward = 0, kInputs = 1, kWeights = 2 };
 
@@ -44,8 +55,8 @@ struct Shape {
   static constexpr int kA = BM * KCH * 2, kB = NT * KCH * 2;  // bytes of one plane's tile
   static constexpr int kStage = kPlanes * (kA + kB);
   static constexpr int kStages = (192 * 1024) / kStage;
-  static constexpr int kOut = 4 * 32 * 128;  // a 32-row, 128-byte staging tile for each epilogue warp
-  static constexpr int kBars = 256;
+  static constexpr int kOut = kEpiWarps * 16 * 128;  // a 16-row, 128-byte staging tile for each epilogue warp
+  static constexpr int kBars = 320;
   static constexpr int smem(int K) { return 1024 + kStages * kStage + kOut + kBars + (K + 1) * 4; }
   static_assert(kStages >= 2, "shared-memory budget");
   static_assert(smem(kMaxExperts) <= 227 * 1024, "shared-memory budget");
@@ -56,7 +67,10 @@ struct TcArgs {
   int64_t N;
   int d_in, d_out;
   int a_plane, b_plane;  // columns between the planes of A's and B's rows (float32)
+  const uint16_t *a_rows, *b_rows;  // the same matrices for the gathering warps
+  int a_cols, b_cols;               // columns of their rows in memory
   uint32_t idesc;
+  uint32_t div_mul, div_shift;  // n / top_k = n * div_mul >> div_shift for n < 2^31
   int vec;  // rows of the result start on 16-byte boundaries
 };
 
@@ -127,8 +141,8 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *s_out = smem + S * Sh::kStage;
   uint64_t *bars = reinterpret_cast<uint64_t *>(s_out + Sh::kOut);
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_out + Sh::kOut + Sh::kBars - 64);
-  int *s_warp = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars - 48);  // [8]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_out + Sh::kOut + Sh::kBars - 96);
+  int *s_warp = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars - 80);  // [warps]
   int *s_tile = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars);        // [K + 1]
   const uint32_t bar0 = smem_u32(bars);
   auto FULL = [&](int s) { return bar0 + 8u * s; };
@@ -136,17 +150,18 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   auto TFULL = [&](int b) { return bar0 + 8u * (2 * S + b); };
   auto TEMPTY = [&](int b) { return bar0 + 8u * (2 * S + 2 + b); };
   const uint32_t DONE = bar0 + 8u * (2 * S + 4);
-  static_assert(8 * (2 * S + 5) <= Sh::kBars - 64, "barrier space");
+  static_assert(8 * (2 * S + 5) <= Sh::kBars - 96, "barrier space");
+  static_assert(kThreads / 32 * 4 <= 80, "barrier space");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int R = (int)a.plan.R, K = a.plan.K;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) { mbar_init(FULL(i), 1); mbar_init(EMPTY(i), 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(TFULL(b), 1); mbar_init(TEMPTY(b), 4); }
+    for (int i = 0; i < S; ++i) { mbar_init(FULL(i), MODE == kInputs ? 1 : 1 + kGather); mbar_init(EMPTY(i), 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(TFULL(b), 1); mbar_init(TEMPTY(b), kEpiWarps); }
     mbar_init(DONE, 1);
     fence_mbar_init();
-    prefetch_tmap(&tm_a);
-    prefetch_tmap(&tm_b);
+    if (MODE != kForward) prefetch_tmap(&tm_a);
+    if (MODE != kWeights) prefetch_tmap(&tm_b);
   }
   if (warp == 0) {
     tmem_alloc(smem_u32(tmem_slot), kCols);
@@ -188,76 +203,36 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   Tiles<MODE, NT> tiles(a, s_tile);
 
   if (warp == 0) {
-    // ---------------------------------------------------------------- producer
+    // ---------------------------------------------------------------- TMA
     int stage = 0;
     uint32_t phase = 0;
     int filled = 0;  // stages ever armed, up to S
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x) {
+    for (int t = blockIdx.x; t < tiles.total && ok && lane == 0; t += gridDim.x) {
       const Tile x = tiles.at(t);
-      int src[4];  // Y: the points of this lane's four rows
-      if (MODE == kForward) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = lane * 4 + i;
-          const int p = r < x.rows ? row_point(a.plan.order, x.r0 + r, R, a.plan.top_k) : -1;
-          src[i] = p >= 0 ? p : (int)a.N;  // a row outside the tensor: zeros
-        }
-      }
       for (int c = 0; c < x.nk; ++c) {
-        ok = __shfl_sync(0xffffffffu, lane == 0 ? (int)mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty) : 0, 0);
-        if (!ok) break;
+        if (!mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty)) { ok = false; break; }
         const uint32_t base = smem_u32(smem + stage * Sh::kStage), base_b = base + P * Sh::kA;
-        if (MODE == kForward) {
-          const int quads = (x.rows + 3) / 4;
-          if (lane == 0) mbar_arrive_expect_tx(FULL(stage), P * (quads * 512 + Sh::kB));
-          __syncwarp();
+        if (MODE == kWeights && x.r0 + (c + 1) * KCH > x.r1) {
+          mbar_arrive(FULL(stage));  // the gathering warps fetch the last rows of both operands
+        } else {
+          mbar_arrive_expect_tx(FULL(stage), P * ((MODE != kForward ? Sh::kA : 0) + (MODE != kWeights ? Sh::kB : 0)));
 #pragma unroll
           for (int p = 0; p < P; ++p) {
-            if (lane < quads)
-              tma_gather4(base + p * Sh::kA + lane * 512, &tm_a, p * a.a_plane + c * KCH, src[0], src[1], src[2], src[3], FULL(stage));
-            if (lane == 0) tma_load_3d(base_b + p * Sh::kB, &tm_b, p * a.b_plane + c * KCH, x.n0, x.e, FULL(stage));
-          }
-        } else if (MODE == kInputs) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(FULL(stage), Sh::kStage);
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
+            if (MODE == kForward) {
+              tma_load_3d(base_b + p * Sh::kB, &tm_b, p * a.b_plane + c * KCH, x.n0, x.e, FULL(stage));
+            } else if (MODE == kInputs) {
               tma_load_2d(base + p * Sh::kA, &tm_a, p * a.a_plane + c * KCH, x.r0, FULL(stage));
 #pragma unroll
               for (int j = 0; j < NT / 64; ++j)
                 tma_load_3d(base_b + p * Sh::kB + j * 64 * 128, &tm_b, p * a.b_plane + x.n0 + j * 64, c * KCH, x.e, FULL(stage));
-            }
-          }
-        } else {
-          // 64 rows of the contraction: lanes 0-15 fetch four each of DY, lanes 16-31 of X
-          const int q = lane & 15, r = x.r0 + c * KCH + q * 4;
-          int row[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (lane < 16) {
-              row[i] = r + i < x.r1 ? r + i : R;
             } else {
-              const int p = r + i < x.r1 ? row_point(a.plan.order, r + i, R, a.plan.top_k) : -1;
-              row[i] = p >= 0 ? p : (int)a.N;
-            }
-          }
-          if (lane == 0) mbar_arrive_expect_tx(FULL(stage), Sh::kStage);
-          __syncwarp();
-#pragma unroll
-          for (int p = 0; p < P; ++p) {
-            if (lane < 16) {
 #pragma unroll
               for (int j = 0; j < BM / 64; ++j)
-                tma_gather4(base + p * Sh::kA + j * 64 * 128 + q * 512, &tm_a, p * a.a_plane + x.m0 + j * 64, row[0], row[1], row[2], row[3], FULL(stage));
-            } else {
-#pragma unroll
-              for (int j = 0; j < NT / 64; ++j)
-                tma_gather4(base_b + p * Sh::kB + j * 64 * 128 + q * 512, &tm_b, p * a.b_plane + x.n0 + j * 64, row[0], row[1], row[2], row[3], FULL(stage));
+                tma_load_2d(base + p * Sh::kA + j * 64 * 128, &tm_a, p * a.a_plane + x.m0 + j * 64, x.r0 + c * KCH, FULL(stage));
             }
           }
         }
-        __syncwarp();
         filled = min(S, filled + 1);
         if (++stage == S) { stage = 0; phase ^= 1; }
       }
@@ -296,6 +271,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           const int first = c, end = SPLIT ? min(nk, c + kSegment) : nk;
           for (; c < end; ++c) {
             if (!mbar_wait(FULL(stage), phase, kErrWaitFull)) { ok = false; break; }
+            if (MODE != kInputs) fence_proxy_async_smem();  // the gathered rows were written through the generic proxy
             tc_fence_after();
             const uint64_t ad = a0 + (uint64_t)((stage * Sh::kStage) >> 4), bd = b0 + (uint64_t)((stage * Sh::kStage) >> 4);
 #pragma unroll
@@ -322,52 +298,150 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       mbar_wait_drain(DONE, 0);
     }
     __syncwarp();
-  } else if (warp < 4) {
-    // ---------------------------------------------------------------- rows of no expert
-    if (MODE == kForward) {
+  } else if (warp < 2 + kGather / 32) {
+    // ---------------------------------------------------------------- gathered rows
+    if (MODE != kInputs) {
+      // Eight threads share a 128-byte row of a tile, thread j its 16 bytes, stored at chunk j ^ (row % 8); a thread
+      // takes the rows rr, rr + 16, ...  Its arrival on a stage follows by itself when its copies are complete.
+      constexpr int kStep = kGather / 8, kRows = (MODE == kForward ? BM : KCH) / kStep;
+      const int j = lane & 7, rr = (threadIdx.x - 64) >> 3;
+      const uint32_t at = rr * 128 + ((j ^ (rr & 7)) << 4);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x) {
+        const Tile x = tiles.at(t);
+        int id[kRows];  // routes of this thread's rows, -1: none
+        auto routes = [&](int r0, int r1) {
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) id[i] = r0 + rr + kStep * i < r1 ? ld_now(a.plan.order + r0 + rr + kStep * i) : -1;
+        };
+        auto point = [&](int i) { return (int)(((uint64_t)(uint32_t)id[i] * a.div_mul) >> a.div_shift); };
+        routes(x.r0, MODE == kForward ? x.r0 + x.rows : x.r1);
+        if (MODE == kForward) {
+          const uint16_t *src[kRows];
+          uint32_t live = 0;
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const bool in = id[i] >= 0 && id[i] < R;
+            src[i] = a.a_rows + (in ? (int64_t)point(i) * a.a_cols + j * 8 : 0);
+            live |= (uint32_t)in << i;
+          }
+          for (int c = 0; c < x.nk; ++c) {
+            ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty));
+            if (!ok) break;
+            const uint32_t base = smem_u32(smem + stage * Sh::kStage) + at;
+            const uint32_t now = c * KCH + j * 8 < a.a_plane ? live : 0;  // columns behind the last are zeros
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+              for (int i = 0; i < kRows; ++i) {
+                if (kStep * i >= x.rows) break;
+                cp_async16(base + p * Sh::kA + i * kStep * 128, ((now >> i) & 1) ? src[i] + p * a.a_plane + c * KCH : a.a_rows, ((now >> i) & 1) * 16);
+              }
+            cp_async_arrive(FULL(stage));
+            if (++stage == S) { stage = 0; phase ^= 1; }
+          }
+        } else {
+          // columns of B that exist, a bit per 64-column atom
+          uint32_t cols = 0;
+#pragma unroll
+          for (int n = 0; n < NT / 64; ++n) cols |= (uint32_t)(x.n0 + n * 64 + j * 8 < a.b_plane) << n;
+          for (int c = 0; c < x.nk; ++c) {
+            const uint16_t *src[kRows];
+            uint32_t live = 0;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+              const bool in = id[i] >= 0 && id[i] < R;
+              src[i] = a.b_rows + (in ? (int64_t)point(i) * a.b_cols + x.n0 + j * 8 : 0);
+              live |= (uint32_t)in << i;
+            }
+            const int r = x.r0 + c * KCH;
+            if (c + 1 < x.nk) routes(r + KCH, x.r1);
+            ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty));
+            if (!ok) break;
+            const uint32_t base = smem_u32(smem + stage * Sh::kStage) + at;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+              for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                for (int n = 0; n < NT / 64; ++n) {
+                  const uint32_t on = (live >> i) & (cols >> n) & 1;
+                  cp_async16(base + P * Sh::kA + p * Sh::kB + n * KCH * 128 + i * kStep * 128, on ? src[i] + p * a.b_plane + n * 64 : a.b_rows, on * 16);
+                }
+            if (r + KCH > x.r1) {  // the last rows of A too
+#pragma unroll
+              for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                  for (int m = 0; m < BM / 64; ++m) {
+                    const int row = r + rr + kStep * i, col = x.m0 + m * 64 + j * 8;
+                    const bool on = row < x.r1 && col < a.a_plane;
+                    cp_async16(base + p * Sh::kA + m * KCH * 128 + i * kStep * 128,
+                               on ? a.a_rows + (int64_t)row * a.a_cols + p * a.a_plane + col : a.a_rows, on ? 16 : 0);
+                  }
+            }
+            cp_async_arrive(FULL(stage));
+            if (++stage == S) { stage = 0; phase ^= 1; }
+          }
+        }
+      }
+      cp_async_wait_all();
+    }
+    if (MODE == kForward) {  // rows of no expert
       const int64_t first = (int64_t)min(max(__ldg(a.plan.offsets + K), 0), R) * a.d_out, end = (int64_t)R * a.d_out;
-      for (int64_t i = first + blockIdx.x * 64 + threadIdx.x - 64; i < end; i += (int64_t)gridDim.x * 64) out[i] = from_f32<OUT>(0.0f);
+      for (int64_t i = first + blockIdx.x * kGather + threadIdx.x - 64; i < end; i += (int64_t)gridDim.x * kGather) out[i] = from_f32<OUT>(0.0f);
     }
   } else {
     // ---------------------------------------------------------------- epilogue
     constexpr int CW = 128 / sizeof(OUT), EPV = 16 / sizeof(OUT);  // columns of a staging row, of 16 bytes
-    constexpr int W = SPLIT ? NT : CW;                             // columns held in registers
-    const int q = warp & 3;
-    const uint32_t lane_tmem = tmem + ((uint32_t)(q * 32) << 16);
-    uint8_t *stg = s_out + q * 32 * 128;
+    constexpr int HC = NT / 2;                                     // columns of this warp
+    constexpr int W = SPLIT ? HC : CW;                             // columns held in registers
+    static_assert(HC % CW == 0, "whole staging rows");
+    const int q = warp & 3, half = (warp - 2 - kGather / 32) / 4 * HC;
+    const uint32_t lane_tmem = tmem + ((uint32_t)(q * 32) << 16) + half;
+    uint8_t *stg = s_out + (warp - 2 - kGather / 32) * 16 * 128;
     const int width = MODE == kForward ? a.d_out : a.d_in;
     int seg = 0, count = 0;
     bool ok = true;
-    // 32 rows x CW columns (from column c0 of the tile) through shared memory, so that the global writes are whole lines
+    // 32 rows x CW columns (from column c0 of the tile) through shared memory, 16 rows at a time, so that the global
+    // writes are whole lines
     auto write = [&](const float *v, const Tile &x, int c0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<uint4 *>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack16<OUT>(v + j * EPV);
-      __syncwarp();
       const int64_t row0 = MODE == kWeights ? (int64_t)x.e * a.d_out + x.m0 : x.r0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3), j = lane & 7;
-        const int col = x.n0 + c0 + j * EPV;
-        if (q * 32 + r < x.rows && col < width) {
-          const uint4 u = *reinterpret_cast<const uint4 *>(stg + r * 128 + ((j ^ (r & 7)) << 4));
-          OUT *p = out + (row0 + q * 32 + r) * width + col;
-          if (a.vec) {  // then the width is a multiple of EPV
-            *reinterpret_cast<uint4 *>(p) = u;
-          } else {
-            OUT h[EPV];
-            *reinterpret_cast<uint4 *>(h) = u;
+      for (int h = 0; h < 2; ++h) {
+        if ((lane >> 4) == h) {
 #pragma unroll
-            for (int k = 0; k < EPV; ++k)
-              if (col + k < width) p[k] = h[k];
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4 *>(stg + (lane & 15) * 128 + ((j ^ (lane & 7)) << 4)) = pack16<OUT>(v + j * EPV);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 4 + (lane >> 3), j = lane & 7;
+          const int col = x.n0 + c0 + j * EPV, row = q * 32 + h * 16 + r;
+          if (row < x.rows && col < width) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(stg + r * 128 + ((j ^ (r & 7)) << 4));
+            OUT *p = out + (row0 + row) * width + col;
+            if (a.vec) {  // then the width is a multiple of EPV
+              *reinterpret_cast<uint4 *>(p) = u;
+            } else {
+              OUT e[EPV];
+              *reinterpret_cast<uint4 *>(e) = u;
+#pragma unroll
+              for (int k = 0; k < EPV; ++k)
+                if (col + k < width) p[k] = e[k];
+            }
           }
         }
+        __syncwarp();
       }
-      __syncwarp();
     };
     for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, ++count) {
       const Tile x = tiles.at(t);
-      const bool live = q * 32 < x.rows;
+      const bool live = q * 32 < x.rows && x.n0 + half < width;
       float acc[W];
       if constexpr (SPLIT) {
 #pragma unroll
@@ -382,49 +456,40 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         c = SPLIT ? c + kSegment : x.nk;
         if constexpr (SPLIT) {
           if (live && x.nk > 0) {
+            auto add = [&](uint32_t from) {
 #pragma unroll
-            for (int i = 0; i < NT / 32; ++i) {
-              float v[32];
-              tmem_ld32(lane_tmem + buf * NT + i * 32, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) acc[i * 32 + k] += v[k];
-            }
-            if (c >= x.nk) {
-#pragma unroll
-              for (int i = 0; i < NT / 32; ++i) {
+              for (int i = 0; i < HC / 32; ++i) {
                 float v[32];
-                tmem_ld32(lane_tmem + (2 + (count & 1)) * NT + i * 32, v);
+                tmem_ld32(from + i * 32, v);
                 tmem_wait_ld();
 #pragma unroll
                 for (int k = 0; k < 32; ++k) acc[i * 32 + k] += v[k];
               }
-            }
+            };
+            add(lane_tmem + buf * NT);
+            if (c >= x.nk) add(lane_tmem + (2 + (count & 1)) * NT);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(TEMPTY(buf));
+        } else if (live) {
+          for (int i = 0; i < HC / CW; ++i) {
+            if (x.n0 + half + i * CW >= width) break;
+#pragma unroll
+            for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
+            tmem_wait_ld();
+            if (x.nk == 0) {  // an expert without a row
+#pragma unroll
+              for (int k = 0; k < CW; ++k) acc[k] = 0.0f;
+            }
+            write(acc, x, half + i * CW);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(TEMPTY(buf));
+        if constexpr (SPLIT) {
           if (c >= x.nk && live) {
 #pragma unroll
-            for (int i = 0; i < NT / CW; ++i) write(acc + i * CW, x, i * CW);
+            for (int i = 0; i < HC / CW; ++i) write(acc + i * CW, x, half + i * CW);
           }
-        } else {
-          if (live) {
-            for (int i = 0; i < NT / CW; ++i) {
-              if (x.n0 + i * CW >= width) break;
-#pragma unroll
-              for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
-              tmem_wait_ld();
-              if (x.nk == 0) {  // an expert without a row
-#pragma unroll
-                for (int k = 0; k < CW; ++k) acc[k] = 0.0f;
-              }
-              write(acc, x, i * CW);
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(TEMPTY(buf));
         }
         ++seg;
       } while (c < x.nk);
@@ -547,9 +612,10 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
            cudaStream_t st) {
   using Sh = Shape<NT, SPLIT>;
   const int bf16 = dtype != FGMM_F16, width = MODE == kForward ? d_out : d_in;
-  CUtensorMap ma, mb;
-  int rc = make_map(&ma, oa, bf16, MODE == kInputs ? BM : 1, 0);
-  if (!rc) rc = MODE == kWeights ? make_map(&mb, ob, bf16, 1, 0) : make_map(&mb, ob, bf16, MODE == kForward ? NT : KCH, p.K);
+  CUtensorMap ma{}, mb{};
+  int rc = FGMM_OK;
+  if (MODE != kForward) rc = make_map(&ma, oa, bf16, MODE == kInputs ? BM : KCH, 0);
+  if (!rc && MODE != kWeights) rc = make_map(&mb, ob, bf16, MODE == kForward ? NT : KCH, p.K);
   if (rc) return rc;
   TcArgs a{};
   a.plan = p;
@@ -558,6 +624,14 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   a.d_out = d_out;
   a.a_plane = oa.plane;
   a.b_plane = ob.plane;
+  a.a_rows = static_cast<const uint16_t *>(oa.p);
+  a.b_rows = static_cast<const uint16_t *>(ob.p);
+  a.a_cols = oa.cols;
+  a.b_cols = ob.cols;
+  // exact for n < 2^31: with 2^(l - 1) < top_k <= 2^l the multiplier exceeds 2^(31 + l) / top_k by less than 1
+  a.div_shift = 31;
+  while ((1u << (a.div_shift - 31)) < (uint32_t)p.top_k) ++a.div_shift;
+  a.div_mul = (uint32_t)((((uint64_t)1 << a.div_shift) + p.top_k - 1) / p.top_k);
   a.idesc = idesc_f16(BM, NT, MODE == kWeights, MODE != kForward, bf16);
   a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
