@@ -1,4 +1,4 @@
-// Shared by the expert operators (fgmm_experts.cu, fgmm_experts_simt.cu, fgmm_experts_tc.cu):
+// Shared by the expert operators (fgmm_experts.cu, fgmm_experts_route.cu, fgmm_experts_tc.cu):
 // element types, the grouped rows' plan, and the launchers behind the C ABI.
 #pragma once
 #include <cuda_bf16.h>
@@ -44,13 +44,15 @@ __device__ __forceinline__ int row_point(const int32_t *order, int r, int R, int
   return id >= 0 && id < R ? id / top_k : -1;
 }
 
-// ---- fgmm_experts.cu ----
+// ---- fgmm_experts_route.cu ----
 int route_forward(const void *scores, int dtype, int64_t N, int K, int64_t stride, const float *bias,
                   int top_k, int func, int n_groups, int top_groups, bool renorm, float scale,
                   float *weights, int32_t *indices, cudaStream_t st);
 int route_backward(const float *dw, const void *scores, int dtype, int64_t N, int K, int64_t stride,
                    const int32_t *indices, int top_k, int func, bool renorm, float scale, void *dz,
                    cudaStream_t st);
+
+// ---- fgmm_experts.cu ----
 size_t group_workspace_bytes(int64_t R, int K);
 int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32_t *offsets,
                  int32_t *position, void *ws, cudaStream_t st);

@@ -391,8 +391,12 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       cp_async_wait_all();
     }
     if (MODE == kForward) {  // rows of no expert
-      const int64_t first = (int64_t)min(max(__ldg(a.plan.offsets + K), 0), R) * a.d_out, end = (int64_t)R * a.d_out;
-      for (int64_t i = first + blockIdx.x * kGather + threadIdx.x - 64; i < end; i += (int64_t)gridDim.x * kGather) out[i] = from_f32<OUT>(0.0f);
+      const int64_t none = min(max(__ldg(a.plan.offsets + K), 0), R), first = none * a.d_out, end = (int64_t)R * a.d_out;
+      const int step = a.vec ? 16 / sizeof(OUT) : 1;
+      for (int64_t i = first + (int64_t)(blockIdx.x * kGather + threadIdx.x - 64) * step; i < end; i += (int64_t)gridDim.x * kGather * step) {
+        if (a.vec) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
+        else out[i] = from_f32<OUT>(0.0f);
+      }
     }
   } else {
     // ---------------------------------------------------------------- epilogue
