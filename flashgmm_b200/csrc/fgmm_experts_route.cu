@@ -1,0 +1,703 @@
+// Routing to experts: the choice of every point's experts, their weights, and the scores' gradient.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "fgmm_experts.cuh"
+
+namespace fgmm {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ------------------------------------------------------------------------------ routing
+//
+// s = softmax(z), sigmoid(z) or z; c = s + bias; the top_groups groups with the largest sums of
+// their two best c stay; the top_k experts by c, ties to the lowest index; w = s, divided by the
+// chosen ones' sum where asked, times the scale.  Without bias and groups the order of c is that of z,
+// and z itself is compared.  A score of -inf or NaN is masked; +inf counts as the largest finite value.
+//
+// A row is held in registers by 8, 16 or 32 lanes.  c is fp32; the order is defined on 64-bit values, so a row where
+// two deciding values lie closer than the fp32 error allows (and are not the same score and bias) is decided
+// again in fp64, from its scores, by route_row64.
+
+// Unsigned order of floats; 0 is below every float.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // -0 and 0 are equal
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+
+// A score as it counts: masked ones as -inf.
+__device__ __forceinline__ float clean(float z) { return fminf(fmaxf(z, -INFINITY), FLT_MAX); }  // fmaxf drops a NaN
+
+struct RouteArgs {
+  int64_t N, stride;
+  int K, top_k, func, n_groups, top_groups;
+  const float *bias;
+  bool renorm;
+  float scale;
+};
+
+template <typename T> __device__ __forceinline__ float score_at(const T *row, int c) { return clean(to_f32(row[c])); }
+
+// (v, i) comes before (w, j): a larger value, or an equal one of a lower index.
+__device__ __forceinline__ bool before(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
+
+// Decides one row in 64 bits, the whole warp on it: a lane holds the values of columns lane, lane + 32, ...
+// Lane j returns slot j's expert.  Rare; its values are kept in local memory (indexed at run time), because
+// registers for them would halve the occupancy of the rows that do not come here.
+template <typename T, int COLS>
+__device__ __noinline__ int route_row64(const T *row, const RouteArgs &a) {
+  const int lane = threadIdx.x & 31, per = a.K / a.n_groups, n = (a.K - lane + 31) / 32;
+  double v[COLS];
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) v[i] = (double)score_at(row, lane + 32 * i);
+  double m = -INFINITY, total = 0.0;
+  if (a.func == FGMM_SCORE_SOFTMAX) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) m = fmax(m, v[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(kFull, m, o));
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) v[i] = v[i] > -INFINITY ? exp(v[i] - m) : -INFINITY;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) total += fmax(v[i], 0.0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
+  }
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    double s = v[i];
+    if (s > -INFINITY) {
+      if (a.func == FGMM_SCORE_SOFTMAX) s /= total;
+      else if (a.func == FGMM_SCORE_SIGMOID) s = 1.0 / (1.0 + exp(-s));
+      if (a.bias) s += (double)__ldg(a.bias + lane + 32 * i);
+      v[i] = fmax(s, -INFINITY);  // -inf for NaN
+    }
+  }
+  if (a.n_groups > 1) {
+    double mine = -INFINITY;  // lane g: group g's sum
+    for (int g = 0; g < a.n_groups; ++g) {
+      double b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int c = lane + 32 * i;
+        const double x = c >= g * per && c < (g + 1) * per ? v[i] : -INFINITY;
+        b2 = fmax(b2, fmin(b1, x));
+        b1 = fmax(b1, x);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const double o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+        b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+        b1 = fmax(b1, o1);
+      }
+      if (lane == g) mine = b2 > -INFINITY ? b1 + b2 : b1;
+    }
+    int rank = 0;
+    for (int g = 0; g < a.n_groups; ++g) {
+      const double x = __shfl_sync(kFull, mine, g);
+      if (before(x, g, mine, lane)) ++rank;
+    }
+    const unsigned kept = __ballot_sync(kFull, lane < a.n_groups && rank < a.top_groups);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i)
+      if (!((kept >> ((lane + 32 * i) / per & 31)) & 1u)) v[i] = -INFINITY;
+  }
+  int chosen = -1;
+  for (int j = 0; j < a.top_k; ++j) {
+    double bv = -INFINITY;
+    int bi = a.K;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i)
+      if (v[i] > bv) { bv = v[i]; bi = lane + 32 * i; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const double ov = __shfl_xor_sync(kFull, bv, o);
+      const int oi = __shfl_xor_sync(kFull, bi, o);
+      if (before(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+    }
+    if (bi >= a.K) break;
+    if (lane == j) chosen = bi;
+    if (lane == (bi & 31)) v[bi >> 5] = -INFINITY;
+  }
+  return chosen;
+}
+
+// A row belongs to L neighbouring lanes (32 / L rows a warp); reductions over them, in all of them.
+template <int L> __device__ __forceinline__ float seg_max(float v) {
+  if constexpr (L == 32) return of_key(__reduce_max_sync(kFull, key_of(v)));
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <int L> __device__ __forceinline__ float seg_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+template <int L> __device__ __forceinline__ uint32_t seg_min(uint32_t v) {
+  if constexpr (L == 32) return __reduce_min_sync(kFull, v);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = min(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <int L> __device__ __forceinline__ unsigned seg_ballot(bool p) {
+  const unsigned b = __ballot_sync(kFull, p);
+  if constexpr (L == 32) return b;
+  return b >> ((threadIdx.x & 31) / L * L) & ((1u << L) - 1u);
+}
+template <int L, typename X> __device__ __forceinline__ X seg_get(X v, int from) { return __shfl_sync(kFull, v, from, L); }
+
+// One row as it is in memory: value i of lane l of the row is this column, masked past K.
+template <int V, int L> __device__ __forceinline__ int column(int i, int l) { return (i / V * L + l) * V + i % V; }
+template <typename T, int VPT> struct alignas(16) Row {
+  T v[VPT];
+};
+template <typename T, int VPT, int V, int L>
+__device__ __forceinline__ void load_row(const T *row, int K, int l, Row<T, VPT> &r) {
+#pragma unroll
+  for (int i = 0; i < VPT; i += V) {
+    const int c = column<V, L>(i, l);
+    if (V > 1 && c + V <= K) {
+      if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4 *>(r.v + i) = __ldg(reinterpret_cast<const uint4 *>(row + c));
+      else if constexpr (V * sizeof(T) == 8) *reinterpret_cast<uint2 *>(r.v + i) = __ldg(reinterpret_cast<const uint2 *>(row + c));
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.v[i + v] = c + v < K ? row[c + v] : from_f32<T>(-INFINITY);
+    }
+  }
+}
+
+// z becomes exp(z - m), m its largest; returns their sum (0 for a row without a live score).
+template <int VPT, int L> __device__ __forceinline__ float softmax_terms(float (&z)[VPT], float &m) {
+  float total = 0.0f;
+  m = z[0];
+#pragma unroll
+  for (int i = 1; i < VPT; ++i) m = fmaxf(m, z[i]);
+  m = seg_max<L>(m);
+  if (m == -INFINITY) m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    z[i] = expf(z[i] - m);
+    total += z[i];
+  }
+  return seg_sum<L>(total);
+}
+
+// The chosen scores' shares of their sum (lane j: slot j), from the scores themselves, so that a ratio
+// of values that both underflow is still their ratio; `sum` is the sum before the division.
+template <int L> __device__ __forceinline__ float chosen_share(float z, bool live, int func, float &sum) {
+  float t = 0.0f;
+  if (func == FGMM_SCORE_GIVEN) {
+    t = live ? z : 0.0f;
+  } else {
+    float m = seg_max<L>(live ? z : -INFINITY);
+    if (m == -INFINITY) m = 0.0f;
+    if (func == FGMM_SCORE_SOFTMAX) t = live ? expf(z - m) : 0.0f;
+    else t = live ? expf(fminf(z, 0.0f) - fminf(m, 0.0f)) / (1.0f + expf(-fabsf(z))) : 0.0f;
+  }
+  sum = seg_sum<L>(t);
+  return sum == 0.0f ? 0.0f : t / sum;
+}
+
+__device__ __forceinline__ void top_two(float &b1, float &b2, float v1, float v2) {
+  b2 = fmaxf(fmaxf(b2, v2), fminf(b1, v1));
+  b1 = fmaxf(b1, v1);
+}
+
+// Masks all but the top_groups groups of a row.  False where the sums that decide lie too close.
+template <int VPT, int V, int L>
+__device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a, int l, float bmax, float tol, float *s_group) {
+  const int per = a.K / a.n_groups, span = per / V;
+  // a group is `span` neighbouring lanes of one pack of V: all groups' best two meet in log2 span steps
+  const bool even = per % V == 0 && span <= L && (span & (span - 1)) == 0;
+  __syncwarp();
+  if (even) {
+#pragma unroll
+    for (int i = 0; i < VPT; i += V) {
+      float b1 = c[i], b2 = -INFINITY;
+#pragma unroll
+      for (int v = 1; v < V; ++v) top_two(b1, b2, c[i + v], -INFINITY);
+      for (int o = 1; o < span; o <<= 1) top_two(b1, b2, __shfl_xor_sync(kFull, b1, o), __shfl_xor_sync(kFull, b2, o));
+      const int g = (i / V * L + l) / span;
+      if (l % span == 0 && g < a.n_groups) {
+        s_group[2 * g] = b2 > -INFINITY ? b1 + b2 : b1;
+        s_group[2 * g + 1] = fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.0f);
+      }
+    }
+  } else {
+    for (int g = 0; g < a.n_groups; ++g) {
+      float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int col = column<V, L>(i, l);
+        top_two(b1, b2, col >= g * per && col < (g + 1) * per ? c[i] : -INFINITY, -INFINITY);
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) top_two(b1, b2, __shfl_xor_sync(kFull, b1, o), __shfl_xor_sync(kFull, b2, o));
+      if (l == 0) {
+        s_group[2 * g] = b2 > -INFINITY ? b1 + b2 : b1;
+        s_group[2 * g + 1] = fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.0f);
+      }
+    }
+  }
+  __syncwarp();
+  // each lane ranks its groups against all; low and high: the smallest sum that stays, the largest that goes
+  uint32_t kept = 0;
+  float low = INFINITY, high = -INFINITY, most = 0.0f;
+  for (int g = l; g < a.n_groups; g += L) {
+    const float mine = s_group[2 * g];
+    int rank = 0;
+    for (int h = 0; h < a.n_groups; ++h) {
+      const float v = s_group[2 * h];
+      rank += v > mine || (v == mine && h < g);
+    }
+    const bool alive = mine > -INFINITY;
+    if (rank < a.top_groups) {
+      kept |= 1u << g;
+      if (alive) low = fminf(low, mine);
+    } else if (alive) {
+      high = fmaxf(high, mine);
+    }
+    if (alive) most = fmaxf(most, s_group[2 * g + 1]);
+  }
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) {
+    kept |= __shfl_xor_sync(kFull, kept, o);
+    low = fminf(low, __shfl_xor_sync(kFull, low, o));
+    high = fmaxf(high, __shfl_xor_sync(kFull, high, o));
+    most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+  }
+  if (even) {
+#pragma unroll
+    for (int i = 0; i < VPT; i += V) {
+      if (!((kept >> ((i / V * L + l) / span & 31)) & 1u)) {  // (columns past K are masked already)
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[i + v] = -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (!((kept >> (column<V, L>(i, l) / per & 31)) & 1u)) c[i] = -INFINITY;
+  }
+  return high == -INFINITY || low == INFINITY || low - high > 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
+}
+
+// The row's `rounds` largest values in order (lane j: the j'th, -1 where none is left): the lanes' best ones are compared,
+// and the lane that gave its best looks for its next.
+template <int VPT, int V, int L>
+__device__ __forceinline__ void pick_by_lane(float (&c)[VPT], int rounds, int l, int &chosen, float &value) {
+  float most = c[0];
+#pragma unroll
+  for (int i = 1; i < VPT; ++i) most = fmaxf(most, c[i]);
+  for (int j = 0; j < rounds; ++j) {
+    const float best = seg_max<L>(most);
+    if (L == 32 && best == -INFINITY) break;  // (other rows of a shared warp go on)
+    // the first place of a lane that holds it
+    uint32_t col = kFull;
+    const bool holds = most == best && best > -INFINITY;
+    if (holds) {
+#pragma unroll
+      for (int i = VPT - 1; i >= 0; --i)
+        if (c[i] == best) col = column<V, L>(i, l);
+    }
+    const unsigned holders = seg_ballot<L>(holds);
+    uint32_t first = seg_get<L>(col, holders ? __ffs(holders) - 1 : 0);
+    if (__any_sync(kFull, (holders & (holders - 1)) != 0)) first = seg_min<L>(col);
+    if (l == j && first != kFull) { chosen = (int)first; value = best; }
+    if (holds && col == first) {
+      most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (column<V, L>(i, l) == (int)first) c[i] = -INFINITY;
+        most = fmaxf(most, c[i]);
+      }
+    }
+  }
+}
+
+// The same for a whole warp's row.  With bar the rounds'th largest of the lanes' maxima, what reaches bar is a handful, which
+// move to a lane each (through s_cand) and are picked in order.  Where many equal bar (responsibilities are mostly exact
+// zeros), only what is above it moves, and the slots that leaves are filled by index.  False where more than 32 are
+// above.  c may hold NaN and +inf; value_of(column) gives a value as it counts.
+template <int VPT, int V, typename F>
+__device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int lane, uint64_t *s_cand, F value_of, int &chosen, float &value) {
+  float most = c[0];
+#pragma unroll
+  for (int i = 1; i < VPT; ++i) most = fmaxf(most, c[i]);
+  most = clean(most);
+  uint32_t left = most > -INFINITY ? key_of(most) : 0u, best = 0u;
+  int r = 0;
+  for (; r < rounds; ++r) {  // (equal maxima are taken together: bar is that much lower)
+    best = __reduce_max_sync(kFull, left);
+    if (best == 0u) break;
+    if (left == best) left = 0u;
+  }
+  const float bar = r == rounds ? of_key(best) : -FLT_MAX;  // (masked values are below it)
+  constexpr int kWords = (VPT + 31) / 32;
+  uint32_t some[kWords], equal[kWords];
+  int n = 0;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) {
+    some[w] = equal[w] = 0u;
+#pragma unroll
+    for (int i = w * 32; i < VPT && i < w * 32 + 32; ++i)
+      if (c[i] >= bar) some[w] |= 1u << (i & 31);
+    n += __popc(some[w]);
+  }
+  int count = (int)__reduce_add_sync(kFull, (unsigned)n);
+  if (count > 32) {
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+#pragma unroll
+      for (int i = w * 32; i < VPT && i < w * 32 + 32; ++i)
+        if (c[i] == bar) equal[w] |= 1u << (i & 31);
+      some[w] &= ~equal[w];
+      n += __popc(some[w]);
+    }
+    count = (int)__reduce_add_sync(kFull, (unsigned)n);
+    if (count > 32) return false;
+  }
+  __syncwarp();
+  for (int base = 0; base < count;) {
+    int i = -1;
+#pragma unroll
+    for (int w = kWords - 1; w >= 0; --w)
+      if (some[w]) i = w * 32 + __ffs(some[w]) - 1;
+    const unsigned have = __ballot_sync(kFull, i >= 0);
+    if (i >= 0) {
+      const int col = column<V, 32>(i, lane);
+      s_cand[base + __popc(have & ((1u << lane) - 1u))] = (uint64_t)key_of(value_of(col)) << 32 | (uint32_t)col;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        if (i / 32 == w) some[w] &= some[w] - 1;
+    }
+    base += __popc(have);
+  }
+  __syncwarp();
+  uint32_t key = 0u, at = kFull;  // this lane's candidate
+  if (lane < count) {
+    const uint64_t x = s_cand[lane];
+    key = (uint32_t)(x >> 32);
+    at = (uint32_t)x;
+  }
+  int j = 0;
+  for (const int sorted = min(rounds, count); j < sorted; ++j) {
+    const uint32_t b = __reduce_max_sync(kFull, key);
+    const uint32_t first = __reduce_min_sync(kFull, key == b ? at : kFull);
+    if (lane == j) { chosen = (int)first; value = of_key(b); }
+    if (at == first) key = 0u;
+  }
+  for (; j < rounds; ++j) {  // the lowest column that equals bar
+    uint32_t mine = kFull;
+#pragma unroll
+    for (int w = kWords - 1; w >= 0; --w)
+      if (equal[w]) mine = column<V, 32>(w * 32 + __ffs(equal[w]) - 1, lane);
+    const uint32_t first = __reduce_min_sync(kFull, mine);
+    if (first == kFull) break;
+    if (lane == j) { chosen = (int)first; value = clean(bar); }
+    bool taken = mine == first;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+      if (taken && equal[w]) { equal[w] &= equal[w] - 1; taken = false; }
+  }
+  return true;
+}
+
+constexpr int kRouteWarps = 4;
+
+template <typename T, int VPT, int V, int L>
+__device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T, VPT> &raw, const RouteArgs &a, int l, const float *s_bias,
+                                          float bmax, uint64_t *s_cand, float *weights, int32_t *indices) {
+  // fp32 values of c are off by at most a few 2^-23 of |s| and |bias|: two that differ by more than this (times
+  // their sizes) are in the right order
+  constexpr float kTol = 1.0f / (1 << 20);
+  const bool by_value = a.bias != nullptr || a.n_groups > 1;
+  float c[VPT], m = 0.0f, total = 1.0f, inv = 1.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) c[i] = to_f32(raw.v[i]);
+  if (L < 32 || by_value || (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)) {  // (pick_few takes scores as they are)
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) c[i] = clean(c[i]);
+  }
+  if (a.func == FGMM_SCORE_SOFTMAX && (by_value || !a.renorm)) {
+    if (by_value) {
+      uint32_t live[(VPT + 31) / 32] = {};
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) live[i / 32] |= (uint32_t)(c[i] > -INFINITY) << (i & 31);
+      total = softmax_terms<VPT, L>(c, m);
+      inv = 1.0f / total;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) c[i] = ((live[i / 32] >> (i & 31)) & 1u) ? c[i] * inv : -INFINITY;
+    } else {
+      float e[VPT];
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) e[i] = c[i];
+      total = softmax_terms<VPT, L>(e, m);
+    }
+  }
+  bool sure = true;
+  if (by_value) {
+    if (a.func == FGMM_SCORE_SIGMOID) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) c[i] = c[i] > -INFINITY ? __fdividef(1.0f, 1.0f + expf(-c[i])) : -INFINITY;
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) c[i] = fmaxf(c[i] + s_bias[column<V, L>(i, l)], -INFINITY);  // -inf for NaN
+    }
+    if (a.n_groups > 1) sure = keep_groups<VPT, V, L>(c, a, l, bmax, kTol, reinterpret_cast<float *>(s_cand));
+  }
+  // one choice more than asked, where its distance from the last one is looked at
+  const int rounds = min(L, by_value ? a.top_k + 1 : a.top_k);
+  int chosen = -1;
+  float value = 0.0f;
+  bool done = false;
+  if constexpr (L == 32) {
+    done = pick_few<VPT, V>(c, rounds, l, s_cand, [&](int col) {
+      float v = score_at(row, col);
+      if (by_value) {
+        if (a.func == FGMM_SCORE_SOFTMAX) v = expf(v - m) * inv;
+        else if (a.func == FGMM_SCORE_SIGMOID) v = __fdividef(1.0f, 1.0f + expf(-v));
+        if (a.bias) v += s_bias[col];
+      }
+      return v;
+    }, chosen, value);
+    if (!done) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) c[i] = clean(c[i]);
+    }
+  }
+  if (!done) pick_by_lane<VPT, V, L>(c, rounds, l, chosen, value);
+  if (by_value) {
+    const float z = chosen >= 0 ? score_at(row, chosen) : 0.0f;
+    const float b = chosen >= 0 && a.bias ? s_bias[chosen] : 0.0f;
+    const int prev = __shfl_up_sync(kFull, chosen, 1, L);
+    const float pv = __shfl_up_sync(kFull, value, 1, L), pz = __shfl_up_sync(kFull, z, 1, L), pb = __shfl_up_sync(kFull, b, 1, L);
+    const bool near = l > 0 && chosen >= 0 && prev >= 0 && !(pz == z && pb == b) &&
+                      !(pv - value > kTol * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f);
+    const bool apart = seg_ballot<L>(near) == 0;  // (all lanes take part, whatever their rows' groups said)
+    // as many slots as lanes leave none for the next value
+    sure = sure && a.top_k < L && apart;
+    unsigned unsure = __ballot_sync(kFull, !sure && exists);
+    while (unsure) {  // row by row, the whole warp on it
+      const int from = (__ffs(unsure) - 1) / L * L, lane = threadIdx.x & 31;
+      const T *at = reinterpret_cast<const T *>(__shfl_sync(kFull, (unsigned long long)row, from));
+      const int exact = __shfl_sync(kFull, route_row64<T, (VPT * L + 31) / 32>(at, a), l);
+      if (lane / L * L == from) chosen = exact;
+      unsure &= ~((L == 32 ? kFull : (1u << L) - 1u) << from);
+    }
+  }
+  if (l >= a.top_k) chosen = -1;
+  const bool live = chosen >= 0;
+  const float z = live ? score_at(row, chosen) : 0.0f;
+  float w;
+  if (a.renorm) {
+    float sum;
+    w = chosen_share<L>(z, live, a.func, sum);
+  } else if (a.func == FGMM_SCORE_SOFTMAX) {
+    w = expf(z - m) / total;
+  } else {
+    w = a.func == FGMM_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-z)) : z;
+  }
+  if (l < a.top_k && exists) {
+    weights[l] = live ? w * a.scale : 0.0f;
+    indices[l] = chosen;
+  }
+}
+
+// Values a lane holds of the next row while this one is decided: up to 16 (more would cost occupancy).
+template <typename T, int VPT, int V, int L>
+__global__ void __launch_bounds__(32 * kRouteWarps, VPT <= 8 ? 10 : VPT <= 16 ? 7 : VPT <= 32 ? 6 : 2)
+route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict__ weights, int32_t *__restrict__ indices) {
+  constexpr int RPW = 32 / L;  // rows a warp
+  __shared__ uint64_t s_cand[kRouteWarps * RPW][32];
+  extern __shared__ float s_bias[];  // [VPT * L], zeros behind K
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, seg = lane / L;
+  float bmax = 0.0f;  // the largest finite |bias|
+  if (a.bias) {
+    for (int c = threadIdx.x; c < VPT * L; c += blockDim.x) s_bias[c] = c < a.K ? __ldg(a.bias + c) : 0.0f;
+    __syncthreads();
+    for (int c = lane; c < VPT * L; c += 32) {
+      const float b = fabsf(s_bias[c]);
+      if (b < INFINITY) bmax = fmaxf(bmax, b);
+    }
+    bmax = seg_max<32>(bmax);
+  }
+  const int64_t stride = (int64_t)gridDim.x * kRouteWarps * RPW;
+  int64_t n = ((int64_t)blockIdx.x * kRouteWarps + warp) * RPW + seg;  // the warp's first row is n - seg
+  if (n - seg >= a.N) return;
+  auto at = [&](int64_t r) { return scores + (r < a.N ? r : a.N - 1) * a.stride; };
+  Row<T, VPT> raw;
+  load_row<T, VPT, V, L>(at(n), a.K, l, raw);
+  for (;;) {
+    const int64_t next = n + stride;
+    constexpr bool kAhead = VPT <= 16;  // the next row is on its way while this one is decided
+    Row<T, kAhead ? VPT : 1> ahead;
+    const bool more = next - seg < a.N;
+    if constexpr (kAhead)
+      if (more) load_row<T, VPT, V, L>(at(next), a.K, l, ahead);
+    const bool exists = n < a.N;
+    route_row<T, VPT, V, L>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp * RPW + seg], weights + n * a.top_k, indices + n * a.top_k);
+    if (!more) break;
+    n = next;
+    if constexpr (kAhead) raw = ahead;
+    else load_row<T, VPT, V, L>(at(n), a.K, l, raw);
+  }
+}
+
+// d z from d w.  With p the shares and g = scale dw: renormalised, the chosen get
+// p (g - sum p g), times 1 - s for the sigmoid, or (g - sum p g) / sum for given values, and all
+// others nothing; else the softmax gives s (g [chosen] - sum of g s over the chosen) to every score, and
+// sigmoid and given values pass g s (1 - s) and g on.  The row without the chosen ones' part is written first (the
+// scores are read for the softmax only), then the lane of each slot writes its element.
+template <typename T, int VPT, int V, int L>
+__global__ void __launch_bounds__(128) route_backward_kernel(const float *__restrict__ dw, const T *__restrict__ scores,
+                                                             const int32_t *__restrict__ indices, const RouteArgs a,
+                                                             T *__restrict__ dz) {
+  const int lane = threadIdx.x & 31, l = lane % L;
+  const bool dense = a.func == FGMM_SCORE_SOFTMAX && !a.renorm;
+  const int64_t stride = (int64_t)gridDim.x * (128 / L);
+  for (int64_t n = (int64_t)blockIdx.x * (128 / L) + threadIdx.x / L; n - lane / L < a.N; n += stride) {
+    const bool exists = n < a.N;
+    const int64_t r = exists ? n : a.N - 1;
+    const T *row = scores + r * a.stride;
+    Row<T, VPT> raw;
+    if (dense) load_row<T, VPT, V, L>(row, a.K, l, raw);
+    int chosen = l < a.top_k ? __ldg(indices + r * a.top_k + l) : -1;
+    if (chosen < 0 || chosen >= a.K) chosen = -1;
+    const float z = chosen >= 0 ? score_at(row, chosen) : -INFINITY;
+    const bool live = z > -INFINITY;  // a masked score gets no gradient
+    const float g = live ? __ldg(dw + r * a.top_k + l) * a.scale : 0.0f;
+    float out[VPT], d, base = 0.0f;
+    if (dense) {
+      float m;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) out[i] = clean(to_f32(raw.v[i]));
+      const float total = softmax_terms<VPT, L>(out, m), inv = total > 0.0f ? 1.0f / total : 0.0f;
+      const float s = live ? expf(z - m) * inv : 0.0f;
+      d = s * g;
+      const float all = -seg_sum<L>(d);
+      base = s * all;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) out[i] = out[i] * inv * all;
+    } else {
+      if (a.renorm) {
+        float sum;
+        const float p = chosen_share<L>(z, live, a.func, sum);
+        d = g - seg_sum<L>(p * g);
+        if (a.func == FGMM_SCORE_GIVEN) d = sum == 0.0f ? 0.0f : d / sum;
+        else d *= a.func == FGMM_SCORE_SIGMOID ? p / (1.0f + expf(z)) : p;
+      } else {
+        d = g;
+        if (a.func == FGMM_SCORE_SIGMOID) {
+          const float e = expf(-fabsf(z));
+          d = g * e / ((1.0f + e) * (1.0f + e));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) out[i] = 0.0f;
+    }
+    if (!live) { d = 0.0f; chosen = -1; }
+    float sum = base;  // slots of one expert add up, in all of their lanes alike
+    for (int j = 0; j < a.top_k; ++j) {
+      const int cj = seg_get<L>(chosen, j);
+      const float dj = seg_get<L>(d, j);
+      if (cj == chosen) sum += dj;
+    }
+    T *to = dz + r * a.K;
+    if (exists) {
+#pragma unroll
+      for (int i = 0; i < VPT; i += V) {
+        const int c = column<V, L>(i, l);
+        if (V > 1 && c + V <= a.K) {
+          alignas(16) T pack[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) pack[v] = from_f32<T>(out[i + v]);
+          if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4 *>(to + c) = *reinterpret_cast<uint4 *>(pack);
+          else if constexpr (V * sizeof(T) == 8) *reinterpret_cast<uint2 *>(to + c) = *reinterpret_cast<uint2 *>(pack);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (c + v < a.K) to[c + v] = from_f32<T>(out[i + v]);
+        }
+      }
+    }
+    __syncwarp();  // orders the two writes of a chosen element
+    if (exists && chosen >= 0) to[chosen] = from_f32<T>(sum);
+  }
+}
+
+// Lanes L of a row and values VPT a lane holds, for K columns and `slots` lanes that the choices take.  A row of up to 256
+// columns takes part of a warp where few are chosen, since what a row costs beside its values is then shared
+// (K = 128, two chosen: 442 -> 187 instructions a row); more choices are picked faster by a warp's reductions.
+// Packs are 16 bytes (8 for a 16-bit row of up to 128 columns) where the rows are aligned for them.
+template <typename T, typename F> int by_row_width(int K, int slots, bool vec, F f) {
+  constexpr int V = 16 / sizeof(T);
+#define FGMM_WIDTH(n, v, lanes) \
+  return vec ? f(std::integral_constant<int, n>{}, std::integral_constant<int, v>{}, std::integral_constant<int, lanes>{}) \
+             : f(std::integral_constant<int, n>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, lanes>{});
+  if (K <= 32 && slots <= 8) FGMM_WIDTH(4, 4, 8)
+  if (K <= 128 && slots <= 4) FGMM_WIDTH(16, V, 8)
+  if (K <= 256 && slots <= 4) FGMM_WIDTH(16, V, 16)
+  if (K <= 128) FGMM_WIDTH(4, 4, 32)
+  if (K <= 256) FGMM_WIDTH(8, V, 32)
+  if (K <= 512) FGMM_WIDTH(16, V, 32)
+  if (K <= 1024) FGMM_WIDTH(32, V, 32)
+  FGMM_WIDTH(128, V, 32)
+#undef FGMM_WIDTH
+}
+
+template <typename T>
+int route_forward_t(const T *z, const RouteArgs &a, float *w, int32_t *idx, cudaStream_t st) {
+  const bool vec = reinterpret_cast<uintptr_t>(z) % 16 == 0 && a.stride * sizeof(T) % 16 == 0;
+  const int slots = a.top_k + (a.bias || a.n_groups > 1 ? 1 : 0);
+  return by_row_width<T>(a.K, slots, vec, [&](auto vpt, auto v, auto lanes) {
+    // every warp slot of the device once (64 warps an SM), so that the rows after the first are prefetched
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, kRouteWarps * (32 / lanes())), (int64_t)num_sms() * 64 / kRouteWarps);
+    const size_t smem = a.bias ? vpt() * lanes() * sizeof(float) : 0;
+    route_kernel<T, vpt(), v(), lanes()><<<grid, 32 * kRouteWarps, smem, st>>>(z, a, w, idx);
+    FGMM_LAUNCH_CHECK("route_kernel");
+    return FGMM_OK;
+  });
+}
+
+template <typename T>
+int route_backward_t(const float *dw, const T *z, const int32_t *idx, const RouteArgs &a, T *dz, cudaStream_t st) {
+  const bool vec = reinterpret_cast<uintptr_t>(z) % 16 == 0 && a.stride * sizeof(T) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(dz) % 16 == 0 && a.K * sizeof(T) % 16 == 0;
+  return by_row_width<T>(a.K, a.top_k, vec, [&](auto vpt, auto v, auto lanes) {
+    const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, 128 / lanes()), (int64_t)num_sms() * 16);
+    route_backward_kernel<T, vpt(), v(), lanes()><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
+    FGMM_LAUNCH_CHECK("route_backward_kernel");
+    return FGMM_OK;
+  });
+}
+
+}  // namespace
+
+int route_forward(const void *scores, int dtype, int64_t N, int K, int64_t stride, const float *bias,
+                  int top_k, int func, int n_groups, int top_groups, bool renorm, float scale,
+                  float *weights, int32_t *indices, cudaStream_t st) {
+  const RouteArgs a{N, stride, K, top_k, func, n_groups, top_groups, bias, renorm, scale};
+  if (dtype == FGMM_F32) return route_forward_t((const float *)scores, a, weights, indices, st);
+  if (dtype == FGMM_BF16) return route_forward_t((const __nv_bfloat16 *)scores, a, weights, indices, st);
+  return route_forward_t((const __half *)scores, a, weights, indices, st);
+}
+
+int route_backward(const float *dw, const void *scores, int dtype, int64_t N, int K, int64_t stride,
+                   const int32_t *indices, int top_k, int func, bool renorm, float scale, void *dz,
+                   cudaStream_t st) {
+  const RouteArgs a{N, stride, K, top_k, func, 1, 1, nullptr, renorm, scale};
+  if (dtype == FGMM_F32) return route_backward_t(dw, (const float *)scores, indices, a, (float *)dz, st);
+  if (dtype == FGMM_BF16) return route_backward_t(dw, (const __nv_bfloat16 *)scores, indices, a, (__nv_bfloat16 *)dz, st);
+  return route_backward_t(dw, (const __half *)scores, indices, a, (__half *)dz, st);
+}
+
+}  // namespace fgmm
