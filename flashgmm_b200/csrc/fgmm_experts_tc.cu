@@ -9,11 +9,11 @@
 // the results, and the next tile's products run meanwhile.  A tile has M = 128 rows of one expert (or, for
 // DW, 128 of its output dimensions) and NT columns; a stage holds 64 elements of the contraction.
 //   * The points' rows of X are gathered straight from the points' matrix by 16-byte cp.async, in the
-//     swizzled layout that TMA writes, so a grouped copy of X is never made.  (TMA gather4 measured 80
-//     cycles for four 128-byte rows, a third of what the products consume: 326 us against 39 us of the same
-//     products with contiguous rows at 8,186 rows, 1,000 x 1,016.)  Rows a tile does not have are not loaded: their
-//     accumulator rows hold leftovers that nobody reads.  Where the rows are the contraction (DW), those behind
-//     the expert's last one are zeros in both operands.
+//     swizzled layout that TMA writes, so a grouped copy of X is never made.  (TMA gather4 measured 80 cycles for
+//     four 128-byte rows; a grouped copy read by TMA made DW slower: 32,768 rows 1,024 x 2,048 197 -> 216 us, 8,186 rows
+//     1,000 x 1,016 60 -> 107 us.)  Rows a tile does not have are not loaded: their accumulator rows hold leftovers
+//     that nobody reads.  Where the rows are the contraction (DW), those behind the expert's last one are zeros in
+//     both operands.
 //   * W is fetched as a box of its 3-D tensor, K-major for Y, and MN-major, without a transposed copy, for DX.
 //   * float32 operands are three bf16 planes (x = b0 + b1 + b2, 24 bits together), laid out by
 //     split_planes_kernel, and the six products that matter (b0 b0 into one accumulator; b0 b1, b1 b0, b1 b1,
@@ -38,6 +38,7 @@ constexpr int KCH = 64;       // contraction elements of a stage (128-byte rows)
 constexpr int kGather = 128;   // gathering threads: warps 2-5
 constexpr int kEpiWarps = 8;   // warps 6-13: two per tensor-memory lane quarter, half of the columns each
 constexpr int kThreads = 64 + kGather + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA
+constexpr int kList = 64;      // tiles of a block that are found ahead
 constexpr int kSegment = 4;   // stages between drains of a float32 product (256 elements)
 
 // A load that stays where it is written (a plan's entry fetched a stage ahead of its use).
@@ -57,9 +58,22 @@ struct Shape {
   static constexpr int kStages = (192 * 1024) / kStage;
   static constexpr int kOut = kEpiWarps * 16 * 128;  // a 16-row, 128-byte staging tile for each epilogue warp
   static constexpr int kBars = 320;
-  static constexpr int smem(int K) { return 1024 + kStages * kStage + kOut + kBars + (K + 1) * 4; }
+  static constexpr int smem(int K) { return 1024 + kStages * kStage + kOut + kBars + kList * 16 + (K + 1) * 4; }
   static_assert(kStages >= 2, "shared-memory budget");
   static_assert(smem(kMaxExperts) <= 227 * 1024, "shared-memory budget");
+};
+
+// DW is divided into pieces of at most `most` stages: piece by piece of an expert, all its tiles (so that the blocks at work
+// read the same rows), the pieces going round the blocks.  An expert with most of the rows is shared by many blocks
+// that way (65,536 points over 256 experts, 128 x 128: 137 us of one tile's block alone, while the others had 9 % of its
+// work).  Where an expert has more than one piece, its pieces go as fp32 tiles to slots that join_pieces_kernel adds in order.
+// An expert without rows has one piece, of zeros.
+struct Pieces {
+  const int *first;   // [K + 1] pieces (of a tile) of the experts before
+  const int *slot;    // [K + 1] those of them that are joined
+  const int *joined;  // [K + 1] experts before that are joined
+  float *tiles;       // [slots][BM][NT]
+  int most, slots;
 };
 
 struct TcArgs {
@@ -70,50 +84,83 @@ struct TcArgs {
   const uint16_t *a_rows, *b_rows;  // the same matrices for the gathering warps
   int a_cols, b_cols;               // columns of their rows in memory
   uint32_t idesc;
+  Pieces pieces;  // DW
   uint32_t div_mul, div_shift;  // n / top_k = n * div_mul >> div_shift for n < 2^31
   int vec;  // rows of the result start on 16-byte boundaries
 };
 
-// What one tile covers.  For Y and DX: expert e, rows [r0, r0 + rows), columns from n0.  For DW: expert e, output
-// dimensions from m0 (`rows` of them), columns from n0, contraction over the rows [r0, r1).
+// What one tile covers.  For Y and DX: `rows` rows from r0 of expert e, columns from n0.  For DW: `rows` output dimensions
+// from m0, columns from n0, contraction over the rows [r0, r1).  Stages [c0, c1) of the contraction; a piece of
+// a DW tile goes to slot `slot` of the partial results (-1: a whole tile).
 struct Tile {
-  int e, r0, r1, rows, m0, n0, nk;
+  int e, r0, r1, rows, m0, n0, c0, c1, slot;
 };
 
+// Last expert e with s_first[e] <= m.
+__device__ __forceinline__ int find_expert(const int *s_first, int K, int m) {
+  int lo = 0, hi = K;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_first[mid] <= m) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int expert_stages(const RoutePlan &p, int e) {
+  int lo, hi;
+  expert_rows(p.offsets, e, (int)p.R, lo, hi);
+  return max(1, (hi - lo + KCH - 1) / KCH);
+}
+
+// The tiles of this block, in order.
 template <int MODE, int NT>
 struct Tiles {
   const TcArgs &a;
-  const int *s_tile;  // first tile of rows of each expert (Y, DX)
-  int n_tiles, m_tiles, total, e = 0;
+  const int *s_first;   // tiles of rows (Y, DX) or pieces (DW) of the experts before
+  const int4 *s_list;   // Y, DX: the block's first kList tiles, found by its threads at once
+  int n_tiles, total, i = 0;
 
-  __device__ Tiles(const TcArgs &args, const int *st) : a(args), s_tile(st) {
-    const int width = MODE == kForward ? a.d_out : a.d_in;
-    n_tiles = (width + NT - 1) / NT;
-    m_tiles = (a.d_out + BM - 1) / BM;
-    total = MODE == kWeights ? a.plan.K * m_tiles * n_tiles : s_tile[a.plan.K] * n_tiles;
+  __device__ Tiles(const TcArgs &args, const int *sf, const int4 *sl) : a(args), s_first(sf), s_list(sl) {
+    n_tiles = ((MODE == kForward ? a.d_out : a.d_in) + NT - 1) / NT;
+    total = s_first[a.plan.K] * (MODE == kWeights ? per() : n_tiles);
   }
-  // t never decreases from call to call.
-  __device__ Tile at(int t) {
-    Tile x;
-    const int R = (int)a.plan.R;
-    x.n0 = t % n_tiles * NT;
-    const int m = t / n_tiles;
+  __device__ int per() const { return (a.d_out + BM - 1) / BM * n_tiles; }  // tiles of an expert's DW
+  __device__ int4 find(int t) const {  // {expert, first row, rows, first column}
+    const int m = t / n_tiles, e = find_expert(s_first, a.plan.K, m);
+    int lo, hi;
+    expert_rows(a.plan.offsets, e, (int)a.plan.R, lo, hi);
+    lo += (m - s_first[e]) * BM;
+    return make_int4(e, lo, max(0, min(BM, hi - lo)), t % n_tiles * NT);
+  }
+  __device__ bool next(Tile &x) {
+    const int64_t t = blockIdx.x + (int64_t)i * gridDim.x;
+    if (t >= total) return false;
     if (MODE == kWeights) {
-      x.e = m / m_tiles;
-      x.m0 = m % m_tiles * BM;
+      const int m = (int)t / per(), tile = (int)t % per();
+      x.e = find_expert(s_first, a.plan.K, m);
+      const int piece = m - s_first[x.e], pieces = s_first[x.e + 1] - s_first[x.e];
+      x.m0 = tile / n_tiles * BM;
+      x.n0 = tile % n_tiles * NT;
       x.rows = min(BM, a.d_out - x.m0);
-      expert_rows(a.plan.offsets, x.e, R, x.r0, x.r1);
-      x.nk = (x.r1 - x.r0 + KCH - 1) / KCH;
+      expert_rows(a.plan.offsets, x.e, (int)a.plan.R, x.r0, x.r1);
+      x.c0 = piece * a.pieces.most;
+      x.c1 = min(max(1, (x.r1 - x.r0 + KCH - 1) / KCH), x.c0 + a.pieces.most);
+      x.slot = -1;
+      if (pieces > 1) x.slot = min((__ldg(a.pieces.slot + x.e) + piece) * per() + tile, a.pieces.slots - 1);
+      ++i;
     } else {
-      while (e + 1 < a.plan.K && s_tile[e + 1] <= m) ++e;
-      x.e = e;
-      x.m0 = 0;
-      expert_rows(a.plan.offsets, e, R, x.r0, x.r1);
-      x.r0 += (m - s_tile[e]) * BM;
-      x.rows = max(0, min(BM, x.r1 - x.r0));
-      x.nk = ((MODE == kForward ? a.d_in : a.d_out) + KCH - 1) / KCH;
+      const int4 f = i < kList ? s_list[i] : find((int)t);
+      ++i;
+      x.e = f.x;
+      x.r0 = f.y;
+      x.rows = f.z;
+      x.n0 = f.w;
+      x.r1 = x.r0 + x.rows;
+      x.m0 = x.c0 = 0;
+      x.c1 = ((MODE == kForward ? a.d_in : a.d_out) + KCH - 1) / KCH;
+      x.slot = -1;
     }
-    return x;
+    return true;
   }
 };
 
@@ -143,7 +190,8 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   uint64_t *bars = reinterpret_cast<uint64_t *>(s_out + Sh::kOut);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_out + Sh::kOut + Sh::kBars - 96);
   int *s_warp = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars - 80);  // [warps]
-  int *s_tile = reinterpret_cast<int *>(s_out + Sh::kOut + Sh::kBars);        // [K + 1]
+  int4 *s_list = reinterpret_cast<int4 *>(s_out + Sh::kOut + Sh::kBars);      // [kList]
+  int *s_first = reinterpret_cast<int *>(s_list + kList);                     // [K + 1]
   const uint32_t bar0 = smem_u32(bars);
   auto FULL = [&](int s) { return bar0 + 8u * s; };
   auto EMPTY = [&](int s) { return bar0 + 8u * (S + s); };
@@ -168,15 +216,18 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     tmem_relinquish();
   }
   griddep_wait();
-  if (MODE != kWeights) {  // first tile of rows of each expert
+  if (MODE == kWeights) {
+    for (int e = threadIdx.x; e <= K; e += kThreads) s_first[e] = a.pieces.slots > 1 ? __ldg(a.pieces.first + e) : e;
+  } else {  // tiles of rows of the experts before each
+    auto units = [&](int e) {
+      int lo, hi;
+      expert_rows(a.plan.offsets, e, R, lo, hi);
+      return (hi - lo + BM - 1) / BM;
+    };
     const int per = (K + kThreads - 1) / kThreads;
     const int e0 = min(K, (int)threadIdx.x * per), e1 = min(K, e0 + per);
     int mine = 0;
-    for (int e = e0; e < e1; ++e) {
-      int lo, hi;
-      expert_rows(a.plan.offsets, e, R, lo, hi);
-      mine += (hi - lo + BM - 1) / BM;
-    }
+    for (int e = e0; e < e1; ++e) mine += units(e);
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,19 +239,22 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     int run = sum - mine;
     for (int w = 0; w < warp; ++w) run += s_warp[w];
     for (int e = e0; e < e1; ++e) {
-      int lo, hi;
-      expert_rows(a.plan.offsets, e, R, lo, hi);
-      s_tile[e] = run;
-      run += (hi - lo + BM - 1) / BM;
+      s_first[e] = run;
+      run += units(e);
     }
-    if (threadIdx.x == kThreads - 1) s_tile[K] = run;
+    if (threadIdx.x == kThreads - 1) s_first[K] = run;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   griddep_launch();
   const uint32_t tmem = *tmem_slot;
-  Tiles<MODE, NT> tiles(a, s_tile);
+  Tiles<MODE, NT> tiles(a, s_first, s_list);
+  if (MODE != kWeights) {
+    const int64_t t = blockIdx.x + (int64_t)threadIdx.x * gridDim.x;
+    if (threadIdx.x < kList && t < tiles.total) s_list[threadIdx.x] = tiles.find((int)t);
+    __syncthreads();
+  }
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
@@ -208,13 +262,13 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     uint32_t phase = 0;
     int filled = 0;  // stages ever armed, up to S
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles.total && ok && lane == 0; t += gridDim.x) {
-      const Tile x = tiles.at(t);
-      for (int c = 0; c < x.nk; ++c) {
+    Tile x;
+    while (lane == 0 && ok && tiles.next(x)) {
+      for (int c = x.c0; c < x.c1; ++c) {
         if (!mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty)) { ok = false; break; }
         const uint32_t base = smem_u32(smem + stage * Sh::kStage), base_b = base + P * Sh::kA;
         if (MODE == kWeights && x.r0 + (c + 1) * KCH > x.r1) {
-          mbar_arrive(FULL(stage));  // the gathering warps fetch the last rows of both operands
+          mbar_arrive(FULL(stage));  // the gathering warps fetch an expert's last rows of both operands
         } else {
           mbar_arrive_expect_tx(FULL(stage), P * ((MODE != kForward ? Sh::kA : 0) + (MODE != kWeights ? Sh::kB : 0)));
 #pragma unroll
@@ -259,16 +313,16 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       int stage = 0, seg = 0, count = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, ++count) {
-        const int nk = tiles.at(t).nk;
+      Tile x;
+      for (; ok && tiles.next(x); ++count) {
         const uint32_t low = tmem + (2 + (count & 1)) * NT;  // the smaller products of a float32 tile
-        int c = 0;
+        int c = x.c0;
         do {  // a segment: the whole tile, or kSegment stages of a float32 one
           const int buf = seg & 1;
           if (!mbar_wait(TEMPTY(buf), ((seg >> 1) & 1) ^ 1, kErrWaitTmemEmpty)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem + buf * NT;
-          const int first = c, end = SPLIT ? min(nk, c + kSegment) : nk;
+          const int first = c, end = SPLIT ? min(x.c1, c + kSegment) : x.c1;
           for (; c < end; ++c) {
             if (!mbar_wait(FULL(stage), phase, kErrWaitFull)) { ok = false; break; }
             if (MODE != kInputs) fence_proxy_async_smem();  // the gathered rows were written through the generic proxy
@@ -278,7 +332,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             for (int kk = 0; kk < KCH / 16; ++kk) {
               const uint64_t ak = ad + kk * kStepA, bk = bd + kk * kStepB;
               if constexpr (SPLIT) {
-                mma_f16(low, ak + 2 * kPlA, bk, a.idesc, (c != 0 || kk != 0) ? 1u : 0u);
+                mma_f16(low, ak + 2 * kPlA, bk, a.idesc, (c != x.c0 || kk != 0) ? 1u : 0u);
                 mma_f16(low, ak, bk + 2 * kPlB, a.idesc, 1u);
                 mma_f16(low, ak + kPlA, bk + kPlB, a.idesc, 1u);
                 mma_f16(low, ak + kPlA, bk, a.idesc, 1u);
@@ -292,7 +346,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           if (!ok) break;
           mma_commit(TFULL(buf));
           ++seg;
-        } while (c < nk);
+        } while (c < x.c1);
       }
       mma_commit(DONE);
       mbar_wait_drain(DONE, 0);
@@ -302,101 +356,97 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     // ---------------------------------------------------------------- gathered rows
     if (MODE != kInputs) {
       // Eight threads share a 128-byte row of a tile, thread j its 16 bytes, stored at chunk j ^ (row % 8); a thread
-      // takes the rows rr, rr + 16, ...  Its arrival on a stage follows by itself when its copies are complete.
+      // takes the rows rr, rr + kStep, ...  Its arrival on a stage follows by itself when its copies are complete.
       constexpr int kStep = kGather / 8, kRows = (MODE == kForward ? BM : KCH) / kStep;
       const int j = lane & 7, rr = (threadIdx.x - 64) >> 3;
       const uint32_t at = rr * 128 + ((j ^ (rr & 7)) << 4);
+      const uint16_t *matrix = MODE == kForward ? a.a_rows : a.b_rows;
+      const int matrix_cols = MODE == kForward ? a.a_cols : a.b_cols;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x) {
-        const Tile x = tiles.at(t);
-        int id[kRows];  // routes of this thread's rows, -1: none
-        auto routes = [&](int r0, int r1) {
+      int id[kRows];  // routes of this thread's rows, -1: none; fetched a tile (Y) or a stage (DW) ahead of their use
+      auto routes = [&](int r0, int r1) {
 #pragma unroll
-          for (int i = 0; i < kRows; ++i) id[i] = r0 + rr + kStep * i < r1 ? ld_now(a.plan.order + r0 + rr + kStep * i) : -1;
-        };
-        auto point = [&](int i) { return (int)(((uint64_t)(uint32_t)id[i] * a.div_mul) >> a.div_shift); };
-        routes(x.r0, MODE == kForward ? x.r0 + x.rows : x.r1);
+        for (int i = 0; i < kRows; ++i) id[i] = r0 + rr + kStep * i < r1 ? ld_now(a.plan.order + r0 + rr + kStep * i) : -1;
+      };
+      const uint16_t *src[kRows];
+      int bytes[kRows];
+      auto sources = [&](int col) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const bool in = id[i] >= 0 && id[i] < R;
+          const int point = (int)(((uint64_t)(uint32_t)id[i] * a.div_mul) >> a.div_shift);
+          src[i] = matrix + (in ? (int64_t)point * matrix_cols + col + j * 8 : 0);
+          bytes[i] = in ? 16 : 0;
+        }
+      };
+      Tile x, ahead;
+      bool more = tiles.next(ahead);
+      auto first_routes = [&] { routes(ahead.r0 + ahead.c0 * KCH, ahead.r1); };
+      if (more) first_routes();
+      while (more && ok) {
+        x = ahead;
+        more = tiles.next(ahead);
         if (MODE == kForward) {
-          const uint16_t *src[kRows];
-          uint32_t live = 0;
+          sources(0);
+          if (more) first_routes();
+        }
+        int cols[NT / 64];  // DW: bytes of this thread's 16 in each 64 columns of the tile
 #pragma unroll
-          for (int i = 0; i < kRows; ++i) {
-            const bool in = id[i] >= 0 && id[i] < R;
-            src[i] = a.a_rows + (in ? (int64_t)point(i) * a.a_cols + j * 8 : 0);
-            live |= (uint32_t)in << i;
+        for (int n = 0; n < NT / 64; ++n) cols[n] = x.n0 + n * 64 + j * 8 < a.b_plane ? 16 : 0;
+        for (int c = x.c0; c < x.c1; ++c) {
+          const int r = x.r0 + c * KCH;
+          if (MODE == kWeights) {
+            sources(x.n0);
+            if (c + 1 < x.c1) routes(r + KCH, x.r1);
+            else if (more) first_routes();
           }
-          for (int c = 0; c < x.nk; ++c) {
-            ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty));
-            if (!ok) break;
-            const uint32_t base = smem_u32(smem + stage * Sh::kStage) + at;
-            const uint32_t now = c * KCH + j * 8 < a.a_plane ? live : 0;  // columns behind the last are zeros
+          ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty));
+          if (!ok) break;
+          const uint32_t base = smem_u32(smem + stage * Sh::kStage) + at;
+          if (MODE == kForward) {
+            const bool in = c * KCH + j * 8 < a.a_plane;  // columns behind the last are zeros (and not read)
+            // a few rows (a decoding batch) take one copy a thread; with a test on each copy all tiles paid for it
+            // (32,768 rows, 1,024 -> 2,048: 156 -> 169 us)
+            if (x.rows <= kStep) {
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+              for (int p = 0; p < P; ++p) cp_async16(base + p * Sh::kA, src[0] + p * a.a_plane + c * KCH, in ? bytes[0] : 0);
+            } else {
 #pragma unroll
-              for (int i = 0; i < kRows; ++i) {
-                if (kStep * i >= x.rows) break;
-                cp_async16(base + p * Sh::kA + i * kStep * 128, ((now >> i) & 1) ? src[i] + p * a.a_plane + c * KCH : a.a_rows, ((now >> i) & 1) * 16);
-              }
-            cp_async_arrive(FULL(stage));
-            if (++stage == S) { stage = 0; phase ^= 1; }
-          }
-        } else {
-          // columns of B that exist, a bit per 64-column atom
-          uint32_t cols = 0;
+              for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int n = 0; n < NT / 64; ++n) cols |= (uint32_t)(x.n0 + n * 64 + j * 8 < a.b_plane) << n;
-          for (int c = 0; c < x.nk; ++c) {
-            const uint16_t *src[kRows];
-            uint32_t live = 0;
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-              const bool in = id[i] >= 0 && id[i] < R;
-              src[i] = a.b_rows + (in ? (int64_t)point(i) * a.b_cols + x.n0 + j * 8 : 0);
-              live |= (uint32_t)in << i;
+                for (int i = 0; i < kRows; ++i)
+                  cp_async16(base + p * Sh::kA + i * kStep * 128, src[i] + p * a.a_plane + c * KCH, in ? bytes[i] : 0);
             }
-            const int r = x.r0 + c * KCH;
-            if (c + 1 < x.nk) routes(r + KCH, x.r1);
-            ok = __all_sync(0xffffffffu, mbar_wait(EMPTY(stage), phase ^ 1, kErrWaitEmpty));
-            if (!ok) break;
-            const uint32_t base = smem_u32(smem + stage * Sh::kStage) + at;
+          } else {
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
               for (int i = 0; i < kRows; ++i)
 #pragma unroll
-                for (int n = 0; n < NT / 64; ++n) {
-                  const uint32_t on = (live >> i) & (cols >> n) & 1;
-                  cp_async16(base + P * Sh::kA + p * Sh::kB + n * KCH * 128 + i * kStep * 128, on ? src[i] + p * a.b_plane + n * 64 : a.b_rows, on * 16);
-                }
+                for (int n = 0; n < NT / 64; ++n)
+                  cp_async16(base + P * Sh::kA + p * Sh::kB + n * KCH * 128 + i * kStep * 128, src[i] + p * a.b_plane + n * 64,
+                             bytes[i] & cols[n]);
             if (r + KCH > x.r1) {  // the last rows of A too
-#pragma unroll
+#pragma unroll 1
               for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int i = 0; i < kRows; ++i)
+#pragma unroll 1
+                for (int i = 0; i < KCH; i += kStep)
 #pragma unroll
                   for (int m = 0; m < BM / 64; ++m) {
-                    const int row = r + rr + kStep * i, col = x.m0 + m * 64 + j * 8;
+                    const int row = r + rr + i, col = x.m0 + m * 64 + j * 8;
                     const bool on = row < x.r1 && col < a.a_plane;
-                    cp_async16(base + p * Sh::kA + m * KCH * 128 + i * kStep * 128,
+                    cp_async16(base + p * Sh::kA + m * KCH * 128 + i * 128,
                                on ? a.a_rows + (int64_t)row * a.a_cols + p * a.a_plane + col : a.a_rows, on ? 16 : 0);
                   }
             }
-            cp_async_arrive(FULL(stage));
-            if (++stage == S) { stage = 0; phase ^= 1; }
           }
+          cp_async_arrive(FULL(stage));
+          if (++stage == S) { stage = 0; phase ^= 1; }
         }
       }
       cp_async_wait_all();
-    }
-    if (MODE == kForward) {  // rows of no expert
-      const int64_t none = min(max(__ldg(a.plan.offsets + K), 0), R), first = none * a.d_out, end = (int64_t)R * a.d_out;
-      const int step = a.vec ? 16 / sizeof(OUT) : 1;
-      for (int64_t i = first + (int64_t)(blockIdx.x * kGather + threadIdx.x - 64) * step; i < end; i += (int64_t)gridDim.x * kGather * step) {
-        if (a.vec) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
-        else out[i] = from_f32<OUT>(0.0f);
-      }
     }
   } else {
     // ---------------------------------------------------------------- epilogue
@@ -443,23 +493,36 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         __syncwarp();
       }
     };
-    for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, ++count) {
-      const Tile x = tiles.at(t);
+    if (MODE == kForward) {  // rows of no expert, before the first tile is done
+      const int64_t none = min(max(__ldg(a.plan.offsets + K), 0), R), first = none * a.d_out, end = (int64_t)R * a.d_out;
+      const int step = a.vec ? 16 / sizeof(OUT) : 1;
+      for (int64_t i = first + (int64_t)(blockIdx.x * 32 * kEpiWarps + threadIdx.x - 64 - kGather) * step; i < end; i += (int64_t)gridDim.x * 32 * kEpiWarps * step) {
+        if (a.vec) *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
+        else out[i] = from_f32<OUT>(0.0f);
+      }
+    }
+    // a piece of a tile: fp32, a row a lane
+    auto write_piece = [&](const float *v, int n, const Tile &x, int c0) {
+      float4 *to = reinterpret_cast<float4 *>(a.pieces.tiles + ((int64_t)x.slot * BM + q * 32 + lane) * NT + c0);
+      for (int k = 0; k < n / 4; ++k) to[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    };
+    Tile x;
+    for (; ok && tiles.next(x); ++count) {
       const bool live = q * 32 < x.rows && x.n0 + half < width;
       float acc[W];
       if constexpr (SPLIT) {
 #pragma unroll
         for (int i = 0; i < W; ++i) acc[i] = 0.0f;
       }
-      int c = 0;
+      int c = x.c0;
       do {
         const int buf = seg & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(TFULL(buf), (seg >> 1) & 1, kErrWaitTmemFull));
         if (!ok) break;
         tc_fence_after();
-        c = SPLIT ? c + kSegment : x.nk;
+        c = SPLIT ? c + kSegment : x.c1;
         if constexpr (SPLIT) {
-          if (live && x.nk > 0) {
+          if (live) {
             auto add = [&](uint32_t from) {
 #pragma unroll
               for (int i = 0; i < HC / 32; ++i) {
@@ -471,7 +534,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
               }
             };
             add(lane_tmem + buf * NT);
-            if (c >= x.nk) add(lane_tmem + (2 + (count & 1)) * NT);
+            if (c >= x.c1) add(lane_tmem + (2 + (count & 1)) * NT);
           }
         } else if (live) {
           for (int i = 0; i < HC / CW; ++i) {
@@ -479,24 +542,25 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
             for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
             tmem_wait_ld();
-            if (x.nk == 0) {  // an expert without a row
-#pragma unroll
-              for (int k = 0; k < CW; ++k) acc[k] = 0.0f;
-            }
-            write(acc, x, half + i * CW);
+            if (MODE == kWeights && x.slot >= 0) write_piece(acc, CW, x, half + i * CW);
+            else write(acc, x, half + i * CW);
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(TEMPTY(buf));
         if constexpr (SPLIT) {
-          if (c >= x.nk && live) {
+          if (c >= x.c1 && live) {
+            if (MODE == kWeights && x.slot >= 0) {
+              write_piece(acc, HC, x, half);
+            } else {
 #pragma unroll
-            for (int i = 0; i < HC / CW; ++i) write(acc + i * CW, x, half + i * CW);
+              for (int i = 0; i < HC / CW; ++i) write(acc + i * CW, x, half + i * CW);
+            }
           }
         }
         ++seg;
-      } while (c < x.nk);
+      } while (c < x.c1);
     }
   }
   tc_fence_before();
@@ -504,6 +568,82 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, kCols);
+  }
+}
+
+// The pieces of DW: one block.
+constexpr int kPlanThreads = 512;
+__global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, int most, int *__restrict__ first, int *__restrict__ slot,
+                                                                   int *__restrict__ joined) {
+  __shared__ int s_warp[kPlanThreads / 32][3];
+  griddep_launch();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int run[3] = {0, 0, 0};
+  for (int e0 = 0; e0 <= p.K; e0 += kPlanThreads) {
+    const int e = e0 + threadIdx.x;
+    const int n = e < p.K ? (expert_stages(p, e) + most - 1) / most : 0;
+    const int mine[3] = {n, n > 1 ? n : 0, n > 1};
+    int sum[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      sum[q] = mine[q];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum[q], o);
+        if (lane >= o) sum[q] += v;
+      }
+      if (lane == 31) s_warp[warp][q] = sum[q];
+    }
+    __syncthreads();
+    int before[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      before[q] = run[q] + sum[q] - mine[q];
+      for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w < warp) before[q] += s_warp[w][q];
+        run[q] += s_warp[w][q];
+      }
+    }
+    if (e <= p.K) {
+      first[e] = before[0];
+      slot[e] = before[1];
+      joined[e] = before[2];
+    }
+    __syncthreads();
+  }
+}
+
+// Adds the pieces of the experts that have more than one: blockIdx.x counts their tiles, a block writes kJoinRows rows.
+constexpr int kJoinRows = 8;
+template <int NT, typename OUT>
+__global__ void __launch_bounds__(256) join_pieces_kernel(const __grid_constant__ TcArgs a, OUT *__restrict__ out) {
+  griddep_launch();
+  griddep_wait();
+  const int K = a.plan.K, n_tiles = (a.d_in + NT - 1) / NT, per = (a.d_out + BM - 1) / BM * n_tiles;
+  const int u = blockIdx.x / per, tile = blockIdx.x % per;
+  if (u >= __ldg(a.pieces.joined + K)) return;
+  int lo = 0, hi = K;  // the expert that u experts with pieces to join come before
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(a.pieces.joined + mid) <= u) lo = mid; else hi = mid;
+  }
+  const int first = __ldg(a.pieces.slot + lo), n = __ldg(a.pieces.slot + lo + 1) - first;
+  const int m0 = tile / n_tiles * BM + blockIdx.y * kJoinRows, n0 = tile % n_tiles * NT;
+  for (int i = threadIdx.x; i < kJoinRows * (NT / 4); i += 256) {
+    const int r = i / (NT / 4), c = i % (NT / 4) * 4, o = m0 + r, col = n0 + c;
+    if (o >= a.d_out || col >= a.d_in) continue;
+    const float *from = a.pieces.tiles + (int64_t)(blockIdx.y * kJoinRows + r) * NT + c;
+    float f[4] = {};
+    for (int q = 0; q < n; ++q) {
+      const int s = min((first + q) * per + tile, a.pieces.slots - 1);
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(from + (int64_t)s * BM * NT));
+      f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+    OUT *to = out + ((int64_t)lo * a.d_out + o) * a.d_in + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + k < a.d_in) to[k] = from_f32<OUT>(f[k]);
   }
 }
 
@@ -520,7 +660,7 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const T *__restrict__
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
     const T *p = src + r * cols + c;
-    uint16_t h[PLANES][8];
+    alignas(16) uint16_t h[PLANES][8];
     if constexpr (PLANES == 3) {
       float v[8];
       if (cols % 4 == 0 && c + 8 <= cols) {
@@ -541,6 +681,8 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const T *__restrict__
         h[1][k] = __bfloat16_as_ushort(b1);
         h[2][k] = __bfloat16_as_ushort(b2);
       }
+    } else if (cols % 8 == 0) {
+      *reinterpret_cast<uint4 *>(h[0]) = __ldg(reinterpret_cast<const uint4 *>(p));
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) h[0][k] = c + k < cols ? reinterpret_cast<const uint16_t *>(p)[k] : (uint16_t)0;
@@ -611,9 +753,25 @@ int operand(Operand *o, const void *src, int dtype, int64_t rows, int cols, uint
   return FGMM_OK;
 }
 
+// The pieces' division: none where every SM has three whole tiles; else a third of an SM's share at most, and four stages at
+// least.  (With pieces, their plan and their join 512 tiles of up to 16 stages took 100 us instead of 60.)  A slot count
+// that holds those of every routing: an expert of n > most >= 4 stages has at most 2 n / most pieces, and n is at most 5 / 4 of its rows / KCH.
+struct PieceSizes {
+  int64_t per, most, slots;
+};
+PieceSizes piece_sizes(int64_t R, int K, int d_in, int d_out, int NT) {
+  PieceSizes z;
+  z.per = cdiv(d_out, BM) * cdiv(d_in, NT);
+  z.most = K * z.per >= 3 * num_sms() ? INT32_MAX / 2 : std::max<int64_t>(4, cdiv((cdiv(R, KCH) + K) * z.per, 3 * num_sms()));
+  z.slots = cdiv(R, KCH) <= z.most ? 1 : (cdiv(5 * cdiv(R, KCH), 2 * z.most) + 1) * z.per;
+  return z;
+}
+// Columns of a tile of DW.
+int weights_tile(int dtype, int d_in) { return dtype == FGMM_F32 || d_in <= 128 ? 128 : 256; }
+
 template <int MODE, int NT, bool SPLIT, typename OUT>
 int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
-           cudaStream_t st) {
+           void *pieces, cudaStream_t st) {
   using Sh = Shape<NT, SPLIT>;
   const int bf16 = dtype != FGMM_F16, width = MODE == kForward ? d_out : d_in;
   CUtensorMap ma{}, mb{};
@@ -646,21 +804,42 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
     FGMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(kMaxExperts)));
     if (dev < 64) done[dev].store(true, std::memory_order_release);
   }
-  const int64_t m_tiles = MODE == kWeights ? (int64_t)p.K * cdiv(d_out, BM) : cdiv(p.R, BM) + std::min<int64_t>(p.K, p.R);
-  const int64_t tiles = m_tiles * cdiv(width, NT);
-  if (tiles > INT32_MAX / 2) return fail(FGMM_ERR_UNSUPPORTED, "more than 2^30 tiles");
+  if (MODE == kWeights) {
+    const PieceSizes z = piece_sizes(p.R, p.K, d_in, d_out, NT);
+    if ((cdiv(p.R, KCH) + p.K) * z.per > INT32_MAX) return fail(FGMM_ERR_UNSUPPORTED, "more than 2^31 stages of the weights' gradient");
+    Carve c(pieces);
+    int *first = c.take<int>(p.K + 1), *slot = c.take<int>(p.K + 1), *joined = c.take<int>(p.K + 1);
+    a.pieces = {first, slot, joined, c.take<float>(z.slots * BM * NT), (int)z.most, (int)z.slots};
+    if (z.slots > 1)
+      FGMM_CUDA_TRY(launch_pdl(plan_pieces_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, (int)z.most, first, slot, joined));
+    FGMM_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(num_sms(), (cdiv(p.R, KCH * z.most) + p.K) * z.per)), dim3(kThreads),
+                             Sh::smem(p.K), st, ma, mb, a, out));
+    if (z.slots > 1)
+      FGMM_CUDA_TRY(launch_pdl(join_pieces_kernel<NT, OUT>, dim3((unsigned)(z.slots / 2), BM / kJoinRows), dim3(256), 0, st, a, out));
+    return FGMM_OK;
+  }
+  const int64_t tiles = (cdiv(p.R, BM) + std::min<int64_t>(p.K, p.R)) * cdiv(width, NT);  // at most
+  if (tiles > INT32_MAX) return fail(FGMM_ERR_UNSUPPORTED, "more than 2^31 tiles");
   FGMM_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(tiles, num_sms())), dim3(kThreads), Sh::smem(p.K), st, ma, mb, a, out));
   return FGMM_OK;
 }
 
-// Columns of a tile: 256 where every SM gets two such tiles, else 128.
+// Columns of a tile: 256 where every SM gets two such tiles (of Y and DX; DW is divided evenly anyway), else 128.
 template <int MODE, typename OUT>
 int launch16(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
-             cudaStream_t st) {
+             void *pieces, cudaStream_t st) {
   const int width = MODE == kForward ? d_out : d_in;
-  const int64_t m_tiles = MODE == kWeights ? (int64_t)p.K * cdiv(d_out, BM) : cdiv(p.R, BM);
-  if (width > 128 && m_tiles * cdiv(width, 256) >= 2 * num_sms()) return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, st);
-  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, st);
+  if (MODE == kWeights ? weights_tile(dtype, d_in) == 256 : width > 128 && cdiv(p.R, BM) * cdiv(width, 256) >= 2 * num_sms())
+    return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
+  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
+}
+
+size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
+  const int NT = weights_tile(dtype, d_in);
+  Carve c(nullptr);
+  for (int i = 0; i < 3; ++i) c.take<int>(K + 1);
+  c.take<float>(piece_sizes(R, K, d_in, d_out, NT).slots * BM * NT);
+  return c.bytes();
 }
 
 }  // namespace
@@ -671,7 +850,10 @@ size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, i
   Carve c(nullptr);
   c.take<uint16_t>(copy_elems(dtype, N, d_in));
   c.take<uint16_t>(copy_elems(dtype, (int64_t)K * d_out, d_in));
-  if (backward) c.take<uint16_t>(copy_elems(dtype, N * top_k, d_out));
+  if (backward) {
+    c.take<uint16_t>(copy_elems(dtype, N * top_k, d_out));
+    c.take<char>(piece_bytes(dtype, N * top_k, K, d_in, d_out));
+  }
   return c.bytes() + 256;
 }
 
@@ -683,9 +865,9 @@ int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_i
   int rc = operand(&ox, x, dtype, N, d_in, cx, st);
   if (!rc) rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
   if (rc) return rc;
-  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, st);
-  if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, st);
-  return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, st);
+  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, st);
+  if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, st);
+  return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, nullptr, st);
 }
 
 int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
@@ -693,23 +875,24 @@ int products_tc_backward(const void *dy, const void *x, const void *weight, int 
   Carve c(ws);
   uint16_t *cx = c.take<uint16_t>(copy_elems(dtype, N, d_in)), *cw = c.take<uint16_t>(copy_elems(dtype, (int64_t)p.K * d_out, d_in));
   uint16_t *cg = c.take<uint16_t>(copy_elems(dtype, p.R, d_out));
+  char *pieces = c.take<char>(piece_bytes(dtype, p.R, p.K, d_in, d_out));
   Operand og;
   int rc = operand(&og, dy, dtype, p.R, d_out, cg, st);
   if (rc) return rc;
   if (dx_rows) {
     Operand ow;
     rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
-    if (!rc) rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, st)
-                                    : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, st);
+    if (!rc) rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st)
+                                    : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st);
     if (rc) return rc;
   }
   if (!d_weight) return FGMM_OK;
   Operand ox;
   rc = operand(&ox, x, dtype, N, d_in, cx, st);
   if (rc) return rc;
-  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, st);
-  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, st);
-  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, st);
+  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, pieces, st);
+  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, pieces, st);
+  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, pieces, st);
 }
 
 }  // namespace fgmm
