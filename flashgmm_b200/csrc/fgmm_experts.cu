@@ -16,26 +16,86 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // ----------------------------------------------------------------------------- grouping
 //
-// A stable counting sort of the R routes by expert (routes without one last): every block counts its
-// 2048 routes per key, the counts are summed over the blocks in order, and the same blocks place them.
-// A warp takes 256 routes in their order, 32 at a time; lanes with the same key find each other with one
-// match instruction.
-constexpr int kSortWarps = 8, kSortRounds = 8, kSortItems = kSortWarps * kSortRounds * 32;
+// A stable counting sort of the R routes by expert (routes without one last): every block counts its 4096 routes per key,
+// the counts are summed over the blocks in order, and the same blocks place them (524,288 routes over 1,024 experts: 30 us
+// with the counts key by key and 2,048 routes a block, whose place kernel waited for a line per key).  Up to 4096 routes
+// are one block's work and one launch.
+// A warp takes 256 routes in their order, 32 at a time; lanes with the same key find each other with one match
+// instruction.
+constexpr int kSortWarps = 16, kSortRounds = 8, kSortItems = kSortWarps * kSortRounds * 32, kSortThreads = kSortWarps * 32;
 
 __device__ __forceinline__ int route_key(const int32_t *indices, int64_t i, int K) {
   const int e = __ldg(indices + i);
   return e >= 0 && e < K ? e : K;
 }
 
-// Counts this block's routes per key into s_count[warp][key]; rank[r] is a route's place among those
-// of its key in its warp.
-__device__ __forceinline__ void count_keys(const int32_t *indices, int64_t R, int K, uint16_t *s_count,
-                                           int (&key)[kSortRounds], int (&rank)[kSortRounds]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, keys = K + 1;
+// counts[block][key]
+__global__ void __launch_bounds__(kSortThreads) group_count_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
+                                                                   int32_t *__restrict__ counts) {
+  extern __shared__ int s_hist[];
+  const int keys = K + 1;
+  for (int e = threadIdx.x; e < keys; e += kSortThreads) s_hist[e] = 0;
+  __syncthreads();
+  griddep_wait();
+  griddep_launch();  // after the wait: the place kernel reads the indices before its own
+  const int64_t base = (int64_t)blockIdx.x * kSortItems + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kSortItems / kSortThreads; ++i)
+    if (base + i * kSortThreads < R) atomicAdd(s_hist + route_key(indices, base + i * kSortThreads, K), 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < keys; e += kSortThreads) counts[(int64_t)blockIdx.x * keys + e] = s_hist[e];
+}
+
+// Exclusive sums over the blocks in place, and the keys' totals: 32 keys a block, 16 threads share a key's column.
+constexpr int kScanParts = 16;
+__global__ void __launch_bounds__(32 * kScanParts) group_scan_kernel(int32_t *__restrict__ counts, int K, int blocks,
+                                                                     int32_t *__restrict__ totals) {
+  __shared__ int s_part[kScanParts][32];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, keys = K + 1, e = blockIdx.x * 32 + lane;
+  const int per = (blocks + kScanParts - 1) / kScanParts, b0 = part * per, b1 = min(blocks, b0 + per);
+  griddep_wait();
+  griddep_launch();
+  int sum = 0;
+  if (e < keys) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += counts[(int64_t)b * keys + e];
+  }
+  s_part[part][lane] = sum;
+  __syncthreads();
+  if (e >= keys) return;
+  int run = 0, total = 0;
+#pragma unroll
+  for (int q = 0; q < kScanParts; ++q) {
+    if (q < part) run += s_part[q][lane];
+    total += s_part[q][lane];
+  }
+  if (part == 0) totals[e] = total;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) {
+    int32_t *c = counts + (int64_t)b * keys + e;
+    const int n = *c;
+    *c = run;
+    run += n;
+  }
+}
+
+// Places this block's routes; with ONE it is the only block and its own counts are the totals.
+template <bool ONE>
+__global__ void __launch_bounds__(kSortThreads) group_place_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
+                                                                   const int32_t *__restrict__ counts, const int32_t *__restrict__ totals,
+                                                                   int32_t *__restrict__ order, int32_t *__restrict__ offsets,
+                                                                   int32_t *__restrict__ position) {
+  extern __shared__ uint16_t s_count[];  // [warp][keys]: routes of a key in the warps before, then places
+  const int keys = K + 1;
+  int32_t *s_start = reinterpret_cast<int32_t *>(s_count + kSortWarps * keys);  // [keys]
+  __shared__ int s_warp[kSortWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t *mine = s_count + warp * keys;
-  for (int i = threadIdx.x; i < kSortWarps * keys; i += blockDim.x) s_count[i] = 0;
+  for (int i = threadIdx.x; i < kSortWarps * keys / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(s_count)[i] = 0u;
+  if (ONE) griddep_wait();
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kSortItems + warp * kSortRounds * 32 + lane;
+  int key[kSortRounds], rank[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) key[r] = base + r * 32 < R ? route_key(indices, base + r * 32, K) : -1;
 #pragma unroll
@@ -49,82 +109,8 @@ __device__ __forceinline__ void count_keys(const int32_t *indices, int64_t R, in
     rank[r] = seen + below;
   }
   __syncthreads();
-}
-
-// counts[key][block]
-__global__ void __launch_bounds__(kSortWarps * 32) group_count_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
-                                                                      int blocks, int32_t *__restrict__ counts) {
-  extern __shared__ uint16_t s_count[];
-  int key[kSortRounds], rank[kSortRounds];
-  count_keys(indices, R, K, s_count, key, rank);
-  for (int e = threadIdx.x; e <= K; e += blockDim.x) {
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) n += s_count[w * (K + 1) + e];
-    counts[(int64_t)e * blocks + blockIdx.x] = n;
-  }
-}
-
-// A warp per key: exclusive sums over the blocks in place, and the key's total.
-__global__ void __launch_bounds__(128) group_scan_kernel(int32_t *__restrict__ counts, int K, int blocks,
-                                                         int32_t *__restrict__ totals) {
-  const int e = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (e > K) return;
-  int32_t *c = counts + (int64_t)e * blocks;
-  int run = 0;
-  for (int b0 = 0; b0 < blocks; b0 += 32) {
-    const int n = b0 + lane < blocks ? c[b0 + lane] : 0;
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFull, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (b0 + lane < blocks) c[b0 + lane] = run + sum - n;
-    run += __shfl_sync(kFull, sum, 31);
-  }
-  if (lane == 0) totals[e] = run;
-}
-
-__global__ void __launch_bounds__(kSortWarps * 32) group_place_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
-                                                                      int blocks, const int32_t *__restrict__ counts,
-                                                                      const int32_t *__restrict__ totals,
-                                                                      int32_t *__restrict__ order, int32_t *__restrict__ offsets,
-                                                                      int32_t *__restrict__ position) {
-  extern __shared__ uint16_t s_count[];
-  const int keys = K + 1;
-  int32_t *s_start = reinterpret_cast<int32_t *>(s_count + kSortWarps * keys);  // [keys]
-  __shared__ int s_warp[kSortWarps];
-  __shared__ int s_run;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int key[kSortRounds], rank[kSortRounds];
-  count_keys(indices, R, K, s_count, key, rank);
-  // where each key's routes begin: exclusive sums of the totals
-  if (threadIdx.x == 0) s_run = 0;
-  __syncthreads();
-  for (int e0 = 0; e0 < keys; e0 += blockDim.x) {
-    const int e = e0 + threadIdx.x;
-    const int n = e < keys ? __ldg(totals + e) : 0;
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFull, sum, o);
-      if (lane >= o) sum += v;
-    }
-    if (lane == 31) s_warp[warp] = sum;
-    __syncthreads();
-    int start = s_run + sum - n;
-    for (int w = 0; w < warp; ++w) start += s_warp[w];
-    if (e < keys) {
-      if (blockIdx.x == 0) offsets[e] = start;
-      s_start[e] = start + __ldg(counts + (int64_t)e * blocks + blockIdx.x);
-    }
-    __syncthreads();
-    if (threadIdx.x == blockDim.x - 1) s_run = start + n;
-    __syncthreads();
-  }
-  // the warps before this one
-  for (int e = threadIdx.x; e < keys; e += blockDim.x) {
+  // per key: the warps before each, and (ONE) the total
+  for (int e = threadIdx.x; e < keys; e += kSortThreads) {
     int run = 0;
 #pragma unroll
     for (int w = 0; w < kSortWarps; ++w) {
@@ -132,13 +118,40 @@ __global__ void __launch_bounds__(kSortWarps * 32) group_place_kernel(const int3
       s_count[w * keys + e] = (uint16_t)run;
       run += n;
     }
+    if (ONE) s_start[e] = run;
+  }
+  if (ONE) __syncthreads();
+  else griddep_wait();
+  griddep_launch();
+  // where each key's routes begin: exclusive sums of the totals, a run of neighbouring keys a thread
+  const int per = (keys + kSortThreads - 1) / kSortThreads, e0 = min(keys, (int)threadIdx.x * per), e1 = min(keys, e0 + per);
+  int sum = 0;
+  for (int e = e0; e < e1; ++e) sum += ONE ? s_start[e] : __ldg(totals + e);
+  int end = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kFull, end, o);
+    if (lane >= o) end += v;
+  }
+  if (lane == 31) s_warp[warp] = end;
+  __syncthreads();
+  int start = end - sum;
+  for (int w = 0; w < warp; ++w) start += s_warp[w];
+  for (int e = e0; e < e1; ++e) {
+    const int n = ONE ? s_start[e] : __ldg(totals + e);
+    if (blockIdx.x == 0) offsets[e] = start;
+    s_start[e] = start;
+    start += n;
   }
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortItems + warp * kSortRounds * 32 + lane;
+  if (!ONE) {
+    for (int e = threadIdx.x; e < keys; e += kSortThreads) s_start[e] += __ldg(counts + (int64_t)blockIdx.x * keys + e);
+    __syncthreads();
+  }
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     if (key[r] < 0) continue;
-    const int at = s_start[key[r]] + s_count[warp * keys + key[r]] + rank[r];
+    const int at = s_start[key[r]] + mine[key[r]] + rank[r];
     order[at] = (int32_t)(base + r * 32);
     position[base + r * 32] = key[r] < K ? at : -1;
   }
@@ -172,7 +185,7 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
 template <typename TY, typename T, int V>
 __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
                                                       const int32_t *__restrict__ position, int64_t N, int top_k, int tpr,
-                                                      T *__restrict__ out) {
+                                                      int parts, T *__restrict__ out) {
   const int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   if (n >= N) return;
   for (int c = (threadIdx.x % tpr) * V; c < d; c += tpr * V) {
@@ -181,10 +194,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, 
       const int p = __ldg(position + n * top_k + j);
       if (p < 0 || p >= R) continue;
       const float w = weights ? __ldg(weights + n * top_k + j) : 1.0f;
-      float f[V];
-      load_pack<TY, V>(y + (int64_t)p * d + c, f);
+      for (int q = 0; q < parts; ++q) {
+        float f[V];
+        load_pack<TY, V>(y + (q * R + p) * d + c, f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
+      }
     }
     store_pack<T, V>(out + n * d + c, acc);
   }
@@ -221,14 +236,14 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
 }
 
 template <typename TY, typename T>
-int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st) {
+int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st, int parts = 1) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   int tpr = 1;
   while (tpr < 256 && tpr * (vec ? V : 1) < d) tpr *= 2;
   const unsigned grid = (unsigned)cdiv(N, 256 / tpr);
-  if (vec) combine_kernel<TY, T, V><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
-  else combine_kernel<TY, T, 1><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, out);
+  if (vec) combine_kernel<TY, T, V><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
+  else combine_kernel<TY, T, 1><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
   FGMM_LAUNCH_CHECK("combine_kernel");
   return FGMM_OK;
 }
@@ -251,7 +266,7 @@ static int sort_blocks(int64_t R) { return (int)std::max<int64_t>(1, cdiv(R, kSo
 
 size_t group_workspace_bytes(int64_t R, int K) {
   Carve c(nullptr);
-  c.take<int32_t>((size_t)(K + 1) * sort_blocks(R));
+  c.take<int32_t>(sort_blocks(R) > 1 ? (size_t)(K + 1) * sort_blocks(R) : 0);
   c.take<int32_t>(K + 1);
   return c.bytes();
 }
@@ -260,21 +275,24 @@ int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32
                  int32_t *position, void *ws, cudaStream_t st) {
   const int blocks = sort_blocks(R), keys = K + 1;
   Carve c(ws);
-  int32_t *counts = c.take<int32_t>((size_t)keys * blocks), *totals = c.take<int32_t>(keys);
-  const size_t smem = (size_t)kSortWarps * keys * sizeof(uint16_t), smem_place = smem + (size_t)keys * sizeof(int32_t);
+  int32_t *counts = c.take<int32_t>(blocks > 1 ? (size_t)keys * blocks : 0), *totals = c.take<int32_t>(keys);
+  auto place_smem = [](int n) { return align_up((size_t)kSortWarps * n * sizeof(uint16_t), 4) + (size_t)n * sizeof(int32_t); };
   std::atomic<bool> &once = device_once_flag(8);
   if (!once.load(std::memory_order_acquire)) {
-    const int most = (kMaxExperts + 1) * (kSortWarps * 2 + 4);
-    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    const int most = (int)place_smem(kMaxExperts + 1);
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     once.store(true, std::memory_order_release);
   }
-  group_count_kernel<<<blocks, kSortWarps * 32, smem, st>>>(indices, R, K, blocks, counts);
-  FGMM_LAUNCH_CHECK("group_count_kernel");
-  group_scan_kernel<<<(unsigned)cdiv(keys, 4), 128, 0, st>>>(counts, K, blocks, totals);
-  FGMM_LAUNCH_CHECK("group_scan_kernel");
-  group_place_kernel<<<blocks, kSortWarps * 32, smem_place, st>>>(indices, R, K, blocks, counts, totals, order, offsets, position);
-  FGMM_LAUNCH_CHECK("group_place_kernel");
+  if (blocks == 1) {
+    FGMM_CUDA_TRY(launch_pdl(group_place_kernel<true>, dim3(1), dim3(kSortThreads), place_smem(keys), st, indices, R, K,
+                             (const int32_t *)nullptr, (const int32_t *)nullptr, order, offsets, position));
+    return FGMM_OK;
+  }
+  FGMM_CUDA_TRY(launch_pdl(group_count_kernel, dim3(blocks), dim3(kSortThreads), keys * sizeof(int), st, indices, R, K, counts));
+  FGMM_CUDA_TRY(launch_pdl(group_scan_kernel, dim3((unsigned)cdiv(keys, 32)), dim3(32 * kScanParts), 0, st, counts, K, blocks, totals));
+  FGMM_CUDA_TRY(launch_pdl(group_place_kernel<false>, dim3(blocks), dim3(kSortThreads), place_smem(keys), st, indices, R, K, counts, totals,
+                           order, offsets, position));
   return FGMM_OK;
 }
 
@@ -285,11 +303,11 @@ int combine_forward(const void *y, int dtype, int64_t R, int d, const float *wei
   return combine_forward_t((const __half *)y, R, d, weights, position, N, top_k, (__half *)out, st);
 }
 
-int sum_rows(const float *rows, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
+int sum_rows(const float *rows, int parts, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
              cudaStream_t st) {
-  if (dtype == FGMM_F32) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (float *)out, st);
-  if (dtype == FGMM_BF16) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__nv_bfloat16 *)out, st);
-  return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__half *)out, st);
+  if (dtype == FGMM_F32) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (float *)out, st, parts);
+  if (dtype == FGMM_BF16) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__nv_bfloat16 *)out, st, parts);
+  return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__half *)out, st, parts);
 }
 
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,

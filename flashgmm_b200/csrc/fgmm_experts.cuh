@@ -59,18 +59,28 @@ int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32
 // out[n] = sum_j w[n][j] y[position[n][j]], positions outside [0, R) skipped.
 int combine_forward(const void *y, int dtype, int64_t R, int d, const float *weights,
                     const int32_t *position, int64_t N, int top_k, void *out, cudaStream_t st);
-// The same of fp32 rows with weights 1.
-int sum_rows(const float *rows, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
+// The same of fp32 rows[parts][R][d] with weights 1, summed over the parts.
+int sum_rows(const float *rows, int parts, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
              cudaStream_t st);
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,
                      const RoutePlan &plan, void *dy, float *d_weights, cudaStream_t st);
 
-// ---- fgmm_experts_tc.cu ----
-size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, bool backward);
+// ---- fgmm_experts_few.cu: CUDA-core products for a few rows an expert ----
+int products_few(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y, cudaStream_t st);
+int few_dx_parts(int64_t R, int K, int d_in, int d_out);  // dx_rows there: [parts][R][d_in]
+int products_few_dx(const void *dy, const void *weight, int dtype, int d_in, int d_out, const RoutePlan &p, float *dx_rows, cudaStream_t st);
+int products_few_dw(const void *dy, const void *x, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *d_weight, cudaStream_t st);
+
+// ---- fgmm_experts_tc.cu: tensor-core products ----
+// Which of the three products run there; the others cost no workspace.
+struct TcParts {
+  bool forward, inputs, weights;
+};
+size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, const TcParts &parts);
 int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y,
                 void *ws, cudaStream_t st);
-// dx_rows[R][d_in] and d_weight, either may be null.
+// dx_rows[R][d_in] and d_weight, as parts says.
 int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
-                         const RoutePlan &p, float *dx_rows, void *d_weight, void *ws, cudaStream_t st);
+                         const RoutePlan &p, float *dx_rows, void *d_weight, const TcParts &parts, void *ws, cudaStream_t st);
 
 }  // namespace fgmm

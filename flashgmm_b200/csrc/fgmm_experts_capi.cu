@@ -25,6 +25,26 @@ int check_widths(int d_in, int d_out) {
   return FGMM_OK;
 }
 
+// Which products run on the tensor cores.  The CUDA-core products read float32 weights, and 16-bit ones with rows of no multiple of
+// 16 bytes, as they are, and write the gradients of experts without a row straight.
+// Rows an expert, on average, up to which they are faster; us at 64 experts of 512 x 1,024, CUDA cores / tensor cores:
+//   rows          0.25      1         2          4          8           16
+//   y  float32    9 / 77    16 / 89   28 / 90    43 / 102   66 / 104    103 / 115
+//   dx float32    19 / 89   28 / 89   49 / 91    82 / 113   128 / 114
+//   dW float32    25 / 51   29 / 53   35 / 54    44 / 60    66 / 62
+//   dW bf16       15 / 26   19 / 27   27 / 27    28 / 27
+// and at 16 rows of 509 x 1,024 bf16: y 154 / 55, dx 196 / 54, dW 112 / 101.
+TcParts on_tensor_cores(int dtype, int64_t R, int K, int d_in, int d_out) {
+  const bool f32 = dtype == FGMM_F32, in_copied = f32 || d_in % 8 != 0, out_copied = in_copied || d_out % 8 != 0;
+  const auto few = [&](int rows) { return R <= (int64_t)rows * K; };
+  return {!(in_copied && few(f32 ? 16 : 4)), !(out_copied && few(f32 ? 6 : 4)), !few(out_copied ? 6 : 1)};
+}
+
+// dx_rows: one matrix, or the parts of the CUDA-core product.
+size_t dx_rows_bytes(const TcParts &tc, int64_t R, int K, int d_in, int d_out) {
+  return align_up((size_t)R * d_in * sizeof(float) * (tc.inputs ? 1 : few_dx_parts(R, K, d_in, d_out)), 256);
+}
+
 int check_route(int dtype, int64_t N, int K, int64_t row_stride, int top_k, int func) {
   int rc = check_experts(dtype, N, K, top_k);
   if (rc) return rc;
@@ -98,7 +118,8 @@ int fgmm_group_routes(const int32_t *indices, int64_t R, int32_t K, int32_t *ord
 size_t fgmm_expert_products_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                             int32_t d_out, int32_t top_k) {
   if (check_experts(dtype, N, K, top_k) || check_widths(d_in, d_out)) return 0;
-  return products_tc_workspace(dtype, N, K, d_in, d_out, top_k, false);
+  const TcParts tc = on_tensor_cores(dtype, N * top_k, K, d_in, d_out);
+  return tc.forward ? products_tc_workspace(dtype, N, K, d_in, d_out, top_k, {true, false, false}) : 256;
 }
 
 int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, const void *weight,
@@ -114,13 +135,17 @@ int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, 
   if (workspace_bytes < fgmm_expert_products_workspace_bytes(dtype, N, K, d_in, d_out, top_k))
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
+  if (!on_tensor_cores(dtype, plan.R, K, d_in, d_out).forward)
+    return products_few(x, weight, dtype, N, d_in, d_out, plan, y, (cudaStream_t)stream);
   return products_tc(x, weight, dtype, N, d_in, d_out, plan, y, workspace, (cudaStream_t)stream);
 }
 
 size_t fgmm_expert_products_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                                      int32_t d_out, int32_t top_k) {
   if (check_experts(dtype, N, K, top_k) || check_widths(d_in, d_out)) return 0;
-  return products_tc_workspace(dtype, N, K, d_in, d_out, top_k, true) + align_up((size_t)N * top_k * d_in * sizeof(float), 256);
+  TcParts tc = on_tensor_cores(dtype, N * top_k, K, d_in, d_out);
+  tc.forward = false;
+  return products_tc_workspace(dtype, N, K, d_in, d_out, top_k, tc) + dx_rows_bytes(tc, N * top_k, K, d_in, d_out);
 }
 
 int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, int64_t N, int32_t d_in,
@@ -146,11 +171,19 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
   // the rows of dx first, in fp32: their sum over a point's slots rounds once
-  float *dx_rows = dx ? static_cast<float *>(workspace) : nullptr;
-  void *rest = static_cast<char *>(workspace) + align_up((size_t)plan.R * d_in * sizeof(float), 256);
-  rc = products_tc_backward(dy, x, weight, dtype, N, d_in, d_out, plan, dx_rows, d_weight, rest, st);
+  TcParts tc = on_tensor_cores(dtype, plan.R, K, d_in, d_out);
+  tc.forward = false;
+  float *dx_rows = static_cast<float *>(workspace);
+  void *rest = static_cast<char *>(workspace) + dx_rows_bytes(tc, plan.R, K, d_in, d_out);
+  const int parts = tc.inputs ? 1 : few_dx_parts(plan.R, K, d_in, d_out);
+  if (dx && !tc.inputs) rc = products_few_dx(dy, weight, dtype, d_in, d_out, plan, dx_rows, st);
+  if (!rc && d_weight && !tc.weights) rc = products_few_dw(dy, x, dtype, N, d_in, d_out, plan, d_weight, st);
+  tc.inputs = tc.inputs && dx;
+  tc.weights = tc.weights && d_weight;
+  if (!rc && (tc.inputs || tc.weights))
+    rc = products_tc_backward(dy, x, weight, dtype, N, d_in, d_out, plan, dx_rows, d_weight, tc, rest, st);
   if (rc || !dx) return rc;
-  return sum_rows(dx_rows, dtype, plan.R, d_in, position, N, top_k, dx, st);
+  return sum_rows(dx_rows, parts, dtype, plan.R, d_in, position, N, top_k, dx, st);
 }
 
 int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,

@@ -846,24 +846,35 @@ size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
 
 int experts_device_error(bool reset) { return read_dev_error(reset); }
 
-size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, bool backward) {
-  Carve c(nullptr);
-  c.take<uint16_t>(copy_elems(dtype, N, d_in));
-  c.take<uint16_t>(copy_elems(dtype, (int64_t)K * d_out, d_in));
-  if (backward) {
-    c.take<uint16_t>(copy_elems(dtype, N * top_k, d_out));
-    c.take<char>(piece_bytes(dtype, N * top_k, K, d_in, d_out));
-  }
-  return c.bytes() + 256;
+namespace {
+// The workspace: copies of the operands that TMA cannot read, and DW's pieces.
+struct TcSpace {
+  uint16_t *x, *weight, *dy;
+  char *pieces;
+  size_t bytes;
+};
+TcSpace tc_space(void *ws, int dtype, int64_t N, int K, int d_in, int d_out, int top_k, const TcParts &parts) {
+  Carve c(ws);
+  TcSpace s;
+  s.x = c.take<uint16_t>(parts.forward || parts.weights ? copy_elems(dtype, N, d_in) : 0);
+  s.weight = c.take<uint16_t>(parts.forward || parts.inputs ? copy_elems(dtype, (int64_t)K * d_out, d_in) : 0);
+  s.dy = c.take<uint16_t>(parts.inputs || parts.weights ? copy_elems(dtype, N * top_k, d_out) : 0);
+  s.pieces = c.take<char>(parts.weights ? piece_bytes(dtype, N * top_k, K, d_in, d_out) : 0);
+  s.bytes = c.bytes() + 256;
+  return s;
+}
+}  // namespace
+
+size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, int top_k, const TcParts &parts) {
+  return tc_space(nullptr, dtype, N, K, d_in, d_out, top_k, parts).bytes;
 }
 
 int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y,
                 void *ws, cudaStream_t st) {
-  Carve c(ws);
-  uint16_t *cx = c.take<uint16_t>(copy_elems(dtype, N, d_in)), *cw = c.take<uint16_t>(copy_elems(dtype, (int64_t)p.K * d_out, d_in));
+  const TcSpace s = tc_space(ws, dtype, N, p.K, d_in, d_out, p.top_k, {true, false, false});
   Operand ox, ow;
-  int rc = operand(&ox, x, dtype, N, d_in, cx, st);
-  if (!rc) rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
+  int rc = operand(&ox, x, dtype, N, d_in, s.x, st);
+  if (!rc) rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, st);
   if (rc) return rc;
   if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, st);
   if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, st);
@@ -871,28 +882,23 @@ int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_i
 }
 
 int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
-                         const RoutePlan &p, float *dx_rows, void *d_weight, void *ws, cudaStream_t st) {
-  Carve c(ws);
-  uint16_t *cx = c.take<uint16_t>(copy_elems(dtype, N, d_in)), *cw = c.take<uint16_t>(copy_elems(dtype, (int64_t)p.K * d_out, d_in));
-  uint16_t *cg = c.take<uint16_t>(copy_elems(dtype, p.R, d_out));
-  char *pieces = c.take<char>(piece_bytes(dtype, p.R, p.K, d_in, d_out));
-  Operand og;
-  int rc = operand(&og, dy, dtype, p.R, d_out, cg, st);
+                         const RoutePlan &p, float *dx_rows, void *d_weight, const TcParts &parts, void *ws, cudaStream_t st) {
+  const TcSpace s = tc_space(ws, dtype, N, p.K, d_in, d_out, p.top_k, parts);
+  Operand og, ow, ox;
+  int rc = operand(&og, dy, dtype, p.R, d_out, s.dy, st);
   if (rc) return rc;
-  if (dx_rows) {
-    Operand ow;
-    rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, cw, st);
+  if (parts.inputs) {
+    rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, st);
     if (!rc) rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st)
                                     : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st);
     if (rc) return rc;
   }
-  if (!d_weight) return FGMM_OK;
-  Operand ox;
-  rc = operand(&ox, x, dtype, N, d_in, cx, st);
+  if (!parts.weights) return FGMM_OK;
+  rc = operand(&ox, x, dtype, N, d_in, s.x, st);
   if (rc) return rc;
-  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, pieces, st);
-  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, pieces, st);
-  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, pieces, st);
+  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, st);
+  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, s.pieces, st);
+  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, s.pieces, st);
 }
 
 }  // namespace fgmm

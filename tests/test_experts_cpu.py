@@ -101,6 +101,13 @@ def test_products_refusals():
     assert backward(nb=back - 1) == 3
 
 
+def test_workspaces_of_no_points():
+    lib = _lib.load()
+    for dtype in (0, 1, 2):
+        assert lib.fgmm_expert_products_workspace_bytes(dtype, 0, 8, 32, 64, 2) > 0
+        assert lib.fgmm_expert_products_backward_workspace_bytes(dtype, 0, 8, 32, 64, 2) > 0
+
+
 def test_combine_refusals():
     lib = _lib.load()
     assert lib.fgmm_combine_experts(P, 5, 4, 8, P, P, 2, P, None) == 1
