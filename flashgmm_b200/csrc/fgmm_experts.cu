@@ -159,18 +159,20 @@ __global__ void __launch_bounds__(kSortThreads) group_place_kernel(const int32_t
 
 // ----------------------------------------------------------------------------- the join
 
-template <typename T, int V>
-__device__ __forceinline__ void load_pack(const T *p, float (&f)[V]) {
-  T raw[V];
+// V consecutive elements as they are in memory (16 bytes, or 32 of fp32 rows that become a 16-bit type; 1 element unaligned).
+template <typename T, int V> struct alignas(V * sizeof(T) >= 16 ? 16 : sizeof(T)) Pack {
+  T v[V];
+};
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_raw(const T *p) {
+  Pack<T, V> r;
   if constexpr (V * sizeof(T) >= 16) {
 #pragma unroll
     for (int i = 0; i < V * (int)sizeof(T) / 16; ++i)
-      reinterpret_cast<uint4 *>(raw)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+      reinterpret_cast<uint4 *>(&r)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
   } else {
-    raw[0] = __ldg(p);
+    r.v[0] = __ldg(p);
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = to_f32(raw[i]);
+  return r;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
@@ -181,32 +183,63 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
   else p[0] = raw[0];
 }
 
-// tpr threads share a point; each owns packs of columns.
-template <typename TY, typename T, int V>
+// tpr threads share a point; each owns packs of columns and adds the rows of J slots at a time, whose places are fetched a
+// point ahead and whose packs are on their way together.  PARTS: the rows are sums of `parts` matrices.
+template <typename TY, typename T, int V, int J, bool PARTS>
 __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
                                                       const int32_t *__restrict__ position, int64_t N, int top_k, int tpr,
                                                       int parts, T *__restrict__ out) {
-  const int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
-  if (n >= N) return;
-  for (int c = (threadIdx.x % tpr) * V; c < d; c += tpr * V) {
-    float acc[V] = {};
-    for (int j = 0; j < top_k; ++j) {
-      const int p = __ldg(position + n * top_k + j);
-      if (p < 0 || p >= R) continue;
-      const float w = weights ? __ldg(weights + n * top_k + j) : 1.0f;
-      for (int q = 0; q < parts; ++q) {
-        float f[V];
-        load_pack<TY, V>(y + (q * R + p) * d + c, f);
+  const int64_t stride = (int64_t)gridDim.x * (256 / tpr);
+  int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+  int p[J], ahead[J];
+  float w[J], w_ahead[J];
+  auto places = [&](int64_t n, int j0, int (&p)[J], float (&w)[J]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(w, f[i], acc[i]);
-      }
+    for (int j = 0; j < J; ++j) {
+      const bool slot = n < N && j0 + j < top_k;
+      p[j] = slot ? __ldg(position + n * top_k + j0 + j) : -1;
+      w[j] = slot && weights ? __ldg(weights + n * top_k + j0 + j) : 1.0f;
     }
-    store_pack<T, V>(out + n * d + c, acc);
+  };
+  places(n, 0, ahead, w_ahead);
+  for (; n < N; n += stride) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      p[j] = ahead[j];
+      w[j] = w_ahead[j];
+    }
+    places(n + stride, 0, ahead, w_ahead);
+    for (int c = (threadIdx.x % tpr) * V; c < d; c += tpr * V) {
+      float acc[V] = {};
+      for (int j0 = 0; j0 < top_k; j0 += J) {
+        if (top_k > J && (j0 > 0 || c >= tpr * V)) places(n, j0, p, w);
+        Pack<TY, V> f[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {  // (a slot without an expert reads row 0 and leaves it)
+          if (p[j] >= R) p[j] = -1;
+          f[j] = load_raw<TY, V>(y + (int64_t)max(p[j], 0) * d + c);
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = p[j] >= 0 ? fmaf(w[j], to_f32(f[j].v[i]), acc[i]) : acc[i];
+          if constexpr (PARTS) {
+            for (int q = 1; q < parts && p[j] >= 0; ++q) {
+              const Pack<TY, V> u = load_raw<TY, V>(y + (q * R + p[j]) * d + c);
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[i] = fmaf(w[j], to_f32(u.v[i]), acc[i]);
+            }
+          }
+        }
+      }
+      store_pack<T, V>(out + n * d + c, acc);
+    }
   }
 }
 
-// A warp per grouped row r of route order[r]: dy[r] = w dout[point], dw = <dout[point], y[r]>.
-template <typename T, int V>
+// A warp per grouped row r of route order[r]: dy[r] = w dout[point], dw = <dout[point], y[r]>; U packs of both rows
+// are on their way at once.
+template <typename T, int V, int U>
 __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restrict__ d_out, const T *__restrict__ y, int d,
                                                                const float *__restrict__ weights, RoutePlan p,
                                                                T *__restrict__ dy, float *__restrict__ d_weights) {
@@ -215,23 +248,39 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
   if (r >= p.R) return;
   const int id = __ldg(p.order + r);
   const bool known = id >= 0 && id < p.R, live = known && r < __ldg(p.offsets + p.K);
-  const float w = live ? __ldg(weights + id) : 0.0f;
-  const T *g = d_out + (int64_t)(live ? id / p.top_k : 0) * d, *yr = y + r * d;
+  T *to = dy + r * d;
   float dot = 0.0f;
-  for (int c = lane * V; c < d; c += 32 * V) {
-    float f[V] = {}, o[V];
-    if (live) {
-      float u[V];
-      load_pack<T, V>(g + c, f);
-      load_pack<T, V>(yr + c, u);
+  if (live) {
+    const float w = __ldg(weights + id);
+    const T *g = d_out + (int64_t)(id / p.top_k) * d, *yr = y + r * d;
+    for (int c0 = lane * V; c0 < d; c0 += U * 32 * V) {
+      Pack<T, V> f[U], u[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) dot = fmaf(f[i], u[i], dot);
+      for (int q = 0; q < U; ++q) {  // (behind the row: its first pack again, left unused)
+        const int c = c0 + q * 32 * V < d ? c0 + q * 32 * V : c0;
+        f[q] = load_raw<T, V>(g + c);
+        u[q] = load_raw<T, V>(yr + c);
+      }
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        const int c = c0 + q * 32 * V;
+        if (c < d) {
+          float o[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            o[i] = to_f32(f[q].v[i]);
+            dot = fmaf(o[i], to_f32(u[q].v[i]), dot);
+            o[i] *= w;
+          }
+          store_pack<T, V>(to + c, o);
+        }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = live ? w * f[i] : 0.0f;
-    store_pack<T, V>(dy + r * d + c, o);
+    dot = warp_sum(dot);
+  } else {
+    const float zeros[V] = {};
+    for (int c = lane * V; c < d; c += 32 * V) store_pack<T, V>(to + c, zeros);
   }
-  dot = warp_sum(dot);
   if (lane == 0 && known) d_weights[id] = dot;
 }
 
@@ -241,9 +290,18 @@ int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   int tpr = 1;
   while (tpr < 256 && tpr * (vec ? V : 1) < d) tpr *= 2;
-  const unsigned grid = (unsigned)cdiv(N, 256 / tpr);
-  if (vec) combine_kernel<TY, T, V><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
-  else combine_kernel<TY, T, 1><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(N, 256 / tpr), 8 * num_sms());
+  auto run = [&](auto v, auto j, auto several) {
+    combine_kernel<TY, T, v(), j(), several()><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
+  };
+  auto by_slots = [&](auto v, auto several) {
+    // (elements one by one are bound by instructions, not by loads on their way: one slot after the other)
+    if (top_k == 1 || v() == 1) run(v, std::integral_constant<int, 1>{}, several);
+    else if (top_k == 2) run(v, std::integral_constant<int, 2>{}, several);
+    else run(v, std::integral_constant<int, 4>{}, several);
+  };
+  auto by_parts = [&](auto v) { parts == 1 ? by_slots(v, std::false_type{}) : by_slots(v, std::true_type{}); };
+  vec ? by_parts(std::integral_constant<int, V>{}) : by_parts(std::integral_constant<int, 1>{});
   FGMM_LAUNCH_CHECK("combine_kernel");
   return FGMM_OK;
 }
@@ -254,8 +312,10 @@ int combine_backward_t(const T *g, const T *y, int d, const float *w, const Rout
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(dy) % 16 == 0;
   const unsigned grid = (unsigned)cdiv(p.R, 4);
-  if (vec) combine_backward_kernel<T, V><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
-  else combine_backward_kernel<T, 1><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
+  if (!vec) combine_backward_kernel<T, 1, 4><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
+  else if (d <= 32 * V) combine_backward_kernel<T, V, 1><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
+  else if (d <= 64 * V) combine_backward_kernel<T, V, 2><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
+  else combine_backward_kernel<T, V, 4><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
   FGMM_LAUNCH_CHECK("combine_backward_kernel");
   return FGMM_OK;
 }

@@ -35,13 +35,20 @@ __device__ __forceinline__ float clean(float z) { return fminf(fmaxf(z, -INFINIT
 
 struct RouteArgs {
   int64_t N, stride;
-  int K, top_k, func, n_groups, top_groups;
+  int K, top_k, func, n_groups, top_groups, per;  // per: experts of a group
   const float *bias;
   bool renorm;
   float scale;
 };
 
 template <typename T> __device__ __forceinline__ float score_at(const T *row, int c) { return clean(to_f32(row[c])); }
+
+// 1 / (1 + e^-z) to a few 2^-23 of itself.
+__device__ __forceinline__ float sigmoid(float z) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-z)));
+  return r;
+}
 
 // (v, i) comes before (w, j): a larger value, or an equal one of a lower index.
 __device__ __forceinline__ bool before(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
@@ -51,7 +58,7 @@ __device__ __forceinline__ bool before(double v, int i, double w, int j) { retur
 // registers for them would halve the occupancy of the rows that do not come here.
 template <typename T, int COLS>
 __device__ __noinline__ int route_row64(const T *row, const RouteArgs &a) {
-  const int lane = threadIdx.x & 31, per = a.K / a.n_groups, n = (a.K - lane + 31) / 32;
+  const int lane = threadIdx.x & 31, per = a.per, n = (a.K - lane + 31) / 32;
   double v[COLS];
 #pragma unroll 1
   for (int i = 0; i < n; ++i) v[i] = (double)score_at(row, lane + 32 * i);
@@ -198,7 +205,7 @@ template <int L> __device__ __forceinline__ float chosen_share(float z, bool liv
     float m = seg_max<L>(live ? z : -INFINITY);
     if (m == -INFINITY) m = 0.0f;
     if (func == FGMM_SCORE_SOFTMAX) t = live ? expf(z - m) : 0.0f;
-    else t = live ? expf(fminf(z, 0.0f) - fminf(m, 0.0f)) / (1.0f + expf(-fabsf(z))) : 0.0f;
+    else t = live ? __fdividef(expf(fminf(z, 0.0f) - fminf(m, 0.0f)), 1.0f + expf(-fabsf(z))) : 0.0f;
   }
   sum = seg_sum<L>(t);
   return sum == 0.0f ? 0.0f : t / sum;
@@ -209,12 +216,19 @@ __device__ __forceinline__ void top_two(float &b1, float &b2, float v1, float v2
   b1 = fmaxf(b1, v1);
 }
 
-// Masks all but the top_groups groups of a row.  False where the sums that decide lie too close.
-template <int VPT, int V, int L>
-__device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a, int l, float bmax, float tol, float *s_group) {
-  const int per = a.K / a.n_groups, span = per / V;
+// Masks all but the top_groups groups of a warp's row.  False where the sums that decide lie too close.
+template <int VPT, int V>
+__device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a, int lane, float bmax, float tol, float2 *s_group) {
+  const int per = a.per, span = per / V;
   // a group is `span` neighbouring lanes of one pack of V: all groups' best two meet in log2 span steps
-  const bool even = per % V == 0 && span <= L && (span & (span - 1)) == 0;
+  const bool even = per % V == 0 && span <= 32 && (span & (span - 1)) == 0;
+  const int shift = 31 - __clz(max(span, 1));  // lane >> shift: the lane's group within a pack
+  float2 mine = make_float2(-INFINITY, 0.0f);  // lane g: group g's sum, and the magnitudes in it
+  auto put = [&](int g, float b1, float b2) {
+    const bool two = b2 > -INFINITY;
+    // (a live group's sum stays above -inf; its magnitude then is inf, and the row is decided in 64 bits)
+    s_group[g] = make_float2(two ? fmaxf(b1 + b2, -FLT_MAX) : b1, fabsf(b1) + (two ? fabsf(b2) : 0.0f));
+  };
   __syncwarp();
   if (even) {
 #pragma unroll
@@ -223,59 +237,40 @@ __device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a,
 #pragma unroll
       for (int v = 1; v < V; ++v) top_two(b1, b2, c[i + v], -INFINITY);
       for (int o = 1; o < span; o <<= 1) top_two(b1, b2, __shfl_xor_sync(kFull, b1, o), __shfl_xor_sync(kFull, b2, o));
-      const int g = (i / V * L + l) / span;
-      if (l % span == 0 && g < a.n_groups) {
-        s_group[2 * g] = b2 > -INFINITY ? b1 + b2 : b1;
-        s_group[2 * g + 1] = fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.0f);
-      }
+      const int g = (i / V * 32 + lane) >> shift;
+      if ((lane & (span - 1)) == 0 && g < a.n_groups) put(g, b1, b2);
     }
   } else {
     for (int g = 0; g < a.n_groups; ++g) {
       float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int col = column<V, L>(i, l);
+        const int col = column<V, 32>(i, lane);
         top_two(b1, b2, col >= g * per && col < (g + 1) * per ? c[i] : -INFINITY, -INFINITY);
       }
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) top_two(b1, b2, __shfl_xor_sync(kFull, b1, o), __shfl_xor_sync(kFull, b2, o));
-      if (l == 0) {
-        s_group[2 * g] = b2 > -INFINITY ? b1 + b2 : b1;
-        s_group[2 * g + 1] = fabsf(b1) + (b2 > -INFINITY ? fabsf(b2) : 0.0f);
-      }
+      for (int o = 16; o > 0; o >>= 1) top_two(b1, b2, __shfl_xor_sync(kFull, b1, o), __shfl_xor_sync(kFull, b2, o));
+      if (lane == 0) put(g, b1, b2);
     }
   }
   __syncwarp();
-  // each lane ranks its groups against all; low and high: the smallest sum that stays, the largest that goes
-  uint32_t kept = 0;
-  float low = INFINITY, high = -INFINITY, most = 0.0f;
-  for (int g = l; g < a.n_groups; g += L) {
-    const float mine = s_group[2 * g];
-    int rank = 0;
-    for (int h = 0; h < a.n_groups; ++h) {
-      const float v = s_group[2 * h];
-      rank += v > mine || (v == mine && h < g);
-    }
-    const bool alive = mine > -INFINITY;
-    if (rank < a.top_groups) {
-      kept |= 1u << g;
-      if (alive) low = fminf(low, mine);
-    } else if (alive) {
-      high = fmaxf(high, mine);
-    }
-    if (alive) most = fmaxf(most, s_group[2 * g + 1]);
+  if (lane < a.n_groups) mine = s_group[lane];
+  // the groups that stay, one by one; low: the last one's sum
+  uint32_t key = mine.x > -INFINITY ? key_of(mine.x) : 0u, kept = 0u, low = 0u;
+  const float most = seg_max<32>(key ? mine.y : 0.0f);
+  for (int t = 0; t < a.top_groups; ++t) {
+    const uint32_t best = __reduce_max_sync(kFull, key);
+    if (best == 0u) break;
+    low = best;
+    const int g = __ffs(__ballot_sync(kFull, key == best)) - 1;
+    kept |= 1u << g;
+    if (lane == g) key = 0u;
   }
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    kept |= __shfl_xor_sync(kFull, kept, o);
-    low = fminf(low, __shfl_xor_sync(kFull, low, o));
-    high = fmaxf(high, __shfl_xor_sync(kFull, high, o));
-    most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-  }
+  const uint32_t high = __reduce_max_sync(kFull, key);  // the largest that goes
   if (even) {
 #pragma unroll
     for (int i = 0; i < VPT; i += V) {
-      if (!((kept >> ((i / V * L + l) / span & 31)) & 1u)) {  // (columns past K are masked already)
+      if (!((kept >> (((i / V * 32 + lane) >> shift) & 31)) & 1u)) {  // (columns past K are masked already)
 #pragma unroll
         for (int v = 0; v < V; ++v) c[i + v] = -INFINITY;
       }
@@ -283,9 +278,9 @@ __device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a,
   } else {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if (!((kept >> (column<V, L>(i, l) / per & 31)) & 1u)) c[i] = -INFINITY;
+      if (!((kept >> (column<V, 32>(i, lane) / per & 31)) & 1u)) c[i] = -INFINITY;
   }
-  return high == -INFINITY || low == INFINITY || low - high > 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
+  return high == 0u || of_key(low) - of_key(high) > 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
 }
 
 // The row's `rounds` largest values in order (lane j: the j'th, -1 where none is left): the lanes' best ones are compared,
@@ -365,6 +360,18 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     if (count > 32) return false;
   }
   __syncwarp();
+  if (VPT <= 8) {
+    int to = n;  // the lane's first place
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFull, to, o);
+      if (lane >= o) to += v;
+    }
+    to -= n;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if ((some[0] >> i) & 1u) s_cand[to++] = (uint64_t)key_of(clean(c[i])) << 32 | (uint32_t)column<V, 32>(i, lane);
+  } else
   for (int base = 0; base < count;) {
     int i = -1;
 #pragma unroll
@@ -446,13 +453,14 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
   if (by_value) {
     if (a.func == FGMM_SCORE_SIGMOID) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) c[i] = c[i] > -INFINITY ? __fdividef(1.0f, 1.0f + expf(-c[i])) : -INFINITY;
+      for (int i = 0; i < VPT; ++i) c[i] = c[i] > -INFINITY ? sigmoid(c[i]) : -INFINITY;
     }
     if (a.bias) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) c[i] = fmaxf(c[i] + s_bias[column<V, L>(i, l)], -INFINITY);  // -inf for NaN
     }
-    if (a.n_groups > 1) sure = keep_groups<VPT, V, L>(c, a, l, bmax, kTol, reinterpret_cast<float *>(s_cand));
+    if constexpr (L == 32)
+      if (a.n_groups > 1) sure = keep_groups<VPT, V>(c, a, l, bmax, kTol, reinterpret_cast<float2 *>(s_cand));
   }
   // one choice more than asked, where its distance from the last one is looked at
   const int rounds = min(L, by_value ? a.top_k + 1 : a.top_k);
@@ -464,7 +472,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
       float v = score_at(row, col);
       if (by_value) {
         if (a.func == FGMM_SCORE_SOFTMAX) v = expf(v - m) * inv;
-        else if (a.func == FGMM_SCORE_SIGMOID) v = __fdividef(1.0f, 1.0f + expf(-v));
+        else if (a.func == FGMM_SCORE_SIGMOID) v = sigmoid(v);
         if (a.bias) v += s_bias[col];
       }
       return v;
@@ -657,7 +665,7 @@ template <typename T, typename F> int by_row_width(int K, int slots, bool vec, F
 template <typename T>
 int route_forward_t(const T *z, const RouteArgs &a, float *w, int32_t *idx, cudaStream_t st) {
   const bool vec = reinterpret_cast<uintptr_t>(z) % 16 == 0 && a.stride * sizeof(T) % 16 == 0;
-  const int slots = a.top_k + (a.bias || a.n_groups > 1 ? 1 : 0);
+  const int slots = a.n_groups > 1 ? 32 : a.top_k + (a.bias ? 1 : 0);  // (groups are kept by whole warps)
   return by_row_width<T>(a.K, slots, vec, [&](auto vpt, auto v, auto lanes) {
     // every warp slot of the device once (64 warps an SM), so that the rows after the first are prefetched
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, kRouteWarps * (32 / lanes())), (int64_t)num_sms() * 64 / kRouteWarps);
@@ -685,7 +693,7 @@ int route_backward_t(const float *dw, const T *z, const int32_t *idx, const Rout
 int route_forward(const void *scores, int dtype, int64_t N, int K, int64_t stride, const float *bias,
                   int top_k, int func, int n_groups, int top_groups, bool renorm, float scale,
                   float *weights, int32_t *indices, cudaStream_t st) {
-  const RouteArgs a{N, stride, K, top_k, func, n_groups, top_groups, bias, renorm, scale};
+  const RouteArgs a{N, stride, K, top_k, func, n_groups, top_groups, K / n_groups, bias, renorm, scale};
   if (dtype == FGMM_F32) return route_forward_t((const float *)scores, a, weights, indices, st);
   if (dtype == FGMM_BF16) return route_forward_t((const __nv_bfloat16 *)scores, a, weights, indices, st);
   return route_forward_t((const __half *)scores, a, weights, indices, st);
@@ -694,7 +702,7 @@ int route_forward(const void *scores, int dtype, int64_t N, int K, int64_t strid
 int route_backward(const float *dw, const void *scores, int dtype, int64_t N, int K, int64_t stride,
                    const int32_t *indices, int top_k, int func, bool renorm, float scale, void *dz,
                    cudaStream_t st) {
-  const RouteArgs a{N, stride, K, top_k, func, 1, 1, nullptr, renorm, scale};
+  const RouteArgs a{N, stride, K, top_k, func, 1, 1, K, nullptr, renorm, scale};
   if (dtype == FGMM_F32) return route_backward_t(dw, (const float *)scores, indices, a, (float *)dz, st);
   if (dtype == FGMM_BF16) return route_backward_t(dw, (const __nv_bfloat16 *)scores, indices, a, (__nv_bfloat16 *)dz, st);
   return route_backward_t(dw, (const __half *)scores, indices, a, (__half *)dz, st);
