@@ -316,6 +316,9 @@ __device__ __forceinline__ void pick_by_lane(float (&c)[VPT], int rounds, int l,
   }
 }
 
+// (v, col) as a number that is larger where it comes first: a larger value, or an equal one of a lower column.
+__device__ __forceinline__ uint64_t ranked(float v, int col) { return (uint64_t)key_of(v) << 32 | ~(uint32_t)col; }
+
 // The same for a whole warp's row.  With bar the rounds'th largest of the lanes' maxima, what reaches bar is a handful, which
 // move to a lane each (through s_cand) and are picked in order.  Where many equal bar (responsibilities are mostly exact
 // zeros), only what is above it moves, and the slots that leaves are filled by index.  False where more than 32 are
@@ -327,13 +330,12 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
   for (int i = 1; i < VPT; ++i) most = fmaxf(most, c[i]);
   most = clean(most);
   uint32_t left = most > -INFINITY ? key_of(most) : 0u, best = 0u;
-  int r = 0;
-  for (; r < rounds; ++r) {  // (equal maxima are taken together: bar is that much lower)
+#pragma unroll 2
+  for (int r = 0; r < rounds; ++r) {  // (equal maxima are taken together: bar is that much lower)
     best = __reduce_max_sync(kFull, left);
-    if (best == 0u) break;
-    if (left == best) left = 0u;
+    left = left == best ? 0u : left;
   }
-  const float bar = r == rounds ? of_key(best) : -FLT_MAX;  // (masked values are below it)
+  const float bar = best != 0u ? of_key(best) : -FLT_MAX;  // (masked values are below it)
   constexpr int kWords = (VPT + 31) / 32;
   uint32_t some[kWords], equal[kWords];
   int n = 0;
@@ -370,7 +372,7 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     to -= n;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if ((some[0] >> i) & 1u) s_cand[to++] = (uint64_t)key_of(clean(c[i])) << 32 | (uint32_t)column<V, 32>(i, lane);
+      if ((some[0] >> i) & 1u) s_cand[to++] = ranked(clean(c[i]), column<V, 32>(i, lane));
   } else
   for (int base = 0; base < count;) {
     int i = -1;
@@ -380,7 +382,7 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     const unsigned have = __ballot_sync(kFull, i >= 0);
     if (i >= 0) {
       const int col = column<V, 32>(i, lane);
-      s_cand[base + __popc(have & ((1u << lane) - 1u))] = (uint64_t)key_of(value_of(col)) << 32 | (uint32_t)col;
+      s_cand[base + __popc(have & ((1u << lane) - 1u))] = ranked(value_of(col), col);
 #pragma unroll
       for (int w = 0; w < kWords; ++w)
         if (i / 32 == w) some[w] &= some[w] - 1;
@@ -388,18 +390,18 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     base += __popc(have);
   }
   __syncwarp();
-  uint32_t key = 0u, at = kFull;  // this lane's candidate
-  if (lane < count) {
-    const uint64_t x = s_cand[lane];
-    key = (uint32_t)(x >> 32);
-    at = (uint32_t)x;
-  }
-  int j = 0;
-  for (const int sorted = min(rounds, count); j < sorted; ++j) {
-    const uint32_t b = __reduce_max_sync(kFull, key);
-    const uint32_t first = __reduce_min_sync(kFull, key == b ? at : kFull);
-    if (lane == j) { chosen = (int)first; value = of_key(b); }
-    if (at == first) key = 0u;
+  // each candidate's place is the number of those before it; lane j then takes the j'th
+  const uint64_t x = lane < count ? s_cand[lane] : 0ull;
+  int place = 0;
+#pragma unroll 4
+  for (int q = 0; q < count; ++q) place += s_cand[q] > x;
+  if (lane < count) s_cand[32 + place] = x;
+  __syncwarp();
+  int j = min(rounds, count);
+  if (lane < j) {
+    const uint64_t u = s_cand[32 + lane];
+    chosen = (int)~(uint32_t)u;
+    value = of_key((uint32_t)(u >> 32));
   }
   for (; j < rounds; ++j) {  // the lowest column that equals bar
     uint32_t mine = kFull;
@@ -525,7 +527,7 @@ template <typename T, int VPT, int V, int L>
 __global__ void __launch_bounds__(32 * kRouteWarps, VPT <= 8 ? 10 : VPT <= 16 ? 7 : VPT <= 32 ? 6 : 2)
 route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict__ weights, int32_t *__restrict__ indices) {
   constexpr int RPW = 32 / L;  // rows a warp
-  __shared__ uint64_t s_cand[kRouteWarps * RPW][32];
+  __shared__ uint64_t s_cand[kRouteWarps][L == 32 ? 64 : 1];  // candidates and their order (whole warps)
   extern __shared__ float s_bias[];  // [VPT * L], zeros behind K
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, seg = lane / L;
   float bmax = 0.0f;  // the largest finite |bias|
@@ -552,7 +554,7 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
     if constexpr (kAhead)
       if (more) load_row<T, VPT, V, L>(at(next), a.K, l, ahead);
     const bool exists = n < a.N;
-    route_row<T, VPT, V, L>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp * RPW + seg], weights + n * a.top_k, indices + n * a.top_k);
+    route_row<T, VPT, V, L>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp], weights + n * a.top_k, indices + n * a.top_k);
     if (!more) break;
     n = next;
     if constexpr (kAhead) raw = ahead;
@@ -565,26 +567,25 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
 // others nothing; else the softmax gives s (g [chosen] - sum of g s over the chosen) to every score, and
 // sigmoid and given values pass g s (1 - s) and g on.  The row without the chosen ones' part is written first (the
 // scores are read for the softmax only), then the lane of each slot writes its element.
-template <typename T, int VPT, int V, int L>
-__global__ void __launch_bounds__(128) route_backward_kernel(const float *__restrict__ dw, const T *__restrict__ scores,
+template <typename T, int VPT, int V, int L, bool DENSE>
+__global__ void __launch_bounds__(128, DENSE ? 1 : 12) route_backward_kernel(const float *__restrict__ dw, const T *__restrict__ scores,
                                                              const int32_t *__restrict__ indices, const RouteArgs a,
                                                              T *__restrict__ dz) {
   const int lane = threadIdx.x & 31, l = lane % L;
-  const bool dense = a.func == FGMM_SCORE_SOFTMAX && !a.renorm;
   const int64_t stride = (int64_t)gridDim.x * (128 / L);
   for (int64_t n = (int64_t)blockIdx.x * (128 / L) + threadIdx.x / L; n - lane / L < a.N; n += stride) {
     const bool exists = n < a.N;
     const int64_t r = exists ? n : a.N - 1;
     const T *row = scores + r * a.stride;
-    Row<T, VPT> raw;
-    if (dense) load_row<T, VPT, V, L>(row, a.K, l, raw);
+    Row<T, DENSE ? VPT : 1> raw;
+    if constexpr (DENSE) load_row<T, VPT, V, L>(row, a.K, l, raw);
     int chosen = l < a.top_k ? __ldg(indices + r * a.top_k + l) : -1;
     if (chosen < 0 || chosen >= a.K) chosen = -1;
     const float z = chosen >= 0 ? score_at(row, chosen) : -INFINITY;
     const bool live = z > -INFINITY;  // a masked score gets no gradient
     const float g = live ? __ldg(dw + r * a.top_k + l) * a.scale : 0.0f;
-    float out[VPT], d, base = 0.0f;
-    if (dense) {
+    float out[DENSE ? VPT : 1], d, base = 0.0f;
+    if constexpr (DENSE) {
       float m;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) out[i] = clean(to_f32(raw.v[i]));
@@ -609,8 +610,6 @@ __global__ void __launch_bounds__(128) route_backward_kernel(const float *__rest
           d = g * e / ((1.0f + e) * (1.0f + e));
         }
       }
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) out[i] = 0.0f;
     }
     if (!live) { d = 0.0f; chosen = -1; }
     float sum = base;  // slots of one expert add up, in all of their lanes alike
@@ -627,13 +626,13 @@ __global__ void __launch_bounds__(128) route_backward_kernel(const float *__rest
         if (V > 1 && c + V <= a.K) {
           alignas(16) T pack[V];
 #pragma unroll
-          for (int v = 0; v < V; ++v) pack[v] = from_f32<T>(out[i + v]);
+          for (int v = 0; v < V; ++v) pack[v] = from_f32<T>(DENSE ? out[DENSE ? i + v : 0] : 0.0f);
           if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4 *>(to + c) = *reinterpret_cast<uint4 *>(pack);
           else if constexpr (V * sizeof(T) == 8) *reinterpret_cast<uint2 *>(to + c) = *reinterpret_cast<uint2 *>(pack);
         } else {
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            if (c + v < a.K) to[c + v] = from_f32<T>(out[i + v]);
+            if (c + v < a.K) to[c + v] = from_f32<T>(DENSE ? out[DENSE ? i + v : 0] : 0.0f);
         }
       }
     }
@@ -682,7 +681,10 @@ int route_backward_t(const float *dw, const T *z, const int32_t *idx, const Rout
                    reinterpret_cast<uintptr_t>(dz) % 16 == 0 && a.K * sizeof(T) % 16 == 0;
   return by_row_width<T>(a.K, a.top_k, vec, [&](auto vpt, auto v, auto lanes) {
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, 128 / lanes()), (int64_t)num_sms() * 16);
-    route_backward_kernel<T, vpt(), v(), lanes()><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
+    if (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)
+      route_backward_kernel<T, vpt(), v(), lanes(), true><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
+    else
+      route_backward_kernel<T, vpt(), v(), lanes(), false><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
     FGMM_LAUNCH_CHECK("route_backward_kernel");
     return FGMM_OK;
   });

@@ -86,7 +86,7 @@ struct TcArgs {
   uint32_t idesc;
   Pieces pieces;  // DW
   uint32_t div_mul, div_shift;  // n / top_k = n * div_mul >> div_shift for n < 2^31
-  int vec;  // rows of the result start on 16-byte boundaries
+  int vec, vec32;  // rows of the result start on 16-byte, 32-byte boundaries
 };
 
 // What one tile covers.  For Y and DX: `rows` rows from r0 of expert e, columns from n0.  For DW: `rows` output dimensions
@@ -463,6 +463,20 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     // 32 rows x CW columns (from column c0 of the tile) through shared memory, 16 rows at a time, so that the global
     // writes are whole lines
     auto write = [&](const float *v, const Tile &x, int c0) {
+      if constexpr (sizeof(OUT) == 4) {
+        // fp32: whole 32-byte sectors, a row a lane, past shared memory, whose bandwidth the products take (131,072 rows
+        // 128 -> 128: 81 -> 75 us; 16-bit results lose that way, 18 -> 21 us)
+        if (a.vec32) {
+          const int row = q * 32 + lane;
+          if (row < x.rows) {
+            OUT *p = out + ((MODE == kWeights ? (int64_t)x.e * a.d_out + x.m0 : x.r0) + row) * width + x.n0 + c0;
+#pragma unroll
+            for (int j = 0; j < CW; j += 8)
+              if (x.n0 + c0 + j < width) st_v8(p + j, v + j);
+          }
+          return;
+        }
+      }
       const int64_t row0 = MODE == kWeights ? (int64_t)x.e * a.d_out + x.m0 : x.r0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -648,48 +662,59 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const __grid_constant_
 }
 
 // Rows of `cols` elements to rows of PLANES planes of `colsp` (zeros behind cols): float32 in three bf16
-// planes whose sum it is (to 2^-24), 16-bit types as they are.  An infinite value keeps zeros in the lower planes.
+// planes whose sum it is (to 2^-24), 16-bit types as they are.  An infinite value keeps zeros in the lower planes.  One launch
+// copies a call's operands.
+struct Copies {
+  struct {
+    const void *src;
+    uint16_t *dst;
+    int64_t items;  // rows * colsp / 8
+    int cols, colsp;
+  } job[3];
+  int n;
+};
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) split_planes_kernel(const T *__restrict__ src, int64_t rows, int cols, int colsp,
-                                                           uint16_t *__restrict__ dst) {
-  griddep_launch();
+__global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant__ Copies copies) {
   griddep_wait();
-  const int per = colsp / 8;
-  const int64_t n = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 8;
-    const T *p = src + r * cols + c;
-    alignas(16) uint16_t h[PLANES][8];
-    if constexpr (PLANES == 3) {
-      float v[8];
-      if (cols % 4 == 0 && c + 8 <= cols) {
-        *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(p));
-        *reinterpret_cast<float4 *>(v + 4) = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+  griddep_launch();
+  for (int q = 0; q < copies.n; ++q) {
+    const auto &job = copies.job[q];
+    const T *__restrict__ src = static_cast<const T *>(job.src);
+    uint16_t *__restrict__ dst = job.dst;
+    const int cols = job.cols, colsp = job.colsp, per = colsp / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < job.items; i += (int64_t)gridDim.x * 256) {
+      const int64_t r = i / per;
+      const int c = (int)(i - r * per) * 8;
+      const T *p = src + r * cols + c;
+      alignas(16) uint16_t h[PLANES][8];
+      if constexpr (PLANES == 3) {
+        float v[8];
+        if (cols % 4 == 0 && c + 8 <= cols) {
+          *reinterpret_cast<float4 *>(v) = __ldg(reinterpret_cast<const float4 *>(p));
+          *reinterpret_cast<float4 *>(v + 4) = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(p[k]) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const __nv_bfloat16 b0 = __float2bfloat16_rn(v[k]);
+          float rest = v[k] - __bfloat162float(b0);
+          if (!isfinite(rest)) rest = 0.0f;
+          const __nv_bfloat16 b1 = __float2bfloat16_rn(rest);
+          const __nv_bfloat16 b2 = __float2bfloat16_rn(rest - __bfloat162float(b1));
+          h[0][k] = __bfloat16_as_ushort(b0);
+          h[1][k] = __bfloat16_as_ushort(b1);
+          h[2][k] = __bfloat16_as_ushort(b2);
+        }
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(p[k]) : 0.0f;
+        for (int k = 0; k < 8; ++k) h[0][k] = c + k < cols ? reinterpret_cast<const uint16_t *>(p)[k] : (uint16_t)0;
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const __nv_bfloat16 b0 = __float2bfloat16_rn(v[k]);
-        float rest = v[k] - __bfloat162float(b0);
-        if (!isfinite(rest)) rest = 0.0f;
-        const __nv_bfloat16 b1 = __float2bfloat16_rn(rest);
-        const __nv_bfloat16 b2 = __float2bfloat16_rn(rest - __bfloat162float(b1));
-        h[0][k] = __bfloat16_as_ushort(b0);
-        h[1][k] = __bfloat16_as_ushort(b1);
-        h[2][k] = __bfloat16_as_ushort(b2);
-      }
-    } else if (cols % 8 == 0) {
-      *reinterpret_cast<uint4 *>(h[0]) = __ldg(reinterpret_cast<const uint4 *>(p));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) h[0][k] = c + k < cols ? reinterpret_cast<const uint16_t *>(p)[k] : (uint16_t)0;
+      for (int l = 0; l < PLANES; ++l)
+        *reinterpret_cast<uint4 *>(dst + (r * PLANES + l) * colsp + c) = *reinterpret_cast<uint4 *>(h[l]);
     }
-#pragma unroll
-    for (int q = 0; q < PLANES; ++q)
-      *reinterpret_cast<uint4 *>(dst + (r * PLANES + q) * colsp + c) = *reinterpret_cast<uint4 *>(h[q]);
   }
 }
 
@@ -736,20 +761,20 @@ size_t copy_elems(int dtype, int64_t rows, int cols) {
   return needs_copy(dtype, cols) ? (size_t)rows * plane_cols(dtype, cols) * (dtype == FGMM_F32 ? 3 : 1) : 0;
 }
 
-// The operand of `src` [rows][cols], copied into `dst` where TMA cannot read it as it is.
-int operand(Operand *o, const void *src, int dtype, int64_t rows, int cols, uint16_t *dst, cudaStream_t st) {
-  if (!needs_copy(dtype, cols)) {
-    *o = {src, rows, cols, cols};
-    return FGMM_OK;
-  }
+// The operand of `src` [rows][cols], to be copied into `dst` where TMA cannot read it as it is.
+Operand operand(const void *src, int dtype, int64_t rows, int cols, uint16_t *dst, Copies &copies) {
+  if (!needs_copy(dtype, cols)) return {src, rows, cols, cols};
   const int colsp = plane_cols(dtype, cols);
-  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(rows * (colsp / 8), 256), 8 * num_sms());
-  if (dtype == FGMM_F32)
-    FGMM_CUDA_TRY(launch_pdl(split_planes_kernel<float, 3>, dim3(grid), dim3(256), 0, st, (const float *)src, rows, cols, colsp, dst));
-  else
-    FGMM_CUDA_TRY(launch_pdl(split_planes_kernel<__half, 1>, dim3(grid), dim3(256), 0, st, (const __half *)src, rows, cols, colsp, dst));
-  const int planes = dtype == FGMM_F32 ? 3 : 1;
-  *o = {dst, rows, colsp * planes, colsp};
+  copies.job[copies.n++] = {src, dst, rows * (colsp / 8), cols, colsp};
+  return {dst, rows, colsp * (dtype == FGMM_F32 ? 3 : 1), colsp};
+}
+
+int run_copies(const Copies &copies, int dtype, cudaStream_t st) {
+  int64_t most = 0;
+  for (int i = 0; i < copies.n; ++i) most = std::max(most, copies.job[i].items);
+  if (most == 0) return FGMM_OK;
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(most, 256), 8 * num_sms());
+  FGMM_CUDA_TRY(launch_pdl(dtype == FGMM_F32 ? split_planes_kernel<float, 3> : split_planes_kernel<__half, 1>, dim3(grid), dim3(256), 0, st, copies));
   return FGMM_OK;
 }
 
@@ -795,6 +820,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   while ((1u << (a.div_shift - 31)) < (uint32_t)p.top_k) ++a.div_shift;
   a.div_mul = (uint32_t)((((uint64_t)1 << a.div_shift) + p.top_k - 1) / p.top_k);
   a.idesc = idesc_f16(BM, NT, MODE == kWeights, MODE != kForward, bf16);
+  a.vec32 = (width * sizeof(OUT)) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
   static std::atomic<bool> done[64];  // per device
@@ -872,9 +898,9 @@ size_t products_tc_workspace(int dtype, int64_t N, int K, int d_in, int d_out, i
 int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y,
                 void *ws, cudaStream_t st) {
   const TcSpace s = tc_space(ws, dtype, N, p.K, d_in, d_out, p.top_k, {true, false, false});
-  Operand ox, ow;
-  int rc = operand(&ox, x, dtype, N, d_in, s.x, st);
-  if (!rc) rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, st);
+  Copies copies{};
+  const Operand ox = operand(x, dtype, N, d_in, s.x, copies), ow = operand(weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, copies);
+  int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
   if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, st);
   if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, st);
@@ -884,18 +910,18 @@ int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_i
 int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
                          const RoutePlan &p, float *dx_rows, void *d_weight, const TcParts &parts, void *ws, cudaStream_t st) {
   const TcSpace s = tc_space(ws, dtype, N, p.K, d_in, d_out, p.top_k, parts);
-  Operand og, ow, ox;
-  int rc = operand(&og, dy, dtype, p.R, d_out, s.dy, st);
+  Copies copies{};
+  const Operand og = operand(dy, dtype, p.R, d_out, s.dy, copies);
+  const Operand ow = parts.inputs ? operand(weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, copies) : Operand{};
+  const Operand ox = parts.weights ? operand(x, dtype, N, d_in, s.x, copies) : Operand{};
+  int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
   if (parts.inputs) {
-    rc = operand(&ow, weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, st);
-    if (!rc) rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st)
-                                    : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st);
+    rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st)
+                           : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st);
     if (rc) return rc;
   }
   if (!parts.weights) return FGMM_OK;
-  rc = operand(&ox, x, dtype, N, d_in, s.x, st);
-  if (rc) return rc;
   if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, st);
   if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, s.pieces, st);
   return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, s.pieces, st);

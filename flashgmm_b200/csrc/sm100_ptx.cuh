@@ -204,6 +204,13 @@ __device__ __forceinline__ void st_hint(float *p, float v, uint64_t policy) {
   asm volatile("st.global.L2::cache_hint.f32 [%0], %1, %2;" ::"l"(p), "f"(v), "l"(policy));
 }
 
+// 32 bytes of fp32 to a 32-byte boundary.
+__device__ __forceinline__ void st_v8(float *p, const float *v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 // Drops the 128-byte L2 line at p without writing it back (its data is dead).
 __device__ __forceinline__ void discard_l2_line(const void *p) {
   asm volatile("discard.global.L2 [%0], 128;" ::"l"(p) : "memory");
