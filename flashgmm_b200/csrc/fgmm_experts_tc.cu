@@ -628,8 +628,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, 
   }
 }
 
-// Adds the pieces of the experts that have more than one: blockIdx.x counts their tiles, a block writes kJoinRows rows.
-constexpr int kJoinRows = 8;
+// Adds the pieces of the experts that have more than one, in their order: blockIdx.x counts their tiles, a block writes 1024
+// results (with 32 rows a block, few had work: 28 -> 58 us for 4 experts of 16,384 rows, 256 x 256).
 template <int NT, typename OUT>
 __global__ void __launch_bounds__(256) join_pieces_kernel(const __grid_constant__ TcArgs a, OUT *__restrict__ out) {
   griddep_launch();
@@ -643,12 +643,13 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const __grid_constant_
     if (__ldg(a.pieces.joined + mid) <= u) lo = mid; else hi = mid;
   }
   const int first = __ldg(a.pieces.slot + lo), n = __ldg(a.pieces.slot + lo + 1) - first;
-  const int m0 = tile / n_tiles * BM + blockIdx.y * kJoinRows, n0 = tile % n_tiles * NT;
-  for (int i = threadIdx.x; i < kJoinRows * (NT / 4); i += 256) {
-    const int r = i / (NT / 4), c = i % (NT / 4) * 4, o = m0 + r, col = n0 + c;
-    if (o >= a.d_out || col >= a.d_in) continue;
-    const float *from = a.pieces.tiles + (int64_t)(blockIdx.y * kJoinRows + r) * NT + c;
+  {
+    const int r = blockIdx.y * (1024 / NT) + threadIdx.x / (NT / 4), c = threadIdx.x % (NT / 4) * 4;
+    const int o = tile / n_tiles * BM + r, col = tile % n_tiles * NT + c;
+    if (o >= a.d_out || col >= a.d_in) return;
+    const float *from = a.pieces.tiles + (int64_t)r * NT + c;
     float f[4] = {};
+#pragma unroll 8
     for (int q = 0; q < n; ++q) {
       const int s = min((first + q) * per + tile, a.pieces.slots - 1);
       const float4 v = __ldg(reinterpret_cast<const float4 *>(from + (int64_t)s * BM * NT));
@@ -778,16 +779,18 @@ int run_copies(const Copies &copies, int dtype, cudaStream_t st) {
   return FGMM_OK;
 }
 
-// The pieces' division: none where every SM has three whole tiles; else a third of an SM's share at most, and four stages at
-// least.  (With pieces, their plan and their join 512 tiles of up to 16 stages took 100 us instead of 60.)  A slot count
-// that holds those of every routing: an expert of n > most >= 4 stages has at most 2 n / most pieces, and n is at most 5 / 4 of its rows / KCH.
+// The pieces' division: none where every SM has three whole tiles (with pieces, their plan and their join 512 tiles of up to 16
+// stages took 100 us instead of 60); else an SM's share of the stages at most, of float32's heavier ones (192 KB and 24
+// products against 48 KB and 4, for a piece of 64 KB against 128 KB) a third of it, and four at least.  (With a third
+// for all, 8 experts of 4,096 routes, 1,024 x 1,024 bf16, took 52 us instead of 28.)  A slot count that holds those of every routing:
+// an expert of n > most >= 4 stages has at most 2 n / most pieces, and n is at most 5 / 4 of its rows / KCH.
 struct PieceSizes {
   int64_t per, most, slots;
 };
-PieceSizes piece_sizes(int64_t R, int K, int d_in, int d_out, int NT) {
+PieceSizes piece_sizes(int dtype, int64_t R, int K, int d_in, int d_out, int NT) {
   PieceSizes z;
   z.per = cdiv(d_out, BM) * cdiv(d_in, NT);
-  z.most = K * z.per >= 3 * num_sms() ? INT32_MAX / 2 : std::max<int64_t>(4, cdiv((cdiv(R, KCH) + K) * z.per, 3 * num_sms()));
+  z.most = K * z.per >= 3 * num_sms() ? INT32_MAX / 2 : std::max<int64_t>(4, cdiv((cdiv(R, KCH) + K) * z.per, (dtype == FGMM_F32 ? 3 : 1) * num_sms()));
   z.slots = cdiv(R, KCH) <= z.most ? 1 : (cdiv(5 * cdiv(R, KCH), 2 * z.most) + 1) * z.per;
   return z;
 }
@@ -831,7 +834,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
     if (dev < 64) done[dev].store(true, std::memory_order_release);
   }
   if (MODE == kWeights) {
-    const PieceSizes z = piece_sizes(p.R, p.K, d_in, d_out, NT);
+    const PieceSizes z = piece_sizes(dtype, p.R, p.K, d_in, d_out, NT);
     if ((cdiv(p.R, KCH) + p.K) * z.per > INT32_MAX) return fail(FGMM_ERR_UNSUPPORTED, "more than 2^31 stages of the weights' gradient");
     Carve c(pieces);
     int *first = c.take<int>(p.K + 1), *slot = c.take<int>(p.K + 1), *joined = c.take<int>(p.K + 1);
@@ -841,7 +844,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
     FGMM_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(num_sms(), (cdiv(p.R, KCH * z.most) + p.K) * z.per)), dim3(kThreads),
                              Sh::smem(p.K), st, ma, mb, a, out));
     if (z.slots > 1)
-      FGMM_CUDA_TRY(launch_pdl(join_pieces_kernel<NT, OUT>, dim3((unsigned)(z.slots / 2), BM / kJoinRows), dim3(256), 0, st, a, out));
+      FGMM_CUDA_TRY(launch_pdl(join_pieces_kernel<NT, OUT>, dim3((unsigned)(z.slots / 2), BM * NT / 1024), dim3(256), 0, st, a, out));
     return FGMM_OK;
   }
   const int64_t tiles = (cdiv(p.R, BM) + std::min<int64_t>(p.K, p.R)) * cdiv(width, NT);  // at most
@@ -850,12 +853,19 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   return FGMM_OK;
 }
 
-// Columns of a tile: 256 where every SM gets two such tiles (of Y and DX; DW is divided evenly anyway), else 128.
+// Columns of a tile of Y or DX.  A stage's products are bound by shared memory: 64 KB written and read for 128 columns, 96 KB for
+// 256, so the wider tile takes one and a half times as long and holds twice as much; it is taken where the SMs' rounds of such
+// tiles cost less.  (Every expert's last tile counts as half a tile more.)
+bool wide_tiles(int64_t R, int K, int width) {
+  if (width <= 128) return false;
+  const int64_t m = cdiv(R, BM) + std::min<int64_t>(K, R) / 2;
+  return 3 * cdiv(m * cdiv(width, 256), num_sms()) <= 2 * cdiv(m * cdiv(width, 128), num_sms());
+}
 template <int MODE, typename OUT>
 int launch16(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
              void *pieces, cudaStream_t st) {
   const int width = MODE == kForward ? d_out : d_in;
-  if (MODE == kWeights ? weights_tile(dtype, d_in) == 256 : width > 128 && cdiv(p.R, BM) * cdiv(width, 256) >= 2 * num_sms())
+  if (MODE == kWeights ? weights_tile(dtype, d_in) == 256 : wide_tiles(p.R, p.K, width))
     return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
   return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
 }
@@ -864,7 +874,7 @@ size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
   const int NT = weights_tile(dtype, d_in);
   Carve c(nullptr);
   for (int i = 0; i < 3; ++i) c.take<int>(K + 1);
-  c.take<float>(piece_sizes(R, K, d_in, d_out, NT).slots * BM * NT);
+  c.take<float>(piece_sizes(dtype, R, K, d_in, d_out, NT).slots * BM * NT);
   return c.bytes();
 }
 
