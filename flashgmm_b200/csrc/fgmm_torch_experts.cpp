@@ -4,6 +4,7 @@
 // Rows that are not contiguous are copied; a score matrix is read through its row stride.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "../../include/flashgmm_b200.h"
@@ -50,8 +51,13 @@ Tensor for_products(const Tensor &t) {
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
+// A result or scratch of torch's caching allocator, past the dispatcher (a microsecond of a small call).
+Tensor fresh(torch::IntArrayRef sizes, torch::ScalarType type, const torch::Device &dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
+
 Tensor scratch(size_t bytes, const torch::Device &dev) {
-  return torch::empty({(int64_t)std::max<size_t>(bytes, 256)}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+  return fresh({(int64_t)std::max<size_t>(bytes, 256)}, torch::kUInt8, dev);
 }
 
 void *stream() { return at::cuda::getCurrentCUDAStream().stream(); }
@@ -85,8 +91,8 @@ std::tuple<Tensor, Tensor> route_experts(const Tensor &scores, int64_t top_k, co
   TORCH_CHECK(top_k >= 1 && top_k <= K && top_k <= FGMM_MAX_TOP_K, "top_k must be in [1, min(K, ", FGMM_MAX_TOP_K, ")], got ", top_k);
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor z = with_rows(scores);
-  Tensor w = torch::empty({N, top_k}, z.options().dtype(torch::kFloat32));
-  Tensor idx = torch::empty({N, top_k}, z.options().dtype(torch::kInt32));
+  Tensor w = fresh({N, top_k}, torch::kFloat32, dev);
+  Tensor idx = fresh({N, top_k}, torch::kInt32, dev);
   check_rc(fgmm_route_experts(z.data_ptr(), dtype, N, narrow(K, "K"), row_stride(z), bias ? b.data_ptr<float>() : nullptr,
                               (int)top_k, f, narrow(n_groups, "n_groups"), narrow(top_groups.value_or(n_groups), "top_groups"),
                               renormalize, (float)scale, w.data_ptr<float>(), idx.data_ptr<int32_t>(), stream()),
@@ -109,7 +115,7 @@ Tensor route_experts_backward(const Tensor &d_weights, const Tensor &scores, con
   check_shape(d_weights, "d_weights", {N, top_k});
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor z = with_rows(scores), dw = d_weights.contiguous(), idx = indices.contiguous();
-  Tensor dz = torch::empty({N, K}, z.options());
+  Tensor dz = fresh({N, K}, z.scalar_type(), dev);
   check_rc(fgmm_route_experts_backward(dw.data_ptr<float>(), z.data_ptr(), dtype, N, narrow(K, "K"), row_stride(z),
                                        idx.data_ptr<int32_t>(), narrow(top_k, "top_k"), f, renormalize, (float)scale,
                                        dz.data_ptr(), stream()),
@@ -127,8 +133,8 @@ std::tuple<Tensor, Tensor, Tensor> group_routes(const Tensor &indices, int64_t K
   const torch::Device dev = indices.device();
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor idx = indices.contiguous();
-  Tensor order = torch::empty({R}, idx.options()), offsets = torch::empty({K + 1}, idx.options());
-  Tensor position = torch::empty(indices.sizes(), idx.options());
+  Tensor order = fresh({R}, torch::kInt32, dev), offsets = fresh({K + 1}, torch::kInt32, dev);
+  Tensor position = fresh(indices.sizes(), torch::kInt32, dev);
   Tensor ws = scratch(fgmm_group_routes_workspace_bytes(R, (int)K), dev);
   check_rc(fgmm_group_routes(idx.data_ptr<int32_t>(), R, (int)K, order.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
                              position.data_ptr<int32_t>(), ws.data_ptr(), ws.numel(), stream()),
@@ -172,7 +178,7 @@ Tensor expert_products(const Tensor &x, const Tensor &weight, const Tensor &orde
   check_shape(weight, "weight", {p.K, d_out, d_in});
   TORCH_CHECK(d_in >= 1 && d_out >= 1, "x and weight must have at least one column");
   const Tensor xc = for_products(x), wc = for_products(weight);
-  Tensor y = torch::empty({p.R, d_out}, x.options());
+  Tensor y = fresh({p.R, d_out}, x.scalar_type(), dev);
   const int di = narrow(d_in, "d_in"), dn = narrow(d_out, "d_out");
   const size_t nb = fgmm_expert_products_workspace_bytes(dtype, p.N, p.K, di, dn, p.top_k);
   TORCH_CHECK(nb > 0, "expert_products: ", fgmm_last_error());
@@ -202,8 +208,8 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>> expert_products_backwar
   TORCH_CHECK(d_in >= 1 && d_out >= 1, "x and weight must have at least one column");
   const Tensor xc = for_products(x), wc = for_products(weight), gc = for_products(dy);
   c10::optional<Tensor> dx, dw;
-  if (need_dx) dx = torch::empty({p.N, d_in}, x.options());
-  if (need_dweight) dw = torch::empty({p.K, d_out, d_in}, x.options());
+  if (need_dx) dx = fresh({p.N, d_in}, x.scalar_type(), dev);
+  if (need_dweight) dw = fresh({p.K, d_out, d_in}, x.scalar_type(), dev);
   if (!need_dx && !need_dweight) return {dx, dw};
   const int di = narrow(d_in, "d_in"), dn = narrow(d_out, "d_out");
   const size_t nb = fgmm_expert_products_backward_workspace_bytes(dtype, p.N, p.K, di, dn, p.top_k);
@@ -230,7 +236,7 @@ Tensor combine_experts(const Tensor &y, const Tensor &weights, const Tensor &ord
   check_shape(weights, "weights", {p.N, p.top_k});
   TORCH_CHECK(d >= 1, "y must have at least one column");
   const Tensor yc = y.contiguous(), w = weights.contiguous();
-  Tensor out = torch::empty({p.N, d}, y.options());
+  Tensor out = fresh({p.N, d}, y.scalar_type(), dev);
   check_rc(fgmm_combine_experts(yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(), p.position.data_ptr<int32_t>(),
                                 p.top_k, out.data_ptr(), stream()),
            "combine_experts");
@@ -254,7 +260,7 @@ std::tuple<Tensor, Tensor> combine_experts_backward(const Tensor &d_out, const T
   check_shape(d_out, "d_out", {p.N, d});
   TORCH_CHECK(d >= 1, "y must have at least one column");
   const Tensor yc = y.contiguous(), gc = d_out.contiguous(), w = weights.contiguous();
-  Tensor dy = torch::empty({p.R, d}, y.options()), dw = torch::empty({p.N, p.top_k}, w.options());
+  Tensor dy = fresh({p.R, d}, y.scalar_type(), dev), dw = fresh({p.N, p.top_k}, torch::kFloat32, dev);
   check_rc(fgmm_combine_experts_backward(gc.data_ptr(), yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(),
                                          p.order.data_ptr<int32_t>(), p.offsets.data_ptr<int32_t>(), p.K, p.top_k,
                                          dy.data_ptr(), dw.data_ptr<float>(), stream()),

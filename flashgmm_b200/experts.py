@@ -40,20 +40,28 @@ class Routes(NamedTuple):
     position: torch.Tensor
 
 
-def _check_tensors(**tensors):
+_grad_enabled = torch.is_grad_enabled
+_ops = None  # the compiled module, once loaded
+
+
+def _load():
+    global _ops
+    _ops = _ext.load()
+    return _ops
+
+
+def _refuse(error, routes=None, **tensors):
+    """The RuntimeError for arguments that are no tensors.  The calls below look at their tensors' attributes and hand them to
+    the compiled module, which checks the rest; only what that trips over is looked at here (a call that launches one
+    kernel costs the host about 6 us)."""
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"{name} must be a torch.Tensor")
-
-
-def _check_routes(routes):
-    if not isinstance(routes, Routes):
-        raise RuntimeError("routes must be a Routes (of group_routes)")
-    _check_tensors(order=routes.order, offsets=routes.offsets, position=routes.position)
-
-
-def _records(*tensors):
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+            raise RuntimeError(f"{name} must be a torch.Tensor") from error
+    if routes is not None:
+        if not isinstance(routes, Routes):
+            raise RuntimeError("routes must be a Routes (of group_routes)") from error
+        _refuse(error, order=routes.order, offsets=routes.offsets, position=routes.position)
+    raise RuntimeError(str(error)) from error
 
 
 class _Route(torch.autograd.Function):
@@ -92,26 +100,30 @@ def route_experts(scores, top_k, score_func="softmax", bias=None, n_groups=1, to
     A score of -inf or NaN is masked and +inf counts as the largest finite value; slots that no
     unmasked expert is left for hold index -1 and weight 0.  K <= 4096, top_k <= 32, n_groups <= 32.
     The weights carry a gradient to ``scores``; the choice and ``bias`` have none."""
-    _check_tensors(scores=scores)
-    if bias is not None:
-        _check_tensors(bias=bias)
-    if _records(scores):
-        return _Route.apply(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
-    return _ext.load().route_experts(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
+    try:
+        if scores.requires_grad and _grad_enabled():
+            return _Route.apply(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
+        return (_ops or _load()).route_experts(scores, top_k, score_func, bias, n_groups, top_groups, renormalize, scale)
+    except (AttributeError, TypeError) as error:
+        _refuse(error, scores=scores, **({} if bias is None else {"bias": bias}))
 
 
 def route_experts_backward(d_weights, scores, indices, score_func="softmax", renormalize=True, scale=1.0):
     """``d_scores[N, K]`` (of the scores' type) from the weights' gradient, for the ``indices`` that
     :func:`route_experts` gave with the same ``score_func``, ``renormalize`` and ``scale``."""
-    _check_tensors(d_weights=d_weights, scores=scores, indices=indices)
-    return _ext.load().route_experts_backward(d_weights, scores, indices, score_func, renormalize, scale)
+    try:
+        return (_ops or _load()).route_experts_backward(d_weights, scores, indices, score_func, renormalize, scale)
+    except TypeError as error:
+        _refuse(error, d_weights=d_weights, scores=scores, indices=indices)
 
 
 def group_routes(indices, K):
     """Groups the routes of ``indices[N, top_k]`` (int32) by expert -> :class:`Routes`, stable: an
     expert's routes keep their order.  Indices outside [0, K) are routes without an expert."""
-    _check_tensors(indices=indices)
-    return Routes(*_ext.load().group_routes(indices, K))
+    try:
+        return Routes(*(_ops or _load()).group_routes(indices, K))
+    except TypeError as error:
+        _refuse(error, indices=indices)
 
 
 class _Products(torch.autograd.Function):
@@ -135,19 +147,23 @@ def expert_products(x, weight, routes):
 
     ``x[N, d_in]`` and ``weight[K, d_out, d_in]`` of one type; gradients to both.  float32 operands run
     on the tensor cores as three bf16 planes (24 bits together); an infinite entry gives NaN there."""
-    _check_tensors(x=x, weight=weight)
-    _check_routes(routes)
-    if _records(x, weight):
-        return _Products.apply(x, weight, *routes)
-    return _ext.load().expert_products(x, weight, *routes)
+    try:
+        order, offsets, position = routes
+        if (x.requires_grad or weight.requires_grad) and _grad_enabled():
+            return _Products.apply(x, weight, order, offsets, position)
+        return (_ops or _load()).expert_products(x, weight, order, offsets, position)
+    except (AttributeError, TypeError, ValueError) as error:
+        _refuse(error, routes, x=x, weight=weight)
 
 
 def expert_products_backward(dy, x, weight, routes, need_dx=True, need_dweight=True):
     """``[dx, dweight]`` from ``dy[N top_k, d_out]`` (``None`` where not needed): dx sums a point's
     rows in slot order, dweight an expert's rows; both round once."""
-    _check_tensors(dy=dy, x=x, weight=weight)
-    _check_routes(routes)
-    return list(_ext.load().expert_products_backward(dy, x, weight, *routes, need_dx, need_dweight))
+    try:
+        order, offsets, position = routes
+        return list((_ops or _load()).expert_products_backward(dy, x, weight, order, offsets, position, need_dx, need_dweight))
+    except (TypeError, ValueError) as error:
+        _refuse(error, routes, dy=dy, x=x, weight=weight)
 
 
 class _Combine(torch.autograd.Function):
@@ -167,15 +183,19 @@ def combine_experts(y, weights, routes):
     """``out[n] = sum_j weights[n, j] y[position[n, j]]`` -> ``out[N, d]``, slots without an expert
     left out.  ``y[N top_k, d]`` as :func:`expert_products` gives it, ``weights[N, top_k]`` float32;
     gradients to both."""
-    _check_tensors(y=y, weights=weights)
-    _check_routes(routes)
-    if _records(y, weights):
-        return _Combine.apply(y, weights, *routes)
-    return _ext.load().combine_experts(y, weights, *routes)
+    try:
+        order, offsets, position = routes
+        if (y.requires_grad or weights.requires_grad) and _grad_enabled():
+            return _Combine.apply(y, weights, order, offsets, position)
+        return (_ops or _load()).combine_experts(y, weights, order, offsets, position)
+    except (AttributeError, TypeError, ValueError) as error:
+        _refuse(error, routes, y=y, weights=weights)
 
 
 def combine_experts_backward(d_out, y, weights, routes):
     """``[dy, d_weights]`` from ``d_out[N, d]``; rows and slots of no expert get 0."""
-    _check_tensors(d_out=d_out, y=y, weights=weights)
-    _check_routes(routes)
-    return list(_ext.load().combine_experts_backward(d_out, y, weights, *routes))
+    try:
+        order, offsets, position = routes
+        return list((_ops or _load()).combine_experts_backward(d_out, y, weights, order, offsets, position))
+    except (TypeError, ValueError) as error:
+        _refuse(error, routes, d_out=d_out, y=y, weights=weights)
