@@ -189,6 +189,8 @@ template <typename TY, typename T, int V, int J, bool PARTS>
 __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
                                                       const int32_t *__restrict__ position, int64_t N, int top_k, int tpr,
                                                       int parts, T *__restrict__ out) {
+  griddep_wait();
+  griddep_launch();
   const int64_t stride = (int64_t)gridDim.x * (256 / tpr);
   int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   int p[J], ahead[J];
@@ -243,6 +245,8 @@ template <typename T, int V, int U>
 __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restrict__ d_out, const T *__restrict__ y, int d,
                                                                const float *__restrict__ weights, RoutePlan p,
                                                                T *__restrict__ dy, float *__restrict__ d_weights) {
+  griddep_wait();
+  griddep_launch();
   const int lane = threadIdx.x & 31;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (r >= p.R) return;
@@ -292,17 +296,16 @@ int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32
   while (tpr < 256 && tpr * (vec ? V : 1) < d) tpr *= 2;
   const unsigned grid = (unsigned)std::min<int64_t>(cdiv(N, 256 / tpr), 8 * num_sms());
   auto run = [&](auto v, auto j, auto several) {
-    combine_kernel<TY, T, v(), j(), several()><<<grid, 256, 0, st>>>(y, R, d, w, pos, N, top_k, tpr, parts, out);
+    return launch_pdl(combine_kernel<TY, T, v(), j(), several()>, dim3(grid), dim3(256), 0, st, y, R, d, w, pos, N, top_k, tpr, parts, out);
   };
   auto by_slots = [&](auto v, auto several) {
     // (elements one by one are bound by instructions, not by loads on their way: one slot after the other)
-    if (top_k == 1 || v() == 1) run(v, std::integral_constant<int, 1>{}, several);
-    else if (top_k == 2) run(v, std::integral_constant<int, 2>{}, several);
-    else run(v, std::integral_constant<int, 4>{}, several);
+    if (top_k == 1 || v() == 1) return run(v, std::integral_constant<int, 1>{}, several);
+    if (top_k == 2) return run(v, std::integral_constant<int, 2>{}, several);
+    return run(v, std::integral_constant<int, 4>{}, several);
   };
-  auto by_parts = [&](auto v) { parts == 1 ? by_slots(v, std::false_type{}) : by_slots(v, std::true_type{}); };
-  vec ? by_parts(std::integral_constant<int, V>{}) : by_parts(std::integral_constant<int, 1>{});
-  FGMM_LAUNCH_CHECK("combine_kernel");
+  auto by_parts = [&](auto v) { return parts == 1 ? by_slots(v, std::false_type{}) : by_slots(v, std::true_type{}); };
+  FGMM_CUDA_TRY(vec ? by_parts(std::integral_constant<int, V>{}) : by_parts(std::integral_constant<int, 1>{}));
   return FGMM_OK;
 }
 
@@ -312,11 +315,10 @@ int combine_backward_t(const T *g, const T *y, int d, const float *w, const Rout
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(dy) % 16 == 0;
   const unsigned grid = (unsigned)cdiv(p.R, 4);
-  if (!vec) combine_backward_kernel<T, 1, 4><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
-  else if (d <= 32 * V) combine_backward_kernel<T, V, 1><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
-  else if (d <= 64 * V) combine_backward_kernel<T, V, 2><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
-  else combine_backward_kernel<T, V, 4><<<grid, 128, 0, st>>>(g, y, d, w, p, dy, dw);
-  FGMM_LAUNCH_CHECK("combine_backward_kernel");
+  auto *kernel = !vec ? combine_backward_kernel<T, 1, 4>
+                 : d <= 32 * V ? combine_backward_kernel<T, V, 1>
+                 : d <= 64 * V ? combine_backward_kernel<T, V, 2> : combine_backward_kernel<T, V, 4>;
+  FGMM_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(128), 0, st, g, y, d, w, p, dy, dw));
   return FGMM_OK;
 }
 

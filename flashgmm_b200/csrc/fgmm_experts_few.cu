@@ -71,6 +71,8 @@ template <typename T, bool VEC, int RW>
 __global__ void __launch_bounds__(kThreads) few_forward_kernel(const T *__restrict__ x, const T *__restrict__ w, int64_t N, int d_in,
                                                                int d_out, RoutePlan p, T *__restrict__ y) {
   __shared__ float4 s_x[RW][kDepth / 4];
+  griddep_wait();
+  griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = (int)p.R;
   const int r0 = blockIdx.x * RW, r1 = min(R, r0 + RW), o0 = (blockIdx.y * kWarps + warp) * kOuts;
   for (int r = r0; r < r1;) {
@@ -124,6 +126,8 @@ __global__ void __launch_bounds__(kThreads) few_inputs_kernel(const T *__restric
                                                               RoutePlan p, int part, float *__restrict__ dx) {
   __shared__ float s_g[RW][kDepth];
   __shared__ float4 s_sum[kWarps][32];
+  griddep_wait();
+  griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = (int)p.R;
   const int r0 = blockIdx.x * RW, r1 = min(R, r0 + RW), c = (blockIdx.y * 32 + lane) * 4, left = d_in - c;
   const int k_begin = blockIdx.z * part, k_end = min(d_out, k_begin + part);
@@ -188,6 +192,8 @@ __global__ void __launch_bounds__(kThreads) few_weights_kernel(const T *__restri
                                                                int d_out, RoutePlan p, int spans, T *__restrict__ dw) {
   __shared__ int s_point[kPoints];
   __shared__ float s_g[kPoints][32];
+  griddep_wait();
+  griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = (int)p.R;
   const int e = blockIdx.y, o_tile = blockIdx.x / spans * 32, o0 = o_tile + warp * kOuts, c0 = blockIdx.x % spans * kSpan * 128;
   int lo, hi;
@@ -240,9 +246,8 @@ template <typename T, bool VEC>
 int forward_t(const T *x, const T *w, int64_t N, int d_in, int d_out, const RoutePlan &p, T *y, cudaStream_t st) {
   const int rows = window_rows(p.R, p.K);
   const dim3 grid((unsigned)cdiv(p.R, rows), (unsigned)cdiv(d_out, kWarps * kOuts));
-  if (rows == 8) few_forward_kernel<T, VEC, 8><<<grid, kThreads, 0, st>>>(x, w, N, d_in, d_out, p, y);
-  else few_forward_kernel<T, VEC, 2><<<grid, kThreads, 0, st>>>(x, w, N, d_in, d_out, p, y);
-  FGMM_LAUNCH_CHECK("few_forward_kernel");
+  if (rows == 8) FGMM_CUDA_TRY(launch_pdl(few_forward_kernel<T, VEC, 8>, grid, dim3(kThreads), 0, st, x, w, N, d_in, d_out, p, y));
+  else FGMM_CUDA_TRY(launch_pdl(few_forward_kernel<T, VEC, 2>, grid, dim3(kThreads), 0, st, x, w, N, d_in, d_out, p, y));
   return FGMM_OK;
 }
 
@@ -250,17 +255,15 @@ template <typename T, bool VEC>
 int inputs_t(const T *dy, const T *w, int d_in, int d_out, const RoutePlan &p, int parts, float *dx, cudaStream_t st) {
   const int part = (int)cdiv(d_out, parts), rows = window_rows(p.R, p.K);
   const dim3 grid((unsigned)cdiv(p.R, rows), (unsigned)cdiv(d_in, 128), parts);
-  if (rows == 8) few_inputs_kernel<T, VEC, 8><<<grid, kThreads, 0, st>>>(dy, w, d_in, d_out, p, part, dx);
-  else few_inputs_kernel<T, VEC, 2><<<grid, kThreads, 0, st>>>(dy, w, d_in, d_out, p, part, dx);
-  FGMM_LAUNCH_CHECK("few_inputs_kernel");
+  if (rows == 8) FGMM_CUDA_TRY(launch_pdl(few_inputs_kernel<T, VEC, 8>, grid, dim3(kThreads), 0, st, dy, w, d_in, d_out, p, part, dx));
+  else FGMM_CUDA_TRY(launch_pdl(few_inputs_kernel<T, VEC, 2>, grid, dim3(kThreads), 0, st, dy, w, d_in, d_out, p, part, dx));
   return FGMM_OK;
 }
 
 template <typename T, bool VEC>
 int weights_t(const T *dy, const T *x, int64_t N, int d_in, int d_out, const RoutePlan &p, T *dw, cudaStream_t st) {
   const int spans = (int)cdiv(d_in, kSpan * 128);
-  few_weights_kernel<T, VEC><<<dim3((unsigned)(cdiv(d_out, 32) * spans), p.K), kThreads, 0, st>>>(dy, x, N, d_in, d_out, p, spans, dw);
-  FGMM_LAUNCH_CHECK("few_weights_kernel");
+  FGMM_CUDA_TRY(launch_pdl(few_weights_kernel<T, VEC>, dim3((unsigned)(cdiv(d_out, 32) * spans), p.K), dim3(kThreads), 0, st, dy, x, N, d_in, d_out, p, spans, dw));
   return FGMM_OK;
 }
 

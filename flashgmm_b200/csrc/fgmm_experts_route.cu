@@ -530,6 +530,13 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
   __shared__ uint64_t s_cand[kRouteWarps][L == 32 ? 64 : 1];  // candidates and their order (whole warps)
   extern __shared__ float s_bias[];  // [VPT * L], zeros behind K
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, seg = lane / L;
+  const int64_t stride = (int64_t)gridDim.x * kRouteWarps * RPW;
+  int64_t n = ((int64_t)blockIdx.x * kRouteWarps + warp) * RPW + seg;  // the warp's first row is n - seg
+  auto at = [&](int64_t r) { return scores + (r < a.N ? r : a.N - 1) * a.stride; };
+  griddep_wait();
+  griddep_launch();
+  Row<T, VPT> raw;
+  if (n - seg < a.N) load_row<T, VPT, V, L>(at(n), a.K, l, raw);
   float bmax = 0.0f;  // the largest finite |bias|
   if (a.bias) {
     for (int c = threadIdx.x; c < VPT * L; c += blockDim.x) s_bias[c] = c < a.K ? __ldg(a.bias + c) : 0.0f;
@@ -540,12 +547,7 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
     }
     bmax = seg_max<32>(bmax);
   }
-  const int64_t stride = (int64_t)gridDim.x * kRouteWarps * RPW;
-  int64_t n = ((int64_t)blockIdx.x * kRouteWarps + warp) * RPW + seg;  // the warp's first row is n - seg
   if (n - seg >= a.N) return;
-  auto at = [&](int64_t r) { return scores + (r < a.N ? r : a.N - 1) * a.stride; };
-  Row<T, VPT> raw;
-  load_row<T, VPT, V, L>(at(n), a.K, l, raw);
   for (;;) {
     const int64_t next = n + stride;
     constexpr bool kAhead = VPT <= 16;  // the next row is on its way while this one is decided
@@ -572,6 +574,8 @@ __global__ void __launch_bounds__(128, DENSE ? 1 : 12) route_backward_kernel(con
                                                              const int32_t *__restrict__ indices, const RouteArgs a,
                                                              T *__restrict__ dz) {
   const int lane = threadIdx.x & 31, l = lane % L;
+  griddep_wait();
+  griddep_launch();
   const int64_t stride = (int64_t)gridDim.x * (128 / L);
   for (int64_t n = (int64_t)blockIdx.x * (128 / L) + threadIdx.x / L; n - lane / L < a.N; n += stride) {
     const bool exists = n < a.N;
@@ -669,8 +673,7 @@ int route_forward_t(const T *z, const RouteArgs &a, float *w, int32_t *idx, cuda
     // every warp slot of the device once (64 warps an SM), so that the rows after the first are prefetched
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, kRouteWarps * (32 / lanes())), (int64_t)num_sms() * 64 / kRouteWarps);
     const size_t smem = a.bias ? vpt() * lanes() * sizeof(float) : 0;
-    route_kernel<T, vpt(), v(), lanes()><<<grid, 32 * kRouteWarps, smem, st>>>(z, a, w, idx);
-    FGMM_LAUNCH_CHECK("route_kernel");
+    FGMM_CUDA_TRY(launch_pdl(route_kernel<T, vpt(), v(), lanes()>, dim3(grid), dim3(32 * kRouteWarps), smem, st, z, a, w, idx));
     return FGMM_OK;
   });
 }
@@ -681,11 +684,9 @@ int route_backward_t(const float *dw, const T *z, const int32_t *idx, const Rout
                    reinterpret_cast<uintptr_t>(dz) % 16 == 0 && a.K * sizeof(T) % 16 == 0;
   return by_row_width<T>(a.K, a.top_k, vec, [&](auto vpt, auto v, auto lanes) {
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, 128 / lanes()), (int64_t)num_sms() * 16);
-    if (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)
-      route_backward_kernel<T, vpt(), v(), lanes(), true><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
-    else
-      route_backward_kernel<T, vpt(), v(), lanes(), false><<<grid, 128, 0, st>>>(dw, z, idx, a, dz);
-    FGMM_LAUNCH_CHECK("route_backward_kernel");
+    const bool dense = a.func == FGMM_SCORE_SOFTMAX && !a.renorm;
+    FGMM_CUDA_TRY(launch_pdl(dense ? route_backward_kernel<T, vpt(), v(), lanes(), true> : route_backward_kernel<T, vpt(), v(), lanes(), false>,
+                             dim3(grid), dim3(128), 0, st, dw, z, idx, a, dz));
     return FGMM_OK;
   });
 }
