@@ -16,13 +16,13 @@ __device__ __forceinline__ float warp_sum(float v) {
 
 // ----------------------------------------------------------------------------- grouping
 //
-// A stable counting sort of the R routes by expert (routes without one last): every block counts its 4096 routes per key,
-// the counts are summed over the blocks in order, and the same blocks place them (524,288 routes over 1,024 experts: 30 us
-// with the counts key by key and 2,048 routes a block, whose place kernel waited for a line per key).  Up to 4096 routes
-// are one block's work and one launch.
-// A warp takes 256 routes in their order, 32 at a time; lanes with the same key find each other with one match
-// instruction.
-constexpr int kSortWarps = 16, kSortRounds = 8, kSortItems = kSortWarps * kSortRounds * 32, kSortThreads = kSortWarps * 32;
+// A stable counting sort of the R routes by expert (routes without one last): every block counts its routes per key, the counts
+// are summed over the blocks in order, and the same blocks place them.  Up to 4,096 routes are one block's work and one
+// launch.  A warp takes its routes in their order, 32 at a time (ROUNDS times); lanes with the same key find each other with one
+// match instruction.  Latency, not bytes, bounds it: 524,288 routes over 1,024 experts take 16 us with four rounds a warp
+// and 21 us with eight, 2,097,152 routes over 256 (whose blocks' counts are a long column) 45 and 33 us.
+constexpr int kSortWarps = 16, kSortThreads = kSortWarps * 32;
+constexpr int sort_items(int rounds) { return kSortThreads * rounds; }
 
 __device__ __forceinline__ int route_key(const int32_t *indices, int64_t i, int K) {
   const int e = __ldg(indices + i);
@@ -30,6 +30,7 @@ __device__ __forceinline__ int route_key(const int32_t *indices, int64_t i, int 
 }
 
 // counts[block][key]
+template <int ROUNDS>
 __global__ void __launch_bounds__(kSortThreads) group_count_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
                                                                    int32_t *__restrict__ counts) {
   extern __shared__ int s_hist[];
@@ -38,9 +39,9 @@ __global__ void __launch_bounds__(kSortThreads) group_count_kernel(const int32_t
   __syncthreads();
   griddep_wait();
   griddep_launch();  // after the wait: the place kernel reads the indices before its own
-  const int64_t base = (int64_t)blockIdx.x * kSortItems + threadIdx.x;
+  const int64_t base = (int64_t)blockIdx.x * sort_items(ROUNDS) + threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < kSortItems / kSortThreads; ++i)
+  for (int i = 0; i < ROUNDS; ++i)
     if (base + i * kSortThreads < R) atomicAdd(s_hist + route_key(indices, base + i * kSortThreads, K), 1);
   __syncthreads();
   for (int e = threadIdx.x; e < keys; e += kSortThreads) counts[(int64_t)blockIdx.x * keys + e] = s_hist[e];
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(32 * kScanParts) group_scan_kernel(int32_t *__
 }
 
 // Places this block's routes; with ONE it is the only block and its own counts are the totals.
-template <bool ONE>
+template <bool ONE, int ROUNDS>
 __global__ void __launch_bounds__(kSortThreads) group_place_kernel(const int32_t *__restrict__ indices, int64_t R, int K,
                                                                    const int32_t *__restrict__ counts, const int32_t *__restrict__ totals,
                                                                    int32_t *__restrict__ order, int32_t *__restrict__ offsets,
@@ -94,12 +95,12 @@ __global__ void __launch_bounds__(kSortThreads) group_place_kernel(const int32_t
   for (int i = threadIdx.x; i < kSortWarps * keys / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(s_count)[i] = 0u;
   if (ONE) griddep_wait();
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kSortItems + warp * kSortRounds * 32 + lane;
-  int key[kSortRounds], rank[kSortRounds];
+  const int64_t base = (int64_t)blockIdx.x * sort_items(ROUNDS) + warp * ROUNDS * 32 + lane;
+  int key[ROUNDS], rank[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) key[r] = base + r * 32 < R ? route_key(indices, base + r * 32, K) : -1;
+  for (int r = 0; r < ROUNDS; ++r) key[r] = base + r * 32 < R ? route_key(indices, base + r * 32, K) : -1;
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const unsigned same = __match_any_sync(kFull, key[r]);
     const int below = __popc(same & ((1u << lane) - 1u));
     const int seen = key[r] >= 0 ? mine[key[r]] : 0;
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kSortThreads) group_place_kernel(const int32_t
     __syncthreads();
   }
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     if (key[r] < 0) continue;
     const int at = s_start[key[r]] + mine[key[r]] + rank[r];
     order[at] = (int32_t)(base + r * 32);
@@ -324,7 +325,8 @@ int combine_backward_t(const T *g, const T *y, int d, const float *w, const Rout
 
 }  // namespace
 
-static int sort_blocks(int64_t R) { return (int)std::max<int64_t>(1, cdiv(R, kSortItems)); }
+static int sort_rounds(int64_t R) { return R <= sort_items(8) || R > (1 << 20) ? 8 : 4; }
+static int sort_blocks(int64_t R) { return (int)std::max<int64_t>(1, cdiv(R, sort_items(sort_rounds(R)))); }
 
 size_t group_workspace_bytes(int64_t R, int K) {
   Carve c(nullptr);
@@ -342,19 +344,22 @@ int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32
   std::atomic<bool> &once = device_once_flag(8);
   if (!once.load(std::memory_order_acquire)) {
     const int most = (int)place_smem(kMaxExperts + 1);
-    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<true, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<false, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    FGMM_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<false, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     once.store(true, std::memory_order_release);
   }
   if (blocks == 1) {
-    FGMM_CUDA_TRY(launch_pdl(group_place_kernel<true>, dim3(1), dim3(kSortThreads), place_smem(keys), st, indices, R, K,
+    FGMM_CUDA_TRY(launch_pdl(group_place_kernel<true, 8>, dim3(1), dim3(kSortThreads), place_smem(keys), st, indices, R, K,
                              (const int32_t *)nullptr, (const int32_t *)nullptr, order, offsets, position));
     return FGMM_OK;
   }
-  FGMM_CUDA_TRY(launch_pdl(group_count_kernel, dim3(blocks), dim3(kSortThreads), keys * sizeof(int), st, indices, R, K, counts));
+  const bool eight = sort_rounds(R) == 8;
+  FGMM_CUDA_TRY(launch_pdl(eight ? group_count_kernel<8> : group_count_kernel<4>, dim3(blocks), dim3(kSortThreads), keys * sizeof(int), st,
+                           indices, R, K, counts));
   FGMM_CUDA_TRY(launch_pdl(group_scan_kernel, dim3((unsigned)cdiv(keys, 32)), dim3(32 * kScanParts), 0, st, counts, K, blocks, totals));
-  FGMM_CUDA_TRY(launch_pdl(group_place_kernel<false>, dim3(blocks), dim3(kSortThreads), place_smem(keys), st, indices, R, K, counts, totals,
-                           order, offsets, position));
+  FGMM_CUDA_TRY(launch_pdl(eight ? group_place_kernel<false, 8> : group_place_kernel<false, 4>, dim3(blocks), dim3(kSortThreads), place_smem(keys),
+                           st, indices, R, K, counts, totals, order, offsets, position));
   return FGMM_OK;
 }
 

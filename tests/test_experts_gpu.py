@@ -213,7 +213,8 @@ def test_route_gradient_of_masked_and_repeated_slots():
 
 
 # ------------------------------------------------------------------------------ grouping
-@pytest.mark.parametrize("N,k,K", [(1, 1, 1), (37, 4, 64), (2047, 1, 5), (2049, 3, 300), (5000, 8, 1024), (700, 2, 4096), (40000, 2, 17)])
+@pytest.mark.parametrize("N,k,K", [(1, 1, 1), (37, 4, 64), (2047, 1, 5), (2049, 3, 300), (5000, 8, 1024), (700, 2, 4096), (40000, 2, 17), (4096, 1, 3), (4097, 1, 3),
+                                   (350001, 3, 64)])
 def test_group_routes(N, k, K):
     idx = torch.randint(-1, K + 1, (N, k), generator=gen(N + K), dtype=torch.int32)  # some without an expert, some outside
     routes = C().group_routes(idx.to(DEV), K)
