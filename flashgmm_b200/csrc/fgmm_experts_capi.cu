@@ -15,7 +15,8 @@ int check_experts(int dtype, int64_t N, int K, int top_k) {
     return fail(FGMM_ERR_INVALID, "N must be >= 0, K and top_k >= 1 (got N=" + std::to_string(N) + " K=" + std::to_string(K) +
                                       " top_k=" + std::to_string(top_k) + ")");
   if (K > FGMM_MAX_EXPERTS) return fail(FGMM_ERR_UNSUPPORTED, "K > " + std::to_string(FGMM_MAX_EXPERTS) + " is not supported");
-  if (N > INT32_MAX / top_k) return fail(FGMM_ERR_UNSUPPORTED, "N top_k must be below 2^31");
+  // (row numbers a tile behind the last one stay in 32 bits)
+  if (N > (INT32_MAX - 1024) / top_k) return fail(FGMM_ERR_UNSUPPORTED, "N top_k must be at most 2^31 - 1025");
   return FGMM_OK;
 }
 
@@ -96,7 +97,7 @@ int fgmm_route_experts_backward(const float *d_weights, const void *scores, int3
 }
 
 size_t fgmm_group_routes_workspace_bytes(int64_t R, int32_t K) {
-  if (R < 0 || R > INT32_MAX || K < 1 || K > FGMM_MAX_EXPERTS) return 0;
+  if (R < 0 || R > INT32_MAX - 1024 || K < 1 || K > FGMM_MAX_EXPERTS) return 0;
   return group_workspace_bytes(R, K);
 }
 

@@ -129,7 +129,7 @@ std::tuple<Tensor, Tensor, Tensor> group_routes(const Tensor &indices, int64_t K
   TORCH_CHECK(indices.size(1) >= 1, "indices must have at least one column");
   TORCH_CHECK(K >= 1 && K <= FGMM_MAX_EXPERTS, "K must be in [1, ", FGMM_MAX_EXPERTS, "], got ", K);
   const int64_t R = indices.numel();
-  TORCH_CHECK(R <= INT32_MAX, "indices has 2^31 or more routes");
+  TORCH_CHECK(R <= INT32_MAX - 1024, "indices has more than 2^31 - 1025 routes");
   const torch::Device dev = indices.device();
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor idx = indices.contiguous();
@@ -160,7 +160,7 @@ Plan plan_of(const Tensor &order, const Tensor &offsets, const Tensor &position,
   check_shape(order, "order", {position.numel()});
   TORCH_CHECK(offsets.size(0) >= 2 && offsets.size(0) <= FGMM_MAX_EXPERTS + 1, "offsets must have K + 1 entries, K in [1, ",
               FGMM_MAX_EXPERTS, "]");
-  TORCH_CHECK(order.numel() <= INT32_MAX, "the plan has 2^31 or more routes");
+  TORCH_CHECK(order.numel() <= INT32_MAX - 1024, "the plan has more than 2^31 - 1025 routes");
   return {order.contiguous(), offsets.contiguous(), position.contiguous(), order.size(0), position.size(0),
           (int)offsets.size(0) - 1, (int)position.size(1)};
 }

@@ -94,7 +94,7 @@ def route_experts(scores, top_k, score_func="softmax", bias=None, n_groups=1, to
     choice only, to keep the experts' loads balanced.  With ``n_groups > 1`` the experts form equal
     consecutive groups and only the ``top_groups`` groups (default: all) with the largest sums of
     their two best biased values are chosen from.  Ties go to the lowest index; the order is decided on
-    64-bit values, without bias and groups on the scores themselves.  ``renormalize`` divides a
+    64-bit values, without bias and with all groups kept on the scores themselves.  ``renormalize`` divides a
     point's weights by their sum, ``scale`` multiplies them.
 
     A score of -inf or NaN is masked and +inf counts as the largest finite value; slots that no

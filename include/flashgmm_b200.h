@@ -199,7 +199,8 @@ int fgmm_em_stats_profiled(const float *X, const void *points, int64_t N, int32_
  *
  * Element types of scores, x, weight, y and their gradients: FGMM_F32, FGMM_BF16, FGMM_F16, one type in a
  * call; sums are held in fp32.  Weights, their gradients and the bias are fp32, indices int32.
- * K <= FGMM_MAX_EXPERTS, top_k <= FGMM_MAX_TOP_K, N top_k < 2^31.  N = 0 is allowed. */
+ * K <= FGMM_MAX_EXPERTS, N top_k <= 2^31 - 1025, top_k of the routing <= FGMM_MAX_TOP_K.  N = 0 is
+ * allowed.  All calls only enqueue work on `stream` and may be captured; each uses its own workspace. */
 #define FGMM_F32 0
 #define FGMM_BF16 1
 #define FGMM_F16 2
@@ -215,7 +216,7 @@ int fgmm_em_stats_profiled(const float *X, const void *points, int64_t N, int32_
  * moves the choice, not the weights).  With n_groups > 1 the K experts form equal consecutive
  * groups, and only the top_groups groups with the largest sums of their two best c stay.  Chosen
  * are the top_k largest c, best first, ties to the lowest index, the order decided on 64-bit
- * values (without bias and groups on the scores themselves).  weights[n][j] = scale * s, divided by the
+ * values (without bias and with all groups kept, on the scores themselves).  weights[n][j] = scale * s, divided by the
  * chosen ones' sum if `renormalize` (0 where that is 0).  A score of -inf or NaN is masked, +inf
  * counts as the largest finite fp32 value; a slot that no unmasked expert is left for has index -1
  * and weight 0. */

@@ -51,7 +51,7 @@ def _route(dtype=0, N=4, K=8, stride=8, top_k=2, func=0, n_groups=1, top_groups=
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=3), 1), (dict(N=-1), 1), (dict(K=0), 1), (dict(top_k=0), 1), (dict(top_k=9), 1), (dict(func=3), 1),
     (dict(n_groups=3), 1), (dict(n_groups=0), 1), (dict(n_groups=2, top_groups=3), 1), (dict(n_groups=2, top_groups=0), 1),
-    (dict(stride=-8), 1), (dict(K=4097, stride=4097), 2), (dict(K=64, top_k=33), 1), (dict(N=1 << 31), 2),
+    (dict(stride=-8), 1), (dict(K=4097, stride=4097), 2), (dict(K=64, top_k=33), 1), (dict(N=1 << 31), 2), (dict(N=(1 << 30) - 512), 2),
     (dict(z=None), 1), (dict(w=None), 1), (dict(i=None), 1), (dict(z=ctypes.c_void_p(4098)), 1),
     (dict(K=64, n_groups=64), 1)])
 def test_route_refusals(kw, code):
