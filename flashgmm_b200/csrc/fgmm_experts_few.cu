@@ -191,7 +191,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) few_weights_kernel(const T *__restrict__ dy, const T *__restrict__ x, int64_t N, int d_in,
                                                                int d_out, RoutePlan p, int spans, T *__restrict__ dw) {
   __shared__ int s_point[kPoints];
-  __shared__ float s_g[kPoints][32];
+  __shared__ __align__(16) float s_g[kPoints][32];
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = (int)p.R;

@@ -537,18 +537,22 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         c = SPLIT ? c + kSegment : x.c1;
         if constexpr (SPLIT) {
           if (live) {
-            auto add = [&](uint32_t from) {
+            auto add = [&](uint32_t from, bool smaller) {
 #pragma unroll
               for (int i = 0; i < HC / 32; ++i) {
                 float v[32];
                 tmem_ld32(from + i * 32, v);
                 tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) acc[i * 32 + k] += v[k];
+                for (int k = 0; k < 32; ++k) {
+                  const float sum = acc[i * 32 + k] + v[k];
+                  acc[i * 32 + k] = smaller && isnan(sum) ? acc[i * 32 + k] : sum;
+                }
               }
             };
-            add(lane_tmem + buf * NT);
-            if (c >= x.c1) add(lane_tmem + (2 + (count & 1)) * NT);
+            add(lane_tmem + buf * NT, false);
+            // an infinite operand's products with lower planes (of either sign, or zero) say nothing
+            if (c >= x.c1) add(lane_tmem + (2 + (count & 1)) * NT, true);
           }
         } else if (live) {
           for (int i = 0; i < HC / CW; ++i) {
@@ -699,7 +703,8 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const __nv_bfloat16 b0 = __float2bfloat16_rn(v[k]);
+          __nv_bfloat16 b0 = __float2bfloat16_rn(v[k]);
+          if (__hisinf(b0) && !isinf(v[k])) b0 = __ushort_as_bfloat16(v[k] > 0.0f ? 0x7f7f : 0xff7f);  // (rounded past the largest)
           float rest = v[k] - __bfloat162float(b0);
           if (!isfinite(rest)) rest = 0.0f;
           const __nv_bfloat16 b1 = __float2bfloat16_rn(rest);

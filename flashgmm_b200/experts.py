@@ -146,7 +146,7 @@ def expert_products(x, weight, routes):
     ``y[N top_k, d_out]``; rows behind ``offsets[K]`` (routes without an expert) are 0.
 
     ``x[N, d_in]`` and ``weight[K, d_out, d_in]`` of one type; gradients to both.  float32 operands run
-    on the tensor cores as three bf16 planes (24 bits together); an infinite entry gives NaN there."""
+    on the tensor cores as three bf16 planes (24 bits together)."""
     try:
         order, offsets, position = routes
         if (x.requires_grad or weight.requires_grad) and _grad_enabled():

@@ -244,7 +244,7 @@ int fgmm_group_routes(const int32_t *indices, int64_t R, int32_t K, int32_t *ord
 /* y[r] = weight[e] x[n] for every grouped row r (route order[r] of point n, expert e), x[N][d_in],
  * weight[K][d_out][d_in], y[N top_k][d_out]; rows of no expert are 0.  `order` and `offsets` are those of
  * fgmm_group_routes: entries out of range are treated as rows of no expert, never read through.  x and weight start on 16-byte
- * boundaries.  float32 operands run as three bf16 planes (24 bits): a row with an infinite entry gives NaN. */
+ * boundaries.  float32 operands run as three bf16 planes (24 bits together). */
 size_t fgmm_expert_products_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                             int32_t d_out, int32_t top_k);
 int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, const void *weight,

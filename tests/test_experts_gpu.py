@@ -321,6 +321,49 @@ def test_products_keep_infinities_where_they_belong(dtype):
     assert torch.equal(gx[untouched.to(DEV)], gx0[untouched.to(DEV)])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,k,K,d_in,d_out", [(21, 3, 32, 136, 256), (9, 5, 40, 72, 200), (12, 32, 40, 64, 72), (50, 2, 4096, 64, 64), (7, 3, 4096, 20, 31),
+                                              (2100, 3, 3, 128, 128), (515, 7, 9, 320, 256), (65, 1, 1, 1025, 2050)])
+def test_products_of_more_plans(N, k, K, d_in, d_out, dtype):
+    """Many slots, odd numbers of them, the largest number of experts, one expert with everything."""
+    test_products_and_gradients(N, k, K, d_in, d_out, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [3, 300])
+def test_products_of_infinite_and_largest_values(N, dtype):
+    """Infinite, NaN and largest entries in either operand give what 64 bits give, on the CUDA cores (few rows an expert) and on
+    the tensor cores.  (The scaled columns keep the largest value's products within the type.)"""
+    k, K, d_in, d_out = 1, 4, 136, 72
+    x, w = torch.randn(N, d_in, generator=gen(1)), torch.randn(K, d_out, d_in, generator=gen(2))
+    dy = torch.randn(N * k, d_out, generator=gen(3))
+    w[:, :, 5] *= 2.0 ** (-100 if dtype != torch.float16 else -14)
+    x, w, dy = x.to(dtype), w.to(dtype), dy.to(dtype)
+    x[0, 3], x[1, 130], x[2, 7] = float("inf"), float("-inf"), float("nan")
+    if N > 3:
+        x[3:100:2, 5], x[4:100:2, 5] = torch.finfo(dtype).max, torch.finfo(dtype).min
+        w[1, 2, 9] = float("-inf")
+    idx = torch.arange(N * k, dtype=torch.int32).reshape(N, k) % K
+    routes = C().group_routes(idx.to(DEV), K)
+    order, offsets = routes.order.cpu(), routes.offsets.cpu()
+    y, ya, dx, dxa, dw, dwa = ref.products(x, w, order, offsets, k, dy)
+    gx, gw = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes)
+    counts = offsets[1:] - offsets[:-1]
+    for got, want, size, d, what in ((C().expert_products(x.to(DEV), w.to(DEV), routes), y, ya, d_in, "y"), (gx, dx, dxa, d_out, "dx"),
+                                     (gw, dw, dwa, max(1, int(counts.max())), "dw")):
+        got, big = got.cpu(), torch.finfo(dtype).max
+        plain = size <= big / 2  # (beyond it a sum on the way may pass the type's largest)
+        odd = ~torch.isfinite(want)
+        assert torch.equal(torch.isnan(got) & odd, torch.isnan(want)), what
+        inf = torch.isinf(want)
+        assert torch.equal(got.double()[inf], want[inf]), what
+        assert torch.isfinite(got[plain]).all(), what
+        z = torch.zeros_like(want)
+        err = torch.where(plain, (got.double() - want).abs(), z)
+        tol = 2 * d * 2.0 ** -23 * size + 1.001 * HALF_STEP[dtype] * want.abs() + (2.0 ** -24 if dtype == torch.float16 else 0)
+        assert (err <= torch.where(plain, tol, z)).all(), what
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_products_of_a_plan_that_holds_nonsense(dtype):
     """Entries out of range are read as rows of no expert and never followed."""
@@ -436,6 +479,29 @@ def test_layer_gradient_of_some_inputs_only():
     # a broadcast gradient (of sum()) and an integer output that takes none
     w, idx = C().route_experts((x @ router).requires_grad_(), 2)
     assert w.requires_grad and not idx.requires_grad
+
+
+def test_two_products_one_after_the_other():
+    """Grouped rows as points of one slot each: their plan is the identity, and the layer of two products has its gradients."""
+    N, k, K, d, hidden = 60, 2, 5, 24, 40
+    x, w1, w2 = (torch.randn(*s, generator=gen(i)).to(DEV).requires_grad_() for i, s in enumerate(((N, d), (K, hidden, d), (K, d, hidden))))
+    idx, wt = plan(N, k, K, 9).to(DEV), torch.rand(N, k, generator=gen(5)).to(DEV)
+    routes = C().group_routes(idx, K)
+    same = C().group_routes(idx.flatten()[routes.order.long()][:, None].contiguous(), K)
+    live = int(routes.offsets[-1])
+    assert torch.equal(same.order, torch.arange(N * k, dtype=torch.int32, device=DEV)) and torch.equal(same.offsets, routes.offsets)
+    assert torch.equal(same.position[:live, 0], same.order[:live]) and (same.position[live:] == -1).all()
+    h = torch.nn.functional.silu(C().expert_products(x, w1, routes))
+    out = C().combine_experts(C().expert_products(h, w2, same), wt, routes)
+    grads = torch.autograd.grad(out.sum(), (x, w1, w2))
+    x64, w164, w264 = (t.detach().double().requires_grad_() for t in (x, w1, w2))
+    e = idx.long().clamp(min=0)
+    h64 = torch.nn.functional.silu(torch.einsum("nd,nkhd->nkh", x64, w164[e]))
+    out64 = (torch.einsum("nkh,nkdh->nkd", h64, w264[e]) * (wt.double() * (idx >= 0))[:, :, None]).sum(1)
+    want = torch.autograd.grad(out64.sum(), (x64, w164, w264))
+    # (sums of at most N k + d + hidden fp32 terms in a row)
+    for got, exact in zip((out.detach(), *grads), (out64.detach(), *want)):
+        assert float((got.double() - exact).abs().max()) <= 2 * (N * k + d + hidden) * 2.0 ** -23 * float(exact.abs().max())
 
 
 def test_no_points():
@@ -594,6 +660,22 @@ def test_models_route_by_their_responsibilities(model):
     assert float((out.detach().double() - exact).abs().max()) <= 1e-5 * float(exact.abs().max())
     out.sum().backward()
     assert weight.grad.shape == weight.shape and torch.isfinite(weight.grad).all()
+
+
+def test_model_experts_pass_gradients_to_the_points():
+    from flashgmm_b200 import native_wrapper
+    from flashgmm_b200.data import make_mixture
+    N, K, d, k, d_out = 400, 6, 12, 2, 20
+    X = make_mixture(N, K, d, seed=5)[0].to(DEV)
+    m = native_wrapper.NativeFlashGMM(K, d, max_iter=3)
+    m.fit(X)
+    w, idx = m.route(X, k)
+    weight = torch.randn(K, d_out, d, device=DEV)
+    points = X.clone().requires_grad_()
+    grad, = torch.autograd.grad(m.mix_experts(points, weight, k).sum(), points)
+    exact = (weight.double().sum(1)[idx.long()] * w.double()[:, :, None]).sum(1)  # the gate has no gradient
+    size = (weight.double().abs().sum(1)[idx.long()] * w.double()[:, :, None]).sum(1)
+    assert ((grad.double() - exact).abs() <= 2 * (d_out + k) * 2.0 ** -23 * size).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
