@@ -6,5 +6,8 @@ Public surface (mirrors the reference's ``flash_gmm_native`` op module and its
 * :mod:`flashgmm_b200.flash_gmm_native` -- ``flash_em_fused`` plus the split
   ``em_stats`` / ``em_update`` used by sharded multi-GPU fits.
 * :class:`flashgmm_b200.native_wrapper.NativeFlashGMM`.
+* :mod:`flashgmm_b200.experts` -- a mixture of experts over the same components: routing,
+  grouping, the experts' products and the weighted join, with their gradients (also in
+  ``flash_gmm_native``).
 """
 __version__ = "0.1.0"
