@@ -17,9 +17,11 @@ constexpr unsigned kFull = 0xffffffffu;
 // chosen ones' sum where asked, times the scale.  Without bias and groups the order of c is that of z,
 // and z itself is compared.  A score of -inf or NaN is masked; +inf counts as the largest finite value.
 //
-// A row is held in registers by 8, 16 or 32 lanes.  c is fp32; the order is defined on 64-bit values, so a row where
-// two deciding values lie closer than the fp32 error allows (and are not the same score and bias) is decided
-// again in fp64, from its scores, by route_row64.
+// A row is held in registers by 8, 16 or 32 lanes.  c is fp32; the order is defined on 64-bit values, so where two deciding
+// values lie closer than the fp32 error allows (and are not the same score and bias), they are compared again in fp64:
+// the groups next to the border between those that stay and go, the chosen ones a lane each.  Two values more than asked
+// are chosen, so that a gap behind the last slot shows that nothing else can belong there; a row without one is decided
+// whole, by route_row64.
 
 // Unsigned order of floats; 0 is below every float.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -52,6 +54,44 @@ __device__ __forceinline__ float sigmoid(float z) {
 
 // (v, i) comes before (w, j): a larger value, or an equal one of a lower index.
 __device__ __forceinline__ bool before(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
+
+// c of one expert in 64 bits; m and total are the softmax's.  Masked values are -inf.
+__device__ __noinline__ double exact_value(float z, float bias, int func, float m, double total) {
+  double s = z;
+  if (!(z > -INFINITY)) return -INFINITY;
+  if (func == FGMM_SCORE_SOFTMAX) s = exp(s - (double)m) / total;
+  else if (func == FGMM_SCORE_SIGMOID) s = 1.0 / (1.0 + exp(-s));
+  return fmax(s + (double)bias, -INFINITY);  // -inf for NaN
+}
+
+// The sum of a row's softmax in 64 bits; L lanes have a row.
+template <typename T, int L> __device__ __noinline__ double exact_total(const T *row, int K, float m) {
+  double total = 0.0;
+#pragma unroll 1
+  for (int c = threadIdx.x % L; c < K; c += L) total += exp((double)score_at(row, c) - (double)m);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
+  return total;
+}
+
+// The sum of group g's two best, in 64 bits, the whole warp on it.
+template <typename T> __device__ __noinline__ double exact_group(const T *row, const RouteArgs &a, int g, float m, double total) {
+  double b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll 1
+  for (int c = g * a.per + (int)(threadIdx.x & 31); c < (g + 1) * a.per; c += 32) {
+    const double x = exact_value(score_at(row, c), a.bias ? __ldg(a.bias + c) : 0.0f, a.func, m, total);
+    b2 = fmax(b2, fmin(b1, x));
+    b1 = fmax(b1, x);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+    b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+    b1 = fmax(b1, o1);
+  }
+  return b2 > -INFINITY ? b1 + b2 : b1;
+}
 
 // Decides one row in 64 bits, the whole warp on it: a lane holds the values of columns lane, lane + 32, ...
 // Lane j returns slot j's expert.  Rare; its values are kept in local memory (indexed at run time), because
@@ -216,9 +256,10 @@ __device__ __forceinline__ void top_two(float &b1, float &b2, float v1, float v2
   b1 = fmaxf(b1, v1);
 }
 
-// Masks all but the top_groups groups of a warp's row.  False where the sums that decide lie too close.
-template <int VPT, int V>
-__device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a, int lane, float bmax, float tol, float2 *s_group) {
+// Masks all but the top_groups groups of a warp's row.
+template <typename T, int VPT, int V>
+__device__ __forceinline__ void keep_groups(float (&c)[VPT], const T *row, const RouteArgs &a, int lane, float m, float bmax, float tol,
+                                            float2 *s_group) {
   const int per = a.per, span = per / V;
   // a group is `span` neighbouring lanes of one pack of V: all groups' best two meet in log2 span steps
   const bool even = per % V == 0 && span <= 32 && (span & (span - 1)) == 0;
@@ -226,7 +267,7 @@ __device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a,
   float2 mine = make_float2(-INFINITY, 0.0f);  // lane g: group g's sum, and the magnitudes in it
   auto put = [&](int g, float b1, float b2) {
     const bool two = b2 > -INFINITY;
-    // (a live group's sum stays above -inf; its magnitude then is inf, and the row is decided in 64 bits)
+    // (a live group's sum stays above -inf; its magnitude then is inf, and all groups are compared in 64 bits)
     s_group[g] = make_float2(two ? fmaxf(b1 + b2, -FLT_MAX) : b1, fabsf(b1) + (two ? fabsf(b2) : 0.0f));
   };
   __syncwarp();
@@ -267,6 +308,26 @@ __device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a,
     if (lane == g) key = 0u;
   }
   const uint32_t high = __reduce_max_sync(kFull, key);  // the largest that goes
+  const float lo = of_key(low), hi = of_key(high), cut = 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
+  if (high != 0u && !(lo - hi > cut)) {
+    // those that could be on either side of the border
+    const bool in = mine.x - hi > cut, out = !(mine.x > -INFINITY) || lo - mine.x > cut, near = !in && !out;
+    kept = __ballot_sync(kFull, in);
+    const unsigned some = __ballot_sync(kFull, near);
+    const double total = a.func == FGMM_SCORE_SOFTMAX ? exact_total<T, 32>(row, a.K, m) : 0.0;
+    double sum = -INFINITY;
+    for (unsigned left = some; left; left &= left - 1) {
+      const int g = __ffs(left) - 1;
+      const double x = exact_group(row, a, g, m, total);
+      if (lane == g) sum = x;
+    }
+    int rank = __popc(kept);
+    for (unsigned left = some; left; left &= left - 1) {
+      const int g = __ffs(left) - 1;
+      if (before(__shfl_sync(kFull, sum, g), g, sum, lane)) ++rank;
+    }
+    kept |= __ballot_sync(kFull, near && rank < a.top_groups);
+  }
   if (even) {
 #pragma unroll
     for (int i = 0; i < VPT; i += V) {
@@ -280,7 +341,6 @@ __device__ __forceinline__ bool keep_groups(float (&c)[VPT], const RouteArgs &a,
     for (int i = 0; i < VPT; ++i)
       if (!((kept >> (column<V, 32>(i, lane) / per & 31)) & 1u)) c[i] = -INFINITY;
   }
-  return high == 0u || of_key(low) - of_key(high) > 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
 }
 
 // The row's `rounds` largest values in order (lane j: the j'th, -1 where none is left): the lanes' best ones are compared,
@@ -421,22 +481,22 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
 
 constexpr int kRouteWarps = 4;
 
-template <typename T, int VPT, int V, int L>
+// BY_VALUE: with a bias or groups, where the values c decide; else the scores do.
+template <typename T, int VPT, int V, int L, bool BY_VALUE>
 __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T, VPT> &raw, const RouteArgs &a, int l, const float *s_bias,
                                           float bmax, uint64_t *s_cand, float *weights, int32_t *indices) {
   // fp32 values of c are off by at most a few 2^-23 of |s| and |bias|: two that differ by more than this (times
   // their sizes) are in the right order
   constexpr float kTol = 1.0f / (1 << 20);
-  const bool by_value = a.bias != nullptr || a.n_groups > 1;
   float c[VPT], m = 0.0f, total = 1.0f, inv = 1.0f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) c[i] = to_f32(raw.v[i]);
-  if (L < 32 || by_value || (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)) {  // (pick_few takes scores as they are)
+  if (L < 32 || BY_VALUE || (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)) {  // (pick_few takes scores as they are)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) c[i] = clean(c[i]);
   }
-  if (a.func == FGMM_SCORE_SOFTMAX && (by_value || !a.renorm)) {
-    if (by_value) {
+  if (a.func == FGMM_SCORE_SOFTMAX && (BY_VALUE || !a.renorm)) {
+    if constexpr (BY_VALUE) {
       uint32_t live[(VPT + 31) / 32] = {};
 #pragma unroll
       for (int i = 0; i < VPT; ++i) live[i / 32] |= (uint32_t)(c[i] > -INFINITY) << (i & 31);
@@ -451,8 +511,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
       total = softmax_terms<VPT, L>(e, m);
     }
   }
-  bool sure = true;
-  if (by_value) {
+  if constexpr (BY_VALUE) {
     if (a.func == FGMM_SCORE_SIGMOID) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) c[i] = c[i] > -INFINITY ? sigmoid(c[i]) : -INFINITY;
@@ -462,17 +521,17 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
       for (int i = 0; i < VPT; ++i) c[i] = fmaxf(c[i] + s_bias[column<V, L>(i, l)], -INFINITY);  // -inf for NaN
     }
     if constexpr (L == 32)
-      if (a.n_groups > 1) sure = keep_groups<VPT, V>(c, a, l, bmax, kTol, reinterpret_cast<float2 *>(s_cand));
+      if (a.n_groups > 1) keep_groups<T, VPT, V>(c, row, a, l, m, bmax, kTol, reinterpret_cast<float2 *>(s_cand));
   }
-  // one choice more than asked, where its distance from the last one is looked at
-  const int rounds = min(L, by_value ? a.top_k + 1 : a.top_k);
+  const bool rounded = BY_VALUE && (a.func != FGMM_SCORE_GIVEN || a.bias);  // c is not exact
+  const int rounds = min(L, rounded ? a.top_k + 2 : a.top_k);
   int chosen = -1;
   float value = 0.0f;
   bool done = false;
   if constexpr (L == 32) {
     done = pick_few<VPT, V>(c, rounds, l, s_cand, [&](int col) {
       float v = score_at(row, col);
-      if (by_value) {
+      if constexpr (BY_VALUE) {
         if (a.func == FGMM_SCORE_SOFTMAX) v = expf(v - m) * inv;
         else if (a.func == FGMM_SCORE_SIGMOID) v = sigmoid(v);
         if (a.bias) v += s_bias[col];
@@ -485,17 +544,52 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
     }
   }
   if (!done) pick_by_lane<VPT, V, L>(c, rounds, l, chosen, value);
-  if (by_value) {
-    const float z = chosen >= 0 ? score_at(row, chosen) : 0.0f;
-    const float b = chosen >= 0 && a.bias ? s_bias[chosen] : 0.0f;
+  if (rounded) {
+    const bool have = chosen >= 0;
+    const float z = have ? score_at(row, chosen) : 0.0f, b = have && a.bias ? s_bias[chosen] : 0.0f;
     const int prev = __shfl_up_sync(kFull, chosen, 1, L);
     const float pv = __shfl_up_sync(kFull, value, 1, L), pz = __shfl_up_sync(kFull, z, 1, L), pb = __shfl_up_sync(kFull, b, 1, L);
-    const bool near = l > 0 && chosen >= 0 && prev >= 0 && !(pz == z && pb == b) &&
-                      !(pv - value > kTol * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f);
-    const bool apart = seg_ballot<L>(near) == 0;  // (all lanes take part, whatever their rows' groups said)
-    // as many slots as lanes leave none for the next value
-    sure = sure && a.top_k < L && apart;
-    unsigned unsure = __ballot_sync(kFull, !sure && exists);
+    const bool apart = pv - value > kTol * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f;  // (of the value before)
+    const bool near = l > 0 && l <= a.top_k && have && prev >= 0 && !apart && !(pz == z && pb == b);
+    const bool border = l < rounds && (have ? l >= a.top_k && prev >= 0 && apart : l >= a.top_k || l == rounds - 1);
+    // (all lanes take part in what follows, whatever their rows need)
+    const bool mixed = seg_ballot<L>(near) != 0, open = seg_ballot<L>(border) == 0;
+    bool whole = false;
+    if (__any_sync(kFull, open)) {
+      // no gap behind the slots: whether all that is near the last value is the same score and bias (then its order is known)
+      const float lv = seg_get<L>(value, rounds - 1), lz = seg_get<L>(z, rounds - 1), lb = seg_get<L>(b, rounds - 1);
+      bool other = false;
+#pragma unroll 1
+      for (int q = 0; q < VPT * L; q += L) {
+        const int col = q + l;
+        if (col >= a.K) break;
+        const float u = score_at(row, col), v = a.bias ? s_bias[col] : 0.0f;
+        // (a group's masks are in c only: its experts count as near ones here)
+        float x = u;
+        if (a.func == FGMM_SCORE_SOFTMAX) x = expf(u - m) * inv;
+        else if (a.func == FGMM_SCORE_SIGMOID) x = sigmoid(u);
+        x += v;
+        if (u > -INFINITY && x > -INFINITY && !(fabsf(lv - x) > kTol * (fabsf(lv) + fabsf(x) + 2.0f * bmax) + 1e-36f)) other |= !(u == lz && v == lb);
+      }
+      whole = seg_ballot<L>(other) != 0 && open;
+    }
+    if (__any_sync(kFull, mixed && !whole)) {
+      const double total = a.func == FGMM_SCORE_SOFTMAX ? exact_total<T, L>(row, a.K, m) : 0.0;
+      const double exact = have ? exact_value(z, b, a.func, m, total) : -INFINITY;
+      int rank = 0, moved = -1;
+      for (int j = 0; j < rounds; ++j) {
+        const double x = seg_get<L>(exact, j);
+        const int i = seg_get<L>(chosen, j);
+        rank += i >= 0 && before(x, i, exact, chosen);
+      }
+      if (!have || l >= rounds) rank = -1;
+      for (int j = 0; j < rounds; ++j) {
+        const int to = seg_get<L>(rank, j), i = seg_get<L>(chosen, j);
+        if (to == l) moved = i;
+      }
+      if (mixed) chosen = moved;
+    }
+    unsigned unsure = __ballot_sync(kFull, whole && exists);
     while (unsure) {  // row by row, the whole warp on it
       const int from = (__ffs(unsure) - 1) / L * L, lane = threadIdx.x & 31;
       const T *at = reinterpret_cast<const T *>(__shfl_sync(kFull, (unsigned long long)row, from));
@@ -523,7 +617,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
 }
 
 // Values a lane holds of the next row while this one is decided: up to 16 (more would cost occupancy).
-template <typename T, int VPT, int V, int L>
+template <typename T, int VPT, int V, int L, bool BY_VALUE>
 __global__ void __launch_bounds__(32 * kRouteWarps, VPT <= 8 ? 10 : VPT <= 16 ? 7 : VPT <= 32 ? 6 : 2)
 route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict__ weights, int32_t *__restrict__ indices) {
   constexpr int RPW = 32 / L;  // rows a warp
@@ -538,7 +632,7 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
   Row<T, VPT> raw;
   if (n - seg < a.N) load_row<T, VPT, V, L>(at(n), a.K, l, raw);
   float bmax = 0.0f;  // the largest finite |bias|
-  if (a.bias) {
+  if (BY_VALUE && a.bias) {
     for (int c = threadIdx.x; c < VPT * L; c += blockDim.x) s_bias[c] = c < a.K ? __ldg(a.bias + c) : 0.0f;
     __syncthreads();
     for (int c = lane; c < VPT * L; c += 32) {
@@ -556,7 +650,7 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
     if constexpr (kAhead)
       if (more) load_row<T, VPT, V, L>(at(next), a.K, l, ahead);
     const bool exists = n < a.N;
-    route_row<T, VPT, V, L>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp], weights + n * a.top_k, indices + n * a.top_k);
+    route_row<T, VPT, V, L, BY_VALUE>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp], weights + n * a.top_k, indices + n * a.top_k);
     if (!more) break;
     n = next;
     if constexpr (kAhead) raw = ahead;
@@ -673,7 +767,8 @@ int route_forward_t(const T *z, const RouteArgs &a, float *w, int32_t *idx, cuda
     // every warp slot of the device once (64 warps an SM), so that the rows after the first are prefetched
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, kRouteWarps * (32 / lanes())), (int64_t)num_sms() * 64 / kRouteWarps);
     const size_t smem = a.bias ? vpt() * lanes() * sizeof(float) : 0;
-    FGMM_CUDA_TRY(launch_pdl(route_kernel<T, vpt(), v(), lanes()>, dim3(grid), dim3(32 * kRouteWarps), smem, st, z, a, w, idx));
+    auto *kernel = a.bias || a.n_groups > 1 ? route_kernel<T, vpt(), v(), lanes(), true> : route_kernel<T, vpt(), v(), lanes(), false>;
+    FGMM_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(32 * kRouteWarps), smem, st, z, a, w, idx));
     return FGMM_OK;
   });
 }

@@ -96,6 +96,21 @@ def test_route_ties_and_near_ties(func, G, T):
     assert got[1].cpu().tolist() == [list(range(k))] * 3
 
 
+@pytest.mark.parametrize("func", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("N,K,k,G,T", [(40, 64, 6, 4, 2), (33, 30, 5, 1, 1), (21, 100, 2, 1, 1), (20, 256, 3, 1, 1), (40, 256, 8, 8, 4), (20, 256, 1, 8, 4),
+                                       (20, 200, 32, 1, 1), (9, 1024, 8, 32, 3), (5, 2048, 8, 16, 3), (20, 20, 20, 4, 2)])
+def test_route_equal_and_nearly_equal_together(func, N, K, k, G, T):
+    """Rows of few distinct scores: saturated ones, which fp32 values do not tell apart, and neighbours in fp32, many of each."""
+    g = gen(N + K + k)
+    saturated = 20.0 + torch.randint(0, 5, (N, K), generator=g) * 0.125
+    near = 1.0 + torch.randint(0, 4, (N, K), generator=g) * 2.0 ** -23
+    small = torch.randint(-1, 2, (K,), generator=g).float() * 2.0 ** -26
+    for z in (saturated, near):
+        for bias in (None, torch.zeros(K), small):
+            got = C().route_experts(z.to(DEV), k, score_func=func, bias=None if bias is None else bias.to(DEV), n_groups=G, top_groups=T)
+            check_route(z, got, ref.route(z, k, func, bias, G, T), func, 1.0)
+
+
 @pytest.mark.parametrize("func", FUNCS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("G,T,with_bias", [(1, 1, False), (1, 1, True), (4, 2, True)])
