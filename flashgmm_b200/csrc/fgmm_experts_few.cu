@@ -3,7 +3,9 @@
 // What bounds them is reading each expert's weights once (Y, DX) or writing every expert's gradient once (DW).  float32
 // weights, and 16-bit ones whose rows TMA cannot read, are taken as they are: the tensor-core path would first copy all
 // of them, also those of experts without a row.  A block owns a window of neighbouring grouped rows and a tile of columns; the
-// rows of one expert in the window share each weight that is read.
+// rows of one expert in the window share each weight that is read.  64 experts of 512 x 1,024 float32 with one row each on
+// average (some 40 of them met, 85 MB: 13 us): y 16 us, dx 28, dW 29 (134 MB written: 21 us); the rule that chooses them
+// stands with more figures beside their launches.
 #include <algorithm>
 
 #include "fgmm_experts.cuh"

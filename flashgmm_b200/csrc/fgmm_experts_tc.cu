@@ -20,6 +20,11 @@
 //     b0 b2 and b2 b0, 2^-8 and less of it, into another).  Tensor-memory accumulation truncates, so the
 //     first is drained into fp32 registers every 256 elements of the contraction.
 //   * 16-bit operands whose rows are no multiple of 16 bytes are copied to padded rows first (TMA strides).
+// What bounds it is shared memory at 128 bytes a cycle: a stage of 128 x 256 x 64 16-bit products writes and reads 96 KB, 768
+// cycles, for 512 of tensor time; one of three planes and 128 columns 288 KB, 2,304 for 1,536.  8,192 points with 4 of 64
+// experts, 1,024 -> 2,048 bf16: 152 us, 905 TFLOP/s, 55 % of a library matrix product's; 65,536 points with 2 of 256, 128 ->
+// 128 fp32: 77 us with the planes' copies (20), six times its 57 TFLOP/s in bf16 products.  Two SMs on one tile would halve the
+// weights' part of that, but its 256 rows fit the ends of the experts' rows worse (14 % more products there).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <algorithm>
