@@ -668,9 +668,9 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
 // others nothing; else the softmax gives s (g [chosen] - sum of g s over the chosen) to every score, and
 // sigmoid and given values pass g s (1 - s) and g on.  The row without the chosen ones' part is written first (the
 // scores are read for the softmax only), then the lane of each slot writes its element.  65,521 fp32 rows of 128 (33 MB read, 34
-// written: 10.4 us) take 17 us.
+// written: 10.4 us) take 10.5 us where they stay in L2 (12.1 without the blocks an SM asked for).
 template <typename T, int VPT, int V, int L, bool DENSE>
-__global__ void __launch_bounds__(128, DENSE ? 1 : 12) route_backward_kernel(const float *__restrict__ dw, const T *__restrict__ scores,
+__global__ void __launch_bounds__(128, DENSE ? (VPT <= 16 ? 8 : 1) : 12) route_backward_kernel(const float *__restrict__ dw, const T *__restrict__ scores,
                                                              const int32_t *__restrict__ indices, const RouteArgs a,
                                                              T *__restrict__ dz) {
   const int lane = threadIdx.x & 31, l = lane % L;
@@ -747,7 +747,8 @@ __global__ void __launch_bounds__(128, DENSE ? 1 : 12) route_backward_kernel(con
 
 // Lanes L of a row and values VPT a lane holds, for K columns and `slots` lanes that the choices take.  A row of up to 256
 // columns takes part of a warp where few are chosen, since what a row costs beside its values is then shared
-// (K = 128, two chosen: 442 -> 187 instructions a row); more choices are picked faster by a warp's reductions.
+// (K = 128, two chosen: 442 -> 187 instructions a row); more choices are picked faster by a warp's reductions.  us, part of a
+// warp / whole: 65,536 x 64 with 6 chosen 23 / 33, 8 28 / 35, 10 74 / 38; 16,384 x 256 with 4 10 / 10, 8 16 / 11.
 // Packs are 16 bytes (8 for a 16-bit row of up to 128 columns) where the rows are aligned for them.
 template <typename T, typename F> int by_row_width(int K, int slots, bool vec, F f) {
   constexpr int V = 16 / sizeof(T);
@@ -755,7 +756,7 @@ template <typename T, typename F> int by_row_width(int K, int slots, bool vec, F
   return vec ? f(std::integral_constant<int, n>{}, std::integral_constant<int, v>{}, std::integral_constant<int, lanes>{}) \
              : f(std::integral_constant<int, n>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, lanes>{});
   if (K <= 32 && slots <= 8) FGMM_WIDTH(4, 4, 8)
-  if (K <= 128 && slots <= 4) FGMM_WIDTH(16, V, 8)
+  if (K <= 128 && slots <= 8) FGMM_WIDTH(16, V, 8)
   if (K <= 256 && slots <= 4) FGMM_WIDTH(16, V, 16)
   if (K <= 128) FGMM_WIDTH(4, 4, 32)
   if (K <= 256) FGMM_WIDTH(8, V, 32)
@@ -783,7 +784,8 @@ template <typename T>
 int route_backward_t(const float *dw, const T *z, const int32_t *idx, const RouteArgs &a, T *dz, cudaStream_t st) {
   const bool vec = reinterpret_cast<uintptr_t>(z) % 16 == 0 && a.stride * sizeof(T) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(dz) % 16 == 0 && a.K * sizeof(T) % 16 == 0;
-  return by_row_width<T>(a.K, a.top_k, vec, [&](auto vpt, auto v, auto lanes) {
+  // (nothing is chosen here: up to 8 slots need 8 lanes and no more)
+  return by_row_width<T>(a.K, a.top_k <= 8 ? (a.top_k + 1) / 2 : a.top_k, vec, [&](auto vpt, auto v, auto lanes) {
     const unsigned grid = (unsigned)std::min<int64_t>(cdiv(a.N, 128 / lanes()), (int64_t)num_sms() * 16);
     const bool dense = a.func == FGMM_SCORE_SOFTMAX && !a.renorm;
     FGMM_CUDA_TRY(launch_pdl(dense ? route_backward_kernel<T, vpt(), v(), lanes(), true> : route_backward_kernel<T, vpt(), v(), lanes(), false>,
