@@ -396,6 +396,7 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     left = left == best ? 0u : left;
   }
   const float bar = best != 0u ? of_key(best) : -FLT_MAX;  // (masked values are below it)
+  const float top = bar == FLT_MAX ? INFINITY : bar;       // (+inf counts as the largest finite value)
   constexpr int kWords = (VPT + 31) / 32;
   uint32_t some[kWords], equal[kWords];
   int n = 0;
@@ -414,7 +415,7 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     for (int w = 0; w < kWords; ++w) {
 #pragma unroll
       for (int i = w * 32; i < VPT && i < w * 32 + 32; ++i)
-        if (c[i] == bar) equal[w] |= 1u << (i & 31);
+        if (c[i] >= bar && c[i] <= top) equal[w] |= 1u << (i & 31);
       some[w] &= ~equal[w];
       n += __popc(some[w]);
     }
