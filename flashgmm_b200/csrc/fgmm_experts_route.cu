@@ -248,6 +248,15 @@ template <int L> __device__ __forceinline__ float chosen_share(float z, bool liv
     else t = live ? __fdividef(expf(fminf(z, 0.0f) - fminf(m, 0.0f)), 1.0f + expf(-fabsf(z))) : 0.0f;
   }
   sum = seg_sum<L>(t);
+  // given values whose sum leaves fp32 on the way: at 2^-6 of their size 32 of them do not
+  if (func == FGMM_SCORE_GIVEN && __any_sync(kFull, !(fabsf(sum) < INFINITY))) {
+    const bool large = !(fabsf(sum) < INFINITY);
+    const float less = seg_sum<L>(0x1p-6f * t);
+    if (large) {
+      sum = 0x1p6f * less;
+      return less == 0.0f ? 0.0f : 0x1p-6f * t / less;
+    }
+  }
   return sum == 0.0f ? 0.0f : t / sum;
 }
 

@@ -7,7 +7,7 @@ import torch
 
 import experts_ref as ref
 from experts_ref import F32_MAX
-from test_experts_gpu import C, DEV, FUNCS, gen
+from test_experts_gpu import C, DEV, FUNCS, TYPES, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,22 @@ def test_route_many_infinities_and_largest_scores(func, K, k):
     for renorm in (True, False):
         got = C().route_experts(z.to(DEV), k, score_func=func, renormalize=renorm)
         assert torch.equal(got[1].cpu(), ref.route(z, k, func, renormalize=renorm)[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [20, 512])
+def test_route_shares_of_the_largest_values(K, dtype):
+    """Given values whose sum is beyond fp32 still have their shares: a sum and a quotient, 2^-24 and 2^-23 each."""
+    inf, k = math.inf, 6
+    z = torch.rand(5, K, generator=gen(K)).to(dtype)
+    z[0, 3] = z[0, 17] = inf
+    z[1, :k] = inf
+    z[2] = -inf; z[2, 1] = inf; z[2, 4] = inf; z[2, 6] = -1.0
+    z[3] = -inf; z[3, 5] = inf; z[3, 6] = inf; z[3, 9] = torch.finfo(dtype).min
+    z[4, 2] = torch.finfo(dtype).max; z[4, 8] = torch.finfo(dtype).max; z[4, 9] = torch.finfo(dtype).max / 2
+    w, idx = C().route_experts(z.to(DEV), k, score_func="given")
+    want = ref.route(z, k, "given")
+    assert torch.equal(idx.cpu(), want[1])
+    assert ((w.double().cpu() - want[0]).abs() <= 8 * 2.0 ** -23 * want[0].abs() + 2.0 ** -126).all()
+    dz = C().route_experts_backward(torch.randn(5, k, generator=gen(1)).to(DEV), z.to(DEV), idx, score_func="given")
+    assert torch.isfinite(dz).all()
