@@ -265,7 +265,8 @@ __device__ __forceinline__ void top_two(float &b1, float &b2, float v1, float v2
   b1 = fmaxf(b1, v1);
 }
 
-// Masks all but the top_groups groups of a warp's row.
+// Masks all but the top_groups groups of a warp's row.  tol: the relative error of a c near the row's largest (|z - m| 2^-24 of an s
+// farther off is 0.4 2^-24 of the largest s at most, which tol's spare covers).
 template <typename T, int VPT, int V>
 __device__ __forceinline__ void keep_groups(float (&c)[VPT], const T *row, const RouteArgs &a, int lane, float m, float bmax, float tol,
                                             float2 *s_group) {
@@ -495,10 +496,14 @@ constexpr int kRouteWarps = 4;
 template <typename T, int VPT, int V, int L, bool BY_VALUE>
 __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T, VPT> &raw, const RouteArgs &a, int l, const float *s_bias,
                                           float bmax, uint64_t *s_cand, float *weights, int32_t *indices) {
-  // fp32 values of c are off by at most a few 2^-23 of |s| and |bias|: two that differ by more than this (times
-  // their sizes) are in the right order
-  constexpr float kTol = 1.0f / (1 << 20);
+  // fp32 values of c are off by at most 16 2^-24 of |s| and |bias| (exp, the quotient, the bias, a few steps of the softmax's
+  // sum), and those of a softmax by VPT 2^-24 (a lane's part of the sum) and |z - m| 2^-24 (the exponent's rounding) more:
+  // two that differ by more than this (times their sizes) are in the right order
+  constexpr float kTol = 0x1p-20f;
   float c[VPT], m = 0.0f, total = 1.0f, inv = 1.0f;
+  const auto tolerance = [&](float z1, float z2) {
+    return a.func == FGMM_SCORE_SOFTMAX ? fmaf(m - fminf(z1, z2) + (float)VPT, 0x1p-24f, kTol) : kTol;
+  };
 #pragma unroll
   for (int i = 0; i < VPT; ++i) c[i] = to_f32(raw.v[i]);
   if (L < 32 || BY_VALUE || (a.func == FGMM_SCORE_SOFTMAX && !a.renorm)) {  // (pick_few takes scores as they are)
@@ -531,7 +536,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
       for (int i = 0; i < VPT; ++i) c[i] = fmaxf(c[i] + s_bias[column<V, L>(i, l)], -INFINITY);  // -inf for NaN
     }
     if constexpr (L == 32)
-      if (a.n_groups > 1) keep_groups<T, VPT, V>(c, row, a, l, m, bmax, kTol, reinterpret_cast<float2 *>(s_cand));
+      if (a.n_groups > 1) keep_groups<T, VPT, V>(c, row, a, l, m, bmax, tolerance(m, m), reinterpret_cast<float2 *>(s_cand));
   }
   const bool rounded = BY_VALUE && (a.func != FGMM_SCORE_GIVEN || a.bias);  // c is not exact
   const int rounds = min(L, rounded ? a.top_k + 2 : a.top_k);
@@ -559,7 +564,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
     const float z = have ? score_at(row, chosen) : 0.0f, b = have && a.bias ? s_bias[chosen] : 0.0f;
     const int prev = __shfl_up_sync(kFull, chosen, 1, L);
     const float pv = __shfl_up_sync(kFull, value, 1, L), pz = __shfl_up_sync(kFull, z, 1, L), pb = __shfl_up_sync(kFull, b, 1, L);
-    const bool apart = pv - value > kTol * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f;  // (of the value before)
+    const bool apart = pv - value > tolerance(pz, z) * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f;  // (of the value before)
     const bool near = l > 0 && l <= a.top_k && have && prev >= 0 && !apart && !(pz == z && pb == b);
     const bool border = l < rounds && (have ? l >= a.top_k && prev >= 0 && apart : l >= a.top_k || l == rounds - 1);
     // (all lanes take part in what follows, whatever their rows need)
@@ -579,7 +584,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
         if (a.func == FGMM_SCORE_SOFTMAX) x = expf(u - m) * inv;
         else if (a.func == FGMM_SCORE_SIGMOID) x = sigmoid(u);
         x += v;
-        if (u > -INFINITY && x > -INFINITY && !(fabsf(lv - x) > kTol * (fabsf(lv) + fabsf(x) + 2.0f * bmax) + 1e-36f)) other |= !(u == lz && v == lb);
+        if (u > -INFINITY && x > -INFINITY && !(fabsf(lv - x) > tolerance(lz, u) * (fabsf(lv) + fabsf(x) + 2.0f * bmax) + 1e-36f)) other |= !(u == lz && v == lb);
       }
       whole = seg_ballot<L>(other) != 0 && open;
     }

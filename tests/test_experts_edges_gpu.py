@@ -47,3 +47,23 @@ def test_route_shares_of_the_largest_values(K, dtype):
     assert ((w.double().cpu() - want[0]).abs() <= 8 * 2.0 ** -23 * want[0].abs() + 2.0 ** -126).all()
     dz = C().route_experts_backward(torch.randn(5, k, generator=gen(1)).to(DEV), z.to(DEV), idx, score_func="given")
     assert torch.isfinite(dz).all()
+
+
+@pytest.mark.parametrize("G,T", [(1, 1), (4, 3)])
+@pytest.mark.parametrize("K,k", [(32, 7), (128, 10), (256, 21), (512, 30)])
+def test_route_near_ties_far_below_the_largest_score(K, k, G, T):
+    """exp(z - max) carries the rounding of z - max, |z - max| 2^-24: k - 1 scores 40 or 68 below the row's largest, whose biases
+    (1e-4 of the values) bring the values within 2^-15 of each other, are still ordered in 64 bits.  All others are far below."""
+    for seed in range(24):
+        top, low = ((66.3, -1.7), (40.1, 0.3))[seed % 2]
+        g = gen(100 * K + seed)
+        at = torch.randperm(K, generator=g)
+        z = low - 5 + torch.rand(1, K, generator=g)
+        z[0, at[:k - 1]] = low + 1e-4 * torch.rand(k - 1, generator=g)
+        z[0, at[-1]] = top
+        s = torch.softmax(z.double(), 1)[0]
+        bias = torch.zeros(K)
+        bias[at[:k - 1]] = (s[at[0]] * (1 + (torch.rand(k - 1, generator=g).double() - 0.5) * 2.0 ** -15) - s[at[:k - 1]]).float()
+        got = C().route_experts(z.to(DEV), k, bias=bias.to(DEV), n_groups=G, top_groups=T)
+        want = ref.route(z, k, "softmax", bias.double(), G, T)
+        assert torch.equal(got[1].cpu(), want[1]), seed
