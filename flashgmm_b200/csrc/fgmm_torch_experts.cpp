@@ -17,7 +17,18 @@ void check_rc(int rc, const char *op) {
   TORCH_CHECK(rc == FGMM_OK, op, ": flashgmm_b200 error ", rc, ": ", fgmm_last_error());
 }
 
+// Only tensors that own their memory and whose derivatives autograd records are read through their pointers: a forward-mode tangent
+// would be dropped, and the pointer of a traced, batched or wrapped tensor is none (that of a traced tensor's slice is not null).
+void check_plain(const Tensor &t, const char *name) {
+  constexpr c10::DispatchKeySet kOthers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                         c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor});
+  TORCH_CHECK(t.defined() && t.layout() == torch::kStrided && !t.key_set().has_any(kOthers), name,
+              " must be a plain strided tensor (not a traced, batched, sparse or wrapped one)");
+  TORCH_CHECK(!t._fw_grad(0).defined(), name, " has a forward-mode tangent: flashgmm_b200 has no forward-mode derivatives");
+}
+
 void check_cuda(const Tensor &t, const char *name, int dim, const torch::Device *dev) {
+  check_plain(t, name);
   TORCH_CHECK(t.dim() == dim, name, " must be ", dim, "D");
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (flashgmm_b200 has no CPU path)");
   if (dev) TORCH_CHECK(t.device() == *dev, name, " is on ", t.device(), ", expected ", *dev);

@@ -16,8 +16,9 @@ indices int32), run on the current stream of the tensors' device and hold their 
 input requires a gradient, the functions record one; the ``*_backward`` functions are the same
 gradients without autograd; a step that is captured into a CUDA graph while an eager autograd graph of the
 same leaves is alive takes those (autograd then joins the eager graph's stream to the capture, which CUDA
-refuses).  The reference has no counterpart; its E-step
-(``flash_gmm/csrc/binding.cpp:35-49``) gives the scores of a fitted mixture's gate.
+refuses).  Forward-mode tangents and traced, batched (``torch.func``) or wrapped tensors are refused.  The
+reference has no counterpart; its E-step (``flash_gmm/csrc/binding.cpp:35-49``) gives the scores of a fitted
+mixture's gate.
 """
 from typing import NamedTuple
 

@@ -67,3 +67,29 @@ def test_route_near_ties_far_below_the_largest_score(K, k, G, T):
         got = C().route_experts(z.to(DEV), k, bias=bias.to(DEV), n_groups=G, top_groups=T)
         want = ref.route(z, k, "softmax", bias.double(), G, T)
         assert torch.equal(got[1].cpu(), want[1]), seed
+
+
+# ------------------------------------------------------------------------------- inputs
+def test_derivatives_that_are_not_recorded_are_refused():
+    """Forward-mode, batched and traced tensors are refused: nothing drops their derivative in silence or reads through
+    pointers that they do not have."""
+    import torch.autograd.forward_ad as fw
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    z, x, w = torch.randn(6, 8, device=DEV), torch.randn(6, 16, device=DEV), torch.randn(8, 4, 16, device=DEV)
+    weights, idx = C().route_experts(z, 2)
+    routes = C().group_routes(idx, 8)
+    y = C().expert_products(x, w, routes)
+    calls = [(lambda t: C().route_experts(t, 2)[0], z), (lambda t: C().route_experts(z, 2, bias=t)[0], torch.zeros(8, device=DEV)),
+             (lambda t: C().route_experts_backward(t, z, idx), weights), (lambda t: C().expert_products(t, w, routes), x),
+             (lambda t: C().expert_products(x, t, routes), w), (lambda t: C().expert_products_backward(t, x, w, routes)[0], y),
+             (lambda t: C().combine_experts(t, weights, routes), y), (lambda t: C().combine_experts(y, t, routes), weights),
+             (lambda t: C().combine_experts_backward(y[:6].clone(), t, weights, routes)[0], y)]
+    for call, t in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(t[None].clone())
+        for leaf in (t.clone(), t.clone().requires_grad_()):
+            with fw.dual_level(), pytest.raises(RuntimeError):
+                call(fw.make_dual(leaf, torch.ones_like(t)))
+        call(t)
