@@ -50,15 +50,18 @@ void check_shape(const Tensor &t, const char *name, std::initializer_list<int64_
               torch::IntArrayRef(want));
 }
 
+// Contiguous, with the values in memory (a view may hold them negated).
+Tensor dense(const Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+
 // Rows contiguous; the row stride stays (an expanded or sliced matrix is not copied).
 Tensor with_rows(const Tensor &t) {
-  return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+  return !t.is_neg() && (t.size(1) <= 1 || t.stride(1) == 1) ? t : dense(t);
 }
 int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
 // Contiguous and on a 16-byte boundary, as the products read their matrices.
 Tensor for_products(const Tensor &t) {
-  Tensor c = t.contiguous();
+  Tensor c = dense(t);
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
@@ -97,7 +100,7 @@ std::tuple<Tensor, Tensor> route_experts(const Tensor &scores, int64_t top_k, co
     check_type(*bias, "bias", torch::kFloat32);
     check_cuda(*bias, "bias", 1, &dev);
     check_shape(*bias, "bias", {K});
-    b = bias->contiguous();
+    b = dense(*bias);
   }
   TORCH_CHECK(top_k >= 1 && top_k <= K && top_k <= FGMM_MAX_TOP_K, "top_k must be in [1, min(K, ", FGMM_MAX_TOP_K, ")], got ", top_k);
   const c10::cuda::CUDAGuard guard(dev);
@@ -125,7 +128,7 @@ Tensor route_experts_backward(const Tensor &d_weights, const Tensor &scores, con
   check_shape(indices, "indices", {N, top_k});
   check_shape(d_weights, "d_weights", {N, top_k});
   const c10::cuda::CUDAGuard guard(dev);
-  const Tensor z = with_rows(scores), dw = d_weights.contiguous(), idx = indices.contiguous();
+  const Tensor z = with_rows(scores), dw = dense(d_weights), idx = dense(indices);
   Tensor dz = fresh({N, K}, z.scalar_type(), dev);
   check_rc(fgmm_route_experts_backward(dw.data_ptr<float>(), z.data_ptr(), dtype, N, narrow(K, "K"), row_stride(z),
                                        idx.data_ptr<int32_t>(), narrow(top_k, "top_k"), f, renormalize, (float)scale,
@@ -143,7 +146,7 @@ std::tuple<Tensor, Tensor, Tensor> group_routes(const Tensor &indices, int64_t K
   TORCH_CHECK(R <= INT32_MAX - 1024, "indices has more than 2^31 - 1025 routes");
   const torch::Device dev = indices.device();
   const c10::cuda::CUDAGuard guard(dev);
-  const Tensor idx = indices.contiguous();
+  const Tensor idx = dense(indices);
   Tensor order = fresh({R}, torch::kInt32, dev), offsets = fresh({K + 1}, torch::kInt32, dev);
   Tensor position = fresh(indices.sizes(), torch::kInt32, dev);
   Tensor ws = scratch(fgmm_group_routes_workspace_bytes(R, (int)K), dev);
@@ -172,7 +175,7 @@ Plan plan_of(const Tensor &order, const Tensor &offsets, const Tensor &position,
   TORCH_CHECK(offsets.size(0) >= 2 && offsets.size(0) <= FGMM_MAX_EXPERTS + 1, "offsets must have K + 1 entries, K in [1, ",
               FGMM_MAX_EXPERTS, "]");
   TORCH_CHECK(order.numel() <= INT32_MAX - 1024, "the plan has more than 2^31 - 1025 routes");
-  return {order.contiguous(), offsets.contiguous(), position.contiguous(), order.size(0), position.size(0),
+  return {dense(order), dense(offsets), dense(position), order.size(0), position.size(0),
           (int)offsets.size(0) - 1, (int)position.size(1)};
 }
 
@@ -246,7 +249,7 @@ Tensor combine_experts(const Tensor &y, const Tensor &weights, const Tensor &ord
   check_cuda(weights, "weights", 2, &dev);
   check_shape(weights, "weights", {p.N, p.top_k});
   TORCH_CHECK(d >= 1, "y must have at least one column");
-  const Tensor yc = y.contiguous(), w = weights.contiguous();
+  const Tensor yc = dense(y), w = dense(weights);
   Tensor out = fresh({p.N, d}, y.scalar_type(), dev);
   check_rc(fgmm_combine_experts(yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(), p.position.data_ptr<int32_t>(),
                                 p.top_k, out.data_ptr(), stream()),
@@ -270,7 +273,7 @@ std::tuple<Tensor, Tensor> combine_experts_backward(const Tensor &d_out, const T
   check_cuda(d_out, "d_out", 2, &dev);
   check_shape(d_out, "d_out", {p.N, d});
   TORCH_CHECK(d >= 1, "y must have at least one column");
-  const Tensor yc = y.contiguous(), gc = d_out.contiguous(), w = weights.contiguous();
+  const Tensor yc = dense(y), gc = dense(d_out), w = dense(weights);
   Tensor dy = fresh({p.R, d}, y.scalar_type(), dev), dw = fresh({p.N, p.top_k}, torch::kFloat32, dev);
   check_rc(fgmm_combine_experts_backward(gc.data_ptr(), yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(),
                                          p.order.data_ptr<int32_t>(), p.offsets.data_ptr<int32_t>(), p.K, p.top_k,

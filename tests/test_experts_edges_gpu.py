@@ -70,6 +70,27 @@ def test_route_near_ties_far_below_the_largest_score(K, k, G, T):
 
 
 # ------------------------------------------------------------------------------- inputs
+@pytest.mark.parametrize("strided", [False, True])
+def test_negated_views_are_read_by_value(strided):
+    """A view whose memory holds the opposite sign, as the imaginary part of a conjugate is one."""
+    def negated(*shape, seed):
+        re, im = (torch.randn(*shape, generator=gen(seed + i)).to(DEV) for i in range(2))
+        return torch.complex(re, im).conj().imag if strided else torch._neg_view(im)
+    N, K, k, d = 40, 6, 2, 16
+    z, x, w, dy, wt, b = (negated(*s, seed=10 * i) for i, s in enumerate(((N, K), (N, d), (K, d, d), (N * k, d), (N, k), (K,))))
+    assert all(t.is_neg() for t in (z, x, w, dy, wt, b))
+    plain = [t.clone().resolve_neg() for t in (z, x, w, dy, wt, b)]
+    results = []
+    for zi, xi, wi, gi, ti, bi in ((z, x, w, dy, wt, b), plain):
+        weights, idx = C().route_experts(zi, k, bias=bi)
+        routes = C().group_routes(idx, K)
+        results.append([weights, idx, C().route_experts_backward(ti, zi, idx), C().expert_products(xi, wi, routes),
+                        *C().expert_products_backward(gi, xi, wi, routes), C().combine_experts(gi, ti, routes),
+                        *C().combine_experts_backward(xi, gi, ti, routes)])
+    for a, c in zip(*results):
+        assert torch.equal(a, c)
+
+
 def test_derivatives_that_are_not_recorded_are_refused():
     """Forward-mode, batched and traced tensors are refused: nothing drops their derivative in silence or reads through
     pointers that they do not have."""
