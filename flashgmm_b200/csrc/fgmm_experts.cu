@@ -185,14 +185,15 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
 }
 
 // tpr threads share a point; each owns packs of columns and adds the rows of J slots at a time, whose places are fetched a
-// point ahead and whose packs are on their way together.  Memory bounds it: 8,192 points of 4 rows of 2,048 bf16 (168 MB)
+// point ahead and whose packs are on their way together.  ENDS: places from *rows_end on are skipped.  Memory bounds it: 8,192 points of 4 rows of 2,048 bf16 (168 MB)
 // 32 us, 5.2 TB/s; 16,411 points of 2 rows of 1,000 fp32 (197 MB) 39 us.  PARTS: the rows are sums of `parts` matrices.
-template <typename TY, typename T, int V, int J, bool PARTS>
+template <typename TY, typename T, int V, int J, bool PARTS, bool ENDS>
 __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int64_t R, int d, const float *__restrict__ weights,
                                                       const int32_t *__restrict__ position, int64_t N, int top_k, int tpr,
-                                                      int parts, T *__restrict__ out) {
+                                                      int parts, const int32_t *__restrict__ rows_end, T *__restrict__ out) {
   griddep_wait();
   griddep_launch();
+  const int64_t end = ENDS ? min((int64_t)max(__ldg(rows_end), 0), R) : R;
   const int64_t stride = (int64_t)gridDim.x * (256 / tpr);
   int64_t n = (int64_t)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   int p[J], ahead[J];
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, 
         Pack<TY, V> f[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {  // (a slot without an expert reads row 0 and leaves it)
-          if (p[j] >= R) p[j] = -1;
+          if (p[j] >= end) p[j] = -1;
           f[j] = load_raw<TY, V>(y + (int64_t)max(p[j], 0) * d + c);
         }
 #pragma unroll
@@ -290,15 +291,17 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
   if (lane == 0 && known) d_weights[id] = dot;
 }
 
-template <typename TY, typename T>
-int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st, int parts = 1) {
+template <bool ENDS, typename TY, typename T>
+int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32_t *pos, int64_t N, int top_k, T *out, cudaStream_t st, int parts = 1,
+                      const int32_t *rows_end = nullptr) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   int tpr = 1;
   while (tpr < 256 && tpr * (vec ? V : 1) < d) tpr *= 2;
   const unsigned grid = (unsigned)std::min<int64_t>(cdiv(N, 256 / tpr), 8 * num_sms());
   auto run = [&](auto v, auto j, auto several) {
-    return launch_pdl(combine_kernel<TY, T, v(), j(), several()>, dim3(grid), dim3(256), 0, st, y, R, d, w, pos, N, top_k, tpr, parts, out);
+    return launch_pdl(combine_kernel<TY, T, v(), j(), several(), ENDS>, dim3(grid), dim3(256), 0, st, y, R, d, w, pos, N, top_k, tpr, parts, rows_end,
+                      out);
   };
   auto by_slots = [&](auto v, auto several) {
     // (elements one by one are bound by instructions, not by loads on their way: one slot after the other)
@@ -306,7 +309,11 @@ int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32
     if (top_k == 2) return run(v, std::integral_constant<int, 2>{}, several);
     return run(v, std::integral_constant<int, 4>{}, several);
   };
-  auto by_parts = [&](auto v) { return parts == 1 ? by_slots(v, std::false_type{}) : by_slots(v, std::true_type{}); };
+  auto by_parts = [&](auto v) {
+    if constexpr (ENDS)
+      if (parts > 1) return by_slots(v, std::true_type{});
+    return by_slots(v, std::false_type{});
+  };
   FGMM_CUDA_TRY(vec ? by_parts(std::integral_constant<int, V>{}) : by_parts(std::integral_constant<int, 1>{}));
   return FGMM_OK;
 }
@@ -366,16 +373,16 @@ int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32
 
 int combine_forward(const void *y, int dtype, int64_t R, int d, const float *weights,
                     const int32_t *position, int64_t N, int top_k, void *out, cudaStream_t st) {
-  if (dtype == FGMM_F32) return combine_forward_t((const float *)y, R, d, weights, position, N, top_k, (float *)out, st);
-  if (dtype == FGMM_BF16) return combine_forward_t((const __nv_bfloat16 *)y, R, d, weights, position, N, top_k, (__nv_bfloat16 *)out, st);
-  return combine_forward_t((const __half *)y, R, d, weights, position, N, top_k, (__half *)out, st);
+  if (dtype == FGMM_F32) return combine_forward_t<false>((const float *)y, R, d, weights, position, N, top_k, (float *)out, st);
+  if (dtype == FGMM_BF16) return combine_forward_t<false>((const __nv_bfloat16 *)y, R, d, weights, position, N, top_k, (__nv_bfloat16 *)out, st);
+  return combine_forward_t<false>((const __half *)y, R, d, weights, position, N, top_k, (__half *)out, st);
 }
 
-int sum_rows(const float *rows, int parts, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
-             cudaStream_t st) {
-  if (dtype == FGMM_F32) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (float *)out, st, parts);
-  if (dtype == FGMM_BF16) return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__nv_bfloat16 *)out, st, parts);
-  return combine_forward_t(rows, R, d, nullptr, position, N, top_k, (__half *)out, st, parts);
+int sum_rows(const float *rows, int parts, int dtype, int d, const RoutePlan &p, const int32_t *position, int64_t N, void *out, cudaStream_t st) {
+  const int32_t *end = p.offsets + p.K;
+  if (dtype == FGMM_F32) return combine_forward_t<true>(rows, p.R, d, nullptr, position, N, p.top_k, (float *)out, st, parts, end);
+  if (dtype == FGMM_BF16) return combine_forward_t<true>(rows, p.R, d, nullptr, position, N, p.top_k, (__nv_bfloat16 *)out, st, parts, end);
+  return combine_forward_t<true>(rows, p.R, d, nullptr, position, N, p.top_k, (__half *)out, st, parts, end);
 }
 
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,

@@ -59,8 +59,9 @@ int group_routes(const int32_t *indices, int64_t R, int K, int32_t *order, int32
 // out[n] = sum_j w[n][j] y[position[n][j]], positions outside [0, R) skipped.
 int combine_forward(const void *y, int dtype, int64_t R, int d, const float *weights,
                     const int32_t *position, int64_t N, int top_k, void *out, cudaStream_t st);
-// The same of fp32 rows[parts][R][d] with weights 1, summed over the parts.
-int sum_rows(const float *rows, int parts, int dtype, int64_t R, int d, const int32_t *position, int64_t N, int top_k, void *out,
+// The same of fp32 rows[parts][R][d] with weights 1, summed over the parts; rows behind offsets[K], which no kernel wrote, are
+// skipped whatever position says.
+int sum_rows(const float *rows, int parts, int dtype, int d, const RoutePlan &plan, const int32_t *position, int64_t N, void *out,
              cudaStream_t st);
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,
                      const RoutePlan &plan, void *dy, float *d_weights, cudaStream_t st);

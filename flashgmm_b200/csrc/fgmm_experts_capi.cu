@@ -184,7 +184,7 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
   if (!rc && (tc.inputs || tc.weights))
     rc = products_tc_backward(dy, x, weight, dtype, N, d_in, d_out, plan, dx_rows, d_weight, tc, rest, st);
   if (rc || !dx) return rc;
-  return sum_rows(dx_rows, parts, dtype, plan.R, d_in, position, N, top_k, dx, st);
+  return sum_rows(dx_rows, parts, dtype, d_in, plan, position, N, dx, st);
 }
 
 int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,

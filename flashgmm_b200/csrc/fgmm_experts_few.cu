@@ -182,7 +182,14 @@ __global__ void __launch_bounds__(kThreads) few_inputs_kernel(const T *__restric
         }
       }
     }
-    r += n;  // (rows of no expert are not read afterwards)
+    if (e == p.K && warp == 0) {  // rows of no expert are read afterwards below offsets[K] only (where offsets do not ascend): zeros
+      const int known = min(max(__ldg(p.offsets + p.K), 0), R);
+      for (int i = 0; i < n && r + i < known; ++i) {
+        const float zeros[4] = {};
+        store4<float, VEC>(dx + (int64_t)(r + i) * d_in + c, zeros, left);
+      }
+    }
+    r += n;
   }
 }
 

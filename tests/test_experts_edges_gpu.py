@@ -7,7 +7,7 @@ import torch
 
 import experts_ref as ref
 from experts_ref import F32_MAX
-from test_experts_gpu import C, DEV, FUNCS, TYPES, gen
+from test_experts_gpu import C, DEV, FUNCS, TYPES, close, gen, plan
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,47 @@ def test_derivatives_that_are_not_recorded_are_refused():
             with fw.dual_level(), pytest.raises(RuntimeError):
                 call(fw.make_dual(leaf, torch.ones_like(t)))
         call(t)
+
+
+# -------------------------------------------------------------------------------- plans
+def stale(*shape):
+    """Leaves NaN in the memory that the next results and workspaces come from."""
+    for s in shape:
+        torch.full((s,), float("nan"), device=DEV)
+    torch.cuda.synchronize()
+
+
+PATHS = [(torch.float32, 30, 2, 64, 64, 64), (torch.float32, 90, 2, 40, 33, 150), (torch.bfloat16, 30, 2, 64, 63, 64),
+         (torch.float32, 300, 2, 4, 128, 72), (torch.bfloat16, 300, 2, 4, 64, 136), (torch.float16, 260, 3, 5, 130, 20)]
+
+
+@pytest.mark.parametrize("dtype,N,k,K,d_in,d_out", PATHS)
+def test_dx_of_a_plan_whose_offsets_end_early(dtype, N, k, K, d_in, d_out):
+    """Rows behind offsets[K] belong to no expert, whatever position says of them: they give dx nothing."""
+    x, w = torch.randn(N, d_in, generator=gen(1)).to(dtype), torch.randn(K, d_out, d_in, generator=gen(2)).to(dtype)
+    dy = torch.randn(N * k, d_out, generator=gen(3)).to(dtype)
+    whole = C().group_routes(plan(N, k, K, 3).to(DEV), K)
+    for end in (0, 1, N, N * k):
+        routes = whole._replace(offsets=whole.offsets.clamp(max=end))
+        order, offsets = routes.order.cpu(), routes.offsets.cpu()
+        _, _, dx, dxa, dw, dwa = ref.products(x, w, order, offsets, k, dy)
+        stale(*[1 << i for i in range(10, 25)])
+        gx, gw = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes)
+        close(gx, dx, dxa, d_out + k, dtype, "dx")
+        close(gw, dw, dwa, N * k, dtype, "dw")
+
+
+@pytest.mark.parametrize("dtype,N,k,K,d_in,d_out", PATHS)
+def test_dx_of_a_plan_whose_offsets_do_not_ascend(dtype, N, k, K, d_in, d_out):
+    """Such a plan's results are nobody's, but they are made of its inputs: no stale memory is read."""
+    x, w = torch.randn(N, d_in, generator=gen(1)).to(dtype), torch.randn(K, d_out, d_in, generator=gen(2)).to(dtype)
+    dy = torch.randn(N * k, d_out, generator=gen(3)).to(dtype)
+    whole = C().group_routes(torch.randint(0, K, (N, k), generator=gen(4), dtype=torch.int32).to(DEV), K)
+    for seed in range(3):
+        off = torch.randint(-5, N * k + 5, (K + 1,), generator=gen(seed), dtype=torch.int32)
+        off[0], off[K] = 0, N * k
+        routes = whole._replace(offsets=off.to(DEV))
+        stale(*[1 << i for i in range(10, 25)])
+        assert torch.isfinite(C().expert_products(x.to(DEV), w.to(DEV), routes)).all()
+        gx, gw = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes)
+        assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
