@@ -242,6 +242,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, 
   }
 }
 
+// d_weights of the slots that `order` leaves out (a plan of a part of the experts) stay 0.
+__global__ void __launch_bounds__(256) zero_weights_kernel(float *__restrict__ d_weights, int64_t R) {
+  griddep_wait();
+  griddep_launch();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < R; i += (int64_t)gridDim.x * 256) d_weights[i] = 0.0f;
+}
+
 // A warp per grouped row r of route order[r]: dy[r] = w dout[point], dw = <dout[point], y[r]>; U packs of both rows
 // are on their way at once.  16,411 points of 2 rows of 1,000 fp32 (328 MB) 54 us, 6.1 TB/s.
 template <typename T, int V, int U>
@@ -324,6 +331,7 @@ int combine_backward_t(const T *g, const T *y, int d, const float *w, const Rout
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(dy) % 16 == 0;
   const unsigned grid = (unsigned)cdiv(p.R, 4);
+  FGMM_CUDA_TRY(launch_pdl(zero_weights_kernel, dim3((unsigned)std::min<int64_t>(cdiv(p.R, 256), 8 * num_sms())), dim3(256), 0, st, dw, p.R));
   auto *kernel = !vec ? combine_backward_kernel<T, 1, 4>
                  : d <= 32 * V ? combine_backward_kernel<T, V, 1>
                  : d <= 64 * V ? combine_backward_kernel<T, V, 2> : combine_backward_kernel<T, V, 4>;

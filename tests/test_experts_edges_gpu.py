@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import experts_ref as ref
-from experts_ref import F32_MAX
+from experts_ref import F32_MAX, HALF_STEP
 from test_experts_gpu import C, DEV, FUNCS, TYPES, close, gen, plan
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,24 @@ def test_dx_of_a_plan_whose_offsets_do_not_ascend(dtype, N, k, K, d_in, d_out):
         assert torch.isfinite(C().expert_products(x.to(DEV), w.to(DEV), routes)).all()
         gx, gw = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes)
         assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,k,d", [(5, 3, 7), (40, 2, 64), (300, 4, 264)])
+def test_weights_gradient_of_slots_that_order_leaves_out(dtype, N, k, d):
+    """A plan of a part of the experts: the other routes' places in order hold no route, and their slots' gradient is 0."""
+    K = 8
+    idx = torch.randint(0, K, (N, k), generator=gen(N), dtype=torch.int32)
+    routes = C().group_routes(idx.to(DEV), K)
+    y, wt, g = torch.randn(N * k, d, generator=gen(1)).to(dtype), torch.randn(N, k, generator=gen(2)), torch.randn(N, d, generator=gen(3)).to(dtype)
+    away = idx >= 5
+    order = torch.where(away.flatten()[routes.order.long().cpu()], -1, routes.order.cpu())
+    position = torch.where(away, -1, routes.position.cpu())
+    part = routes._replace(order=order.to(DEV), position=position.to(DEV))
+    _, _, dy, dw, dwa = ref.combine(y, wt, position, g)
+    for _ in range(3):
+        stale(*[1 << i for i in range(2, 16)])
+        gy, gw = C().combine_experts_backward(g.to(DEV), y.to(DEV), wt.to(DEV), part)
+        assert (gw.cpu()[away] == 0).all() and (gy.cpu()[order < 0] == 0).all()
+        assert ((gw.double().cpu() - dw).abs() <= (d / 32 + 8) * 2.0 ** -24 * 2 * dwa).all()
+        assert ((gy.double().cpu() - dy).abs() <= (2.0 ** -24 + HALF_STEP[dtype]) * dy.abs() * 1.001 + 2.0 ** -24 * (dtype == torch.float16)).all()
