@@ -111,6 +111,9 @@ __device__ __forceinline__ int find_expert(const int *s_first, int K, int m) {
   return lo;
 }
 
+// a + b up to `most` (all >= 0).  Offsets that do not ascend can claim more tiles than 32 bits count: those past `most` are left out.
+__device__ __forceinline__ int add_to(int a, int b, int most) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)most); }
+
 __device__ __forceinline__ int expert_stages(const RoutePlan &p, int e) {
   int lo, hi;
   expert_rows(p.offsets, e, (int)p.R, lo, hi);
@@ -151,7 +154,7 @@ struct Tiles {
       x.c0 = piece * a.pieces.most;
       x.c1 = min(max(1, (x.r1 - x.r0 + KCH - 1) / KCH), x.c0 + a.pieces.most);
       x.slot = -1;
-      if (pieces > 1) x.slot = min((__ldg(a.pieces.slot + x.e) + piece) * per() + tile, a.pieces.slots - 1);
+      if (pieces > 1) x.slot = (int)min(((int64_t)__ldg(a.pieces.slot + x.e) + piece) * per() + tile, (int64_t)a.pieces.slots - 1);
       ++i;
     } else {
       const int4 f = i < kList ? s_list[i] : find((int)t);
@@ -231,21 +234,22 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     };
     const int per = (K + kThreads - 1) / kThreads;
     const int e0 = min(K, (int)threadIdx.x * per), e1 = min(K, e0 + per);
-    int mine = 0;
-    for (int e = e0; e < e1; ++e) mine += units(e);
-    int sum = mine;
+    const int most = INT32_MAX / (((MODE == kForward ? a.d_out : a.d_in) + NT - 1) / NT);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) sum = add_to(sum, units(e), most);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
+      if (lane >= o) sum = add_to(sum, v, most);
     }
     if (lane == 31) s_warp[warp] = sum;
+    int run = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane == 0) run = 0;
     __syncthreads();
-    int run = sum - mine;
-    for (int w = 0; w < warp; ++w) run += s_warp[w];
+    for (int w = 0; w < warp; ++w) run = add_to(run, s_warp[w], most);
     for (int e = e0; e < e1; ++e) {
       s_first[e] = run;
-      run += units(e);
+      run = add_to(run, units(e), most);
     }
     if (threadIdx.x == kThreads - 1) s_first[K] = run;
   }
@@ -596,7 +600,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 
 // The pieces of DW: one block.
 constexpr int kPlanThreads = 512;
-__global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, int most, int *__restrict__ first, int *__restrict__ slot,
+__global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, int most, int limit, int *__restrict__ first, int *__restrict__ slot,
                                                                    int *__restrict__ joined) {
   __shared__ int s_warp[kPlanThreads / 32][3];
   griddep_launch();
@@ -610,11 +614,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, 
     int sum[3];
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      sum[q] = mine[q];
+      sum[q] = min(mine[q], limit);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, sum[q], o);
-        if (lane >= o) sum[q] += v;
+        if (lane >= o) sum[q] = add_to(sum[q], v, limit);
       }
       if (lane == 31) s_warp[warp][q] = sum[q];
     }
@@ -622,10 +626,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pieces_kernel(RoutePlan p, 
     int before[3];
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      before[q] = run[q] + sum[q] - mine[q];
+      const int prev = __shfl_up_sync(0xffffffffu, sum[q], 1);
+      before[q] = add_to(run[q], lane > 0 ? prev : 0, limit);
       for (int w = 0; w < kPlanThreads / 32; ++w) {
-        if (w < warp) before[q] += s_warp[w][q];
-        run[q] += s_warp[w][q];
+        if (w < warp) before[q] = add_to(before[q], s_warp[w][q], limit);
+        run[q] = add_to(run[q], s_warp[w][q], limit);
       }
     }
     if (e <= p.K) {
@@ -660,8 +665,8 @@ __global__ void __launch_bounds__(256) join_pieces_kernel(const __grid_constant_
     float f[4] = {};
 #pragma unroll 8
     for (int q = 0; q < n; ++q) {
-      const int s = min((first + q) * per + tile, a.pieces.slots - 1);
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(from + (int64_t)s * BM * NT));
+      const int64_t s = min(((int64_t)first + q) * per + tile, (int64_t)a.pieces.slots - 1);
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(from + s * BM * NT));
       f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
     }
     OUT *to = out + ((int64_t)lo * a.d_out + o) * a.d_in + col;
@@ -850,7 +855,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
     int *first = c.take<int>(p.K + 1), *slot = c.take<int>(p.K + 1), *joined = c.take<int>(p.K + 1);
     a.pieces = {first, slot, joined, c.take<float>(z.slots * BM * NT), (int)z.most, (int)z.slots};
     if (z.slots > 1)
-      FGMM_CUDA_TRY(launch_pdl(plan_pieces_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, (int)z.most, first, slot, joined));
+      FGMM_CUDA_TRY(launch_pdl(plan_pieces_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, (int)z.most, (int)(INT32_MAX / z.per), first, slot, joined));
     FGMM_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(num_sms(), (cdiv(p.R, KCH * z.most) + p.K) * z.per)), dim3(kThreads),
                              Sh::smem(p.K), st, ma, mb, a, out));
     if (z.slots > 1)

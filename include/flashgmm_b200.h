@@ -243,8 +243,9 @@ int fgmm_group_routes(const int32_t *indices, int64_t R, int32_t K, int32_t *ord
 
 /* y[r] = weight[e] x[n] for every grouped row r (route order[r] of point n, expert e), x[N][d_in],
  * weight[K][d_out][d_in], y[N top_k][d_out]; rows of no expert are 0.  `order` and `offsets` are those of
- * fgmm_group_routes: entries out of range are treated as rows of no expert, never read through.  x and weight start on 16-byte
- * boundaries.  float32 operands run as three bf16 planes (24 bits together). */
+ * fgmm_group_routes.  An entry of `order` out of range reads as a point of zeros, offsets as far as they are in range, and
+ * position (below) leads to rows before offsets[K] only; a plan of a part of the experts is made that way.  Offsets that do not
+ * ascend give results of no meaning, without an access out of bounds.  x and weight start on 16-byte boundaries.  float32 operands run as three bf16 planes (24 bits together). */
 size_t fgmm_expert_products_workspace_bytes(int32_t dtype, int64_t N, int32_t K, int32_t d_in,
                                             int32_t d_out, int32_t top_k);
 int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, const void *weight,
@@ -266,7 +267,7 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
 int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,
                          const int32_t *position, int32_t top_k, void *out, void *stream);
 
-/* dy[N top_k][d] and d_weights[N][top_k] from d_out[N][d]; rows and slots of no expert get 0. */
+/* dy[N top_k][d] and d_weights[N][top_k] from d_out[N][d]; rows of no expert, and slots that `order` leaves out or of no expert, get 0. */
 int fgmm_combine_experts_backward(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
                                   const float *weights, const int32_t *order, const int32_t *offsets,
                                   int32_t K, int32_t top_k, void *dy, float *d_weights, void *stream);

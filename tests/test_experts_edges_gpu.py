@@ -161,6 +161,26 @@ def test_dx_of_a_plan_whose_offsets_do_not_ascend(dtype, N, k, K, d_in, d_out):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_a_plan_in_which_half_of_the_experts_claim_every_row(dtype):
+    """2,048 times the tiles of a plan that ascends, counted up to what 32 bits hold."""
+    N, k, K, d = 9000, 2, 4096, 64
+    x, w = torch.randn(N, d, generator=gen(1)).to(dtype).to(DEV), torch.randn(1, d, d, generator=gen(2)).to(dtype).to(DEV).expand(K, d, d).contiguous()
+    dy = torch.randn(N * k, d, generator=gen(3)).to(dtype).to(DEV)
+    whole = C().group_routes(torch.zeros(N, k, dtype=torch.int32, device=DEV), K)
+    off = torch.zeros(K + 1, dtype=torch.int32)
+    off[1::2] = N * k
+    off[K] = N * k
+    routes = whole._replace(offsets=off.to(DEV))
+    stale(*[1 << i for i in range(10, 25)])
+    # every expert holds the same matrix: whichever of them writes a row last, it is the same row
+    assert torch.equal(C().expert_products(x, w, routes), C().expert_products(x, w, whole))
+    gx, gw = C().expert_products_backward(dy, x, w, routes)
+    assert torch.equal(gx, C().expert_products_backward(dy, x, w, whole)[0])
+    assert gw.shape == w.shape
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,k,d", [(5, 3, 7), (40, 2, 64), (300, 4, 264)])
 def test_weights_gradient_of_slots_that_order_leaves_out(dtype, N, k, d):
     """A plan of a part of the experts: the other routes' places in order hold no route, and their slots' gradient is 0."""
