@@ -13,7 +13,7 @@ unmodified on the CUDA kernels.
 from flashgmm_b200._ext import load as _load_ext
 from flashgmm_b200 import experts as _experts
 from flashgmm_b200.experts import (  # noqa: F401
-    Routes, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
+    Routes, check_expert_products, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
     group_routes, route_experts, route_experts_backward)
 from flashgmm_b200.flash_gmm_native import (  # noqa: F401
     StatsWorkspace, em_stats, em_step, em_update, em_update_prepared, family_for,

@@ -19,6 +19,7 @@ FGMM_ERR_CUDA = 4
 FAMILY_AUTO, FAMILY_SIMT, FAMILY_TC, FAMILY_LOWK = 0, 1, 2, 3
 UPDATE_NO_FLOORS = 1
 F32, BF16, F16 = 0, 1, 2
+KERNELS_EM, KERNELS_EXPERTS = 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID, SCORE_GIVEN = 0, 1, 2
 MAX_EXPERTS, MAX_TOP_K, MAX_SCORE_GROUPS = 4096, 32, 32
 
@@ -42,6 +43,8 @@ SIGNATURES = {
     "fgmm_em_step": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp,
                                     _vp, _sz, _i32, _vp]),
     "fgmm_device_error": (ctypes.c_int, [ctypes.c_int]),
+    "fgmm_device_error_of": (ctypes.c_int, [_i32, ctypes.c_int]),
+    "fgmm_expert_error_word": (ctypes.POINTER(ctypes.c_int32), []),
     "fgmm_em_stats_launches": (ctypes.c_int, [_i64, _i32, _i32]),
     "fgmm_em_stats_profiled": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _sz, _vp,
                                               ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_char_p), _i32]),
@@ -113,11 +116,12 @@ class DeviceWaitError(RuntimeError):
     every launch since) are incomplete."""
 
 
-def check_device_error():
-    """Raise :class:`DeviceWaitError` if a tensor-core kernel recorded a wait timeout on
+def check_device_error(kernels=KERNELS_EM):
+    """Raise :class:`DeviceWaitError` if a tensor-core kernel of the EM steps (or of
+    ``KERNELS_EXPERTS``, the expert products) recorded a wait timeout on
     the current device since the last check (the code is cleared).  Synchronises the
     device: call it where the host already waits for results."""
-    code = load().fgmm_device_error(1)
+    code = load().fgmm_device_error_of(kernels, 1)
     if code < 0:
         raise DeviceWaitError("fgmm_device_error: CUDA error while reading the device error word")
     if code:

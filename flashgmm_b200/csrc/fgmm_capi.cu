@@ -299,10 +299,13 @@ int fgmm_m_step(const float *X, int64_t N, int32_t d, const float *gamma, int32_
   return em_update(stats, (double)N, K, d, new_mu, new_var, new_log_pi, st, /*floors=*/false);
 }
 
-int fgmm_device_error(int reset) {
-  const int a = tc_device_error(reset != 0), b = experts_device_error(reset != 0);
+int fgmm_device_error_of(int32_t kernels, int reset) {
+  const int a = kernels & FGMM_KERNELS_EM ? tc_device_error(reset != 0) : 0;
+  const int b = kernels & FGMM_KERNELS_EXPERTS ? experts_device_error(reset != 0) : 0;
   return a ? a : b;
 }
+
+int fgmm_device_error(int reset) { return fgmm_device_error_of(FGMM_KERNELS_EM | FGMM_KERNELS_EXPERTS, reset); }
 
 int fgmm_em_stats_launches(int64_t N, int32_t d, int32_t K) {
   const int fam = resolve_family(N, d, K);

@@ -73,6 +73,8 @@ int products_few_dx(const void *dy, const void *weight, int dtype, int d_in, int
 int products_few_dw(const void *dy, const void *x, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *d_weight, cudaStream_t st);
 
 // ---- fgmm_experts_tc.cu: tensor-core products ----
+int take_failure(cudaStream_t st);  // the error of an earlier product whose wait ran out, once
+int *experts_error_word();
 // Which of the three products run there; the others cost no workspace.
 struct TcParts {
   bool forward, inputs, weights;

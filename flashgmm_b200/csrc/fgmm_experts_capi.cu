@@ -135,6 +135,7 @@ int fgmm_expert_products(const void *x, int32_t dtype, int64_t N, int32_t d_in, 
     return fail(FGMM_ERR_INVALID, "x and weight must be 16-byte aligned, y to its elements, the workspace to 256 bytes");
   if (workspace_bytes < fgmm_expert_products_workspace_bytes(dtype, N, K, d_in, d_out, top_k))
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
+  if ((rc = take_failure((cudaStream_t)stream))) return rc;
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
   if (!on_tensor_cores(dtype, plan.R, K, d_in, d_out).forward)
     return products_few(x, weight, dtype, N, d_in, d_out, plan, y, (cudaStream_t)stream);
@@ -170,6 +171,7 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
     return fail(FGMM_ERR_INVALID, "dy, x and weight must be 16-byte aligned, the results to their elements, the workspace to 256 bytes");
   if (workspace_bytes < fgmm_expert_products_backward_workspace_bytes(dtype, N, K, d_in, d_out, top_k))
     return fail(FGMM_ERR_WORKSPACE, "workspace too small");
+  if ((rc = take_failure(st))) return rc;
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
   // the rows of dx first, in fp32: their sum over a point's slots rounds once
   TcParts tc = on_tensor_cores(dtype, plan.R, K, d_in, d_out);
@@ -186,6 +188,8 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
   if (rc || !dx) return rc;
   return sum_rows(dx_rows, parts, dtype, d_in, plan, position, N, dx, st);
 }
+
+const volatile int32_t *fgmm_expert_error_word(void) { return experts_error_word(); }
 
 int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, const float *weights,
                          const int32_t *position, int32_t top_k, void *out, void *stream) {

@@ -53,6 +53,13 @@ __device__ __forceinline__ int ld_now(const int32_t *p) {
   return v;
 }
 
+// A wait of this launch ran out: the host learns of it without synchronising.
+__device__ __noinline__ void report(int *failed) {
+  const int code = *(volatile int *)&g_dev_error;
+  *(volatile int *)failed = code != 0 ? code : kErrWaitDrain;
+  __threadfence_system();
+}
+
 enum { kForward = 0, kInputs = 1, kWeights = 2 };
 
 template <int NT, bool SPLIT>
@@ -92,6 +99,7 @@ struct TcArgs {
   Pieces pieces;  // DW
   uint32_t div_mul, div_shift;  // n / top_k = n * div_mul >> div_shift for n < 2^31
   int vec, vec32;  // rows of the result start on 16-byte, 32-byte boundaries
+  int *failed;     // the host's word for a wait that ran out
 };
 
 // What one tile covers.  For Y and DX: `rows` rows from r0 of expert e, columns from n0.  For DW: `rows` output dimensions
@@ -305,8 +313,9 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       for (int i = 0; i < filled; ++i) {
         stage = stage == 0 ? S - 1 : stage - 1;
         if (stage == S - 1) phase ^= 1;
-        mbar_wait_drain(FULL(stage), phase);
+        ok = mbar_wait_drain(FULL(stage), phase) && ok;
       }
+      if (!ok) report(a.failed);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -358,7 +367,8 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         } while (c < x.c1);
       }
       mma_commit(DONE);
-      mbar_wait_drain(DONE, 0);
+      ok = mbar_wait_drain(DONE, 0) && ok;
+      if (!ok) report(a.failed);
     }
     __syncwarp();
   } else if (warp < 2 + kGather / 32) {
@@ -456,6 +466,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
       }
       cp_async_wait_all();
+      if (!ok && lane == 0) report(a.failed);
     }
   } else {
     // ---------------------------------------------------------------- epilogue
@@ -589,6 +600,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         ++seg;
       } while (c < x.c1);
     }
+    if (!ok && lane == 0) report(a.failed);
   }
   tc_fence_before();
   __syncthreads();
@@ -734,6 +746,28 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant
   }
 }
 
+// A word of pinned host memory for each device, which a product whose wait ran out sets: the next product on that device fails
+// with it.  Allocated with the first product (also where that is being captured: nothing of it goes into the graph).
+int *failed_word() {
+  static std::mutex mutex;
+  static int *words = nullptr;
+  constexpr int kDevices = 64;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+  std::lock_guard<std::mutex> lock(mutex);
+  if (!words) {
+    void *p = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return nullptr;
+    words = static_cast<int *>(p);
+    std::fill(words, words + kDevices, 0);
+  }
+  return words + dev % kDevices;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -840,6 +874,8 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   a.idesc = idesc_f16(BM, NT, MODE == kWeights, MODE != kForward, bf16);
   a.vec32 = (width * sizeof(OUT)) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  a.failed = failed_word();
+  if (!a.failed) return fail(FGMM_ERR_CUDA, "no pinned memory for the products' error word");
   auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
   static std::atomic<bool> done[64];  // per device
   int dev = 0;
@@ -895,7 +931,35 @@ size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
 
 }  // namespace
 
-int experts_device_error(bool reset) { return read_dev_error(reset); }
+int experts_device_error(bool reset) {
+  const int code = read_dev_error(reset);
+  volatile int *word = failed_word();
+  const int told = word ? *word : 0;
+  if (reset && word) *word = 0;
+  return code ? code : told;
+}
+
+int *experts_error_word() { return failed_word(); }
+
+// Takes an earlier product's failure.  The device's word is cleared in the stream's order, so that later waits do not give up
+// for it; a capture leaves both words as they are.
+int take_failure(cudaStream_t st) {
+  volatile int *word = failed_word();
+  const int code = word ? *word : 0;
+  if (code == 0) return FGMM_OK;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &status) != cudaSuccess) {
+    cudaGetLastError();
+    status = cudaStreamCaptureStatusActive;
+  }
+  if (status == cudaStreamCaptureStatusNone) {
+    static const int zero = 0;
+    *word = 0;
+    FGMM_CUDA_TRY(cudaMemcpyToSymbolAsync(g_dev_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+  }
+  return fail(FGMM_ERR_CUDA, "an earlier expert product on this device gave up a bounded wait (code " + std::to_string(code) +
+                                 "): its results are incomplete");
+}
 
 namespace {
 // The workspace: copies of the operands that TMA cannot read, and DW's pieces.

@@ -16,7 +16,9 @@ indices int32), run on the current stream of the tensors' device and hold their 
 input requires a gradient, the functions record one; the ``*_backward`` functions are the same
 gradients without autograd; a step that is captured into a CUDA graph while an eager autograd graph of the
 same leaves is alive takes those (autograd then joins the eager graph's stream to the capture, which CUDA
-refuses).  Forward-mode tangents and traced, batched (``torch.func``) or wrapped tensors are refused.  The
+refuses).  Every wait inside the products' kernels is bounded: one that runs out leaves incomplete results, which
+the next product on that device raises a RuntimeError for; :func:`check_expert_products` tells of it at once.
+Forward-mode tangents and traced, batched (``torch.func``) or wrapped tensors are refused.  The
 reference has no counterpart; its E-step (``flash_gmm/csrc/binding.cpp:35-49``) gives the scores of a fitted
 mixture's gate.
 """
@@ -24,10 +26,10 @@ from typing import NamedTuple
 
 import torch
 
-from . import _ext
+from . import _ext, _lib
 
 __all__ = ["Routes", "route_experts", "route_experts_backward", "group_routes", "expert_products",
-           "expert_products_backward", "combine_experts", "combine_experts_backward"]
+           "expert_products_backward", "combine_experts", "combine_experts_backward", "check_expert_products"]
 
 
 class Routes(NamedTuple):
@@ -165,6 +167,13 @@ def expert_products_backward(dy, x, weight, routes, need_dx=True, need_dweight=T
         return list((_ops or _load()).expert_products_backward(dy, x, weight, order, offsets, position, need_dx, need_dweight))
     except (TypeError, ValueError) as error:
         _refuse(error, routes, dy=dy, x=x, weight=weight)
+
+
+def check_expert_products():
+    """Raises :class:`flashgmm_b200._lib.DeviceWaitError` if a product on the current device gave up a bounded wait since the
+    last check or error.  Synchronises the device: for places where the host waits anyway, and after the last product of a
+    program or the replay of a captured one, which no later call looks at."""
+    _lib.check_device_error(_lib.KERNELS_EXPERTS)
 
 
 class _Combine(torch.autograd.Function):

@@ -22,7 +22,7 @@ import torch
 from . import _lib
 from . import experts as _experts
 from .experts import (  # noqa: F401
-    Routes, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
+    Routes, check_expert_products, combine_experts, combine_experts_backward, expert_products, expert_products_backward,
     group_routes, route_experts, route_experts_backward)
 
 __all__ = ["flash_em_fused", "standard_e_step", "flash_e_step", "standard_m_step", "em_stats", "em_step",

@@ -61,7 +61,8 @@ class _EMModel:
     def mix_experts(self, X: torch.Tensor, weight: torch.Tensor, top_k: int) -> torch.Tensor:
         """A mixture of linear experts ``weight[K, d_out, d]`` with the fitted mixture as its gate:
         ``out[n] = sum_j w[n, j] weight[indices[n, j]] @ X[n]`` over :meth:`route`'s leading
-        components.  Gradients flow to ``weight`` and ``X`` through the experts, not the gate."""
+        components.  Gradients flow to ``weight`` and ``X`` through the experts, not the gate.  A product that gave
+        up a bounded wait raises in the next call (``check_expert_products()`` tells at once)."""
         X = self._to_device(X)
         weights, indices = self.route(X.detach(), top_k)
         routes = _C.group_routes(indices, self.K)

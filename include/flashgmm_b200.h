@@ -174,6 +174,11 @@ int fgmm_m_step(const float *X, int64_t N, int32_t d, const float *gamma, int32_
  * error.  Has no counterpart in the reference (its kernels have no waits). */
 int fgmm_device_error(int reset);
 
+/* The same of some kernels only: those of the EM steps, of the expert products, or both. */
+#define FGMM_KERNELS_EM 1
+#define FGMM_KERNELS_EXPERTS 2
+int fgmm_device_error_of(int32_t kernels, int reset);
+
 /* Number of kernel launches one fgmm_em_stats call makes for this shape
  * (fgmm_em_update adds one more). */
 int fgmm_em_stats_launches(int64_t N, int32_t d, int32_t K);
@@ -200,7 +205,9 @@ int fgmm_em_stats_profiled(const float *X, const void *points, int64_t N, int32_
  * Element types of scores, x, weight, y and their gradients: FGMM_F32, FGMM_BF16, FGMM_F16, one type in a
  * call; sums are held in fp32.  Weights, their gradients and the bias are fp32, indices int32.
  * K <= FGMM_MAX_EXPERTS, N top_k <= 2^31 - 1025, top_k of the routing <= FGMM_MAX_TOP_K.  N = 0 is
- * allowed.  All calls only enqueue work on `stream` and may be captured; each uses its own workspace. */
+ * allowed.  All calls only enqueue work on `stream` and may be captured; each uses its own workspace.
+ * A product whose bounded wait ran out leaves incomplete results; the next product on that device (outside of a capture) fails with
+ * FGMM_ERR_CUDA and clears it, and fgmm_device_error_of(FGMM_KERNELS_EXPERTS, 1) tells of it where the host waits anyway. */
 #define FGMM_F32 0
 #define FGMM_BF16 1
 #define FGMM_F16 2
@@ -261,6 +268,10 @@ int fgmm_expert_products_backward(const void *dy, const void *x, int32_t dtype, 
                                   const int32_t *offsets, const int32_t *position, int32_t top_k,
                                   void *dx, void *d_weight, void *workspace, size_t workspace_bytes,
                                   void *stream);
+
+/* The current device's word of pinned host memory that such a product sets to its code (0 = none): a program that replays
+ * captured products reads it without synchronising.  NULL on a CUDA error. */
+const volatile int32_t *fgmm_expert_error_word(void);
 
 /* out[n] = sum_j weights[n][j] y[position[n][j]], y[N top_k][d], places outside [0, N top_k)
  * skipped. */

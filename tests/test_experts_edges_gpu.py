@@ -199,3 +199,79 @@ def test_weights_gradient_of_slots_that_order_leaves_out(dtype, N, k, d):
         assert (gw.cpu()[away] == 0).all() and (gy.cpu()[order < 0] == 0).all()
         assert ((gw.double().cpu() - dw).abs() <= (d / 32 + 8) * 2.0 ** -24 * 2 * dwa).all()
         assert ((gy.double().cpu() - dy).abs() <= (2.0 ** -24 + HALF_STEP[dtype]) * dy.abs() * 1.001 + 2.0 ** -24 * (dtype == torch.float16)).all()
+
+
+# --------------------------------------------------------------- waits that have run out
+def a_wait_ran_out():
+    """What the products' kernels leave behind: a code in the device's word of host memory."""
+    from flashgmm_b200 import _lib
+    word = _lib.load().fgmm_expert_error_word()
+    word[0] = 3
+    return word
+
+
+def test_a_wait_that_ran_out_is_raised_by_the_next_product():
+    from flashgmm_b200 import _lib
+    idx = torch.randint(0, 4, (200, 2), generator=gen(1), dtype=torch.int32).to(DEV)
+    routes = C().group_routes(idx, 4)
+    x, w = torch.randn(200, 64, device=DEV).bfloat16(), torch.randn(4, 72, 64, device=DEV).bfloat16()
+    want = C().expert_products(x, w, routes)
+    dx, dw = C().expert_products_backward(want, x, w, routes)
+    leaf = x.clone().requires_grad_()
+    calls = [lambda: C().expert_products(x, w, routes), lambda: C().expert_products_backward(want, x, w, routes),
+             lambda: C().expert_products(leaf, w, routes), lambda: C().expert_products(x[:1, :8].float(), w[:, :8, :8].float(),
+                                                                                       C().group_routes(idx[:1], 4))]
+    for call in calls:
+        word = a_wait_ran_out()
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            call()
+        assert word[0] == 0
+        call()
+    y = C().expert_products(leaf, w, routes)
+    a_wait_ran_out()
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        y.backward(want)
+    a_wait_ran_out()
+    with pytest.raises(_lib.DeviceWaitError):
+        C().check_expert_products()
+    C().check_expert_products()
+    assert torch.equal(C().expert_products(x, w, routes), want)
+    assert all(torch.equal(a, b) for a, b in zip(C().expert_products_backward(want, x, w, routes), (dx, dw)))
+
+
+def test_a_wait_that_ran_out_and_a_capture():
+    """A capture does not clear the word: the call fails, and the next call outside of it fails too, once."""
+    idx = torch.randint(0, 4, (200, 2), generator=gen(1), dtype=torch.int32).to(DEV)
+    x, w = torch.randn(200, 64, device=DEV), torch.randn(4, 72, 64, device=DEV)
+    routes = C().group_routes(idx, 4)
+    want = C().expert_products(x, w, routes)
+    torch.cuda.synchronize()
+    word = a_wait_ran_out()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        with torch.cuda.graph(graph):
+            x + 1
+            C().expert_products(x, w, routes)
+    assert word[0] == 3
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        C().expert_products(x, w, routes)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = C().expert_products(x, w, routes)
+    graph.replay()
+    assert torch.equal(y, want)
+
+
+def test_a_fit_does_not_answer_for_the_products():
+    from flashgmm_b200 import native_wrapper
+    from flashgmm_b200.data import make_mixture
+    N, K, d = 2000, 16, 32
+    X = make_mixture(N, K, d, seed=3)[0].to(DEV)
+    m = native_wrapper.NativeFlashGMM(K, d, max_iter=3)
+    weight = torch.randn(K, 8, d, device=DEV)
+    word = a_wait_ran_out()
+    m.fit(X)
+    assert word[0] == 3
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        m.mix_experts(X, weight, 2)
+    assert torch.isfinite(m.mix_experts(X, weight, 2)).all()
