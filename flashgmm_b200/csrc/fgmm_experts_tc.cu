@@ -19,6 +19,9 @@
 //     split_planes_kernel, and the six products that matter (b0 b0 into one accumulator; b0 b1, b1 b0, b1 b1,
 //     b0 b2 and b2 b0, 2^-8 and less of it, into another).  Tensor-memory accumulation truncates, so the
 //     first is drained into fp32 registers every 256 elements of the contraction.
+//   * 16-bit products are drained every 8,192 elements: truncation takes up to 2^-23 of the sum for every 8, of a sum of one sign
+//     2^-27.3 an element (8,192: 2^-14.3, a tenth of the rounding to fp16; undrained 2^20 rows lost 0.6 %).  The sums of a
+//     longer contraction wait in a tile of fp32 for each block, whose threads read and write their own elements only.
 //   * 16-bit operands whose rows are no multiple of 16 bytes are copied to padded rows first (TMA strides).
 // What bounds it is shared memory at 128 bytes a cycle: a stage of 128 x 256 x 64 16-bit products writes and reads 96 KB, 768
 // cycles, for 512 of tensor time; one of three planes and 128 columns 288 KB, 2,304 for 1,536.  8,192 points with 4 of 64
@@ -45,6 +48,7 @@ constexpr int kEpiWarps = 8;   // warps 6-13: two per tensor-memory lane quarter
 constexpr int kThreads = 64 + kGather + 32 * kEpiWarps;  // warp 0 TMA, warp 1 MMA
 constexpr int kList = 64;      // tiles of a block that are found ahead
 constexpr int kSegment = 4;   // stages between drains of a float32 product (256 elements)
+constexpr int kLong = 128;    // of a 16-bit product (8,192 elements)
 
 // A load that stays where it is written (a plan's entry fetched a stage ahead of its use).
 __device__ __forceinline__ int ld_now(const int32_t *p) {
@@ -97,6 +101,7 @@ struct TcArgs {
   int a_cols, b_cols;               // columns of their rows in memory
   uint32_t idesc;
   Pieces pieces;  // DW
+  float *sums;    // [blocks][NT][BM]: a tile whose contraction is longer than kLong stages (16 bits)
   uint32_t div_mul, div_shift;  // n / top_k = n * div_mul >> div_shift for n < 2^31
   int vec, vec32;  // rows of the result start on 16-byte, 32-byte boundaries
   int *failed;     // the host's word for a wait that ran out
@@ -198,6 +203,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                   const __grid_constant__ TcArgs a, OUT *__restrict__ out) {
   using Sh = Shape<NT, SPLIT>;
   constexpr int P = Sh::kPlanes, S = Sh::kStages;
+  constexpr int kSeg = SPLIT ? kSegment : kLong;
   constexpr int kCols = SPLIT ? 4 * NT : 2 * NT;  // tensor-memory columns
   static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "TMEM budget");
   extern __shared__ uint8_t smem_raw[];
@@ -335,12 +341,12 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       for (; ok && tiles.next(x); ++count) {
         const uint32_t low = tmem + (2 + (count & 1)) * NT;  // the smaller products of a float32 tile
         int c = x.c0;
-        do {  // a segment: the whole tile, or kSegment stages of a float32 one
+        do {  // a segment: kSeg stages
           const int buf = seg & 1;
           if (!mbar_wait(TEMPTY(buf), ((seg >> 1) & 1) ^ 1, kErrWaitTmemEmpty)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem + buf * NT;
-          const int first = c, end = SPLIT ? min(x.c1, c + kSegment) : x.c1;
+          const int first = c, end = min(x.c1, c + kSeg);
           for (; c < end; ++c) {
             if (!mbar_wait(FULL(stage), phase, kErrWaitFull)) { ok = false; break; }
             if (MODE != kInputs) fence_proxy_async_smem();  // the gathered rows were written through the generic proxy
@@ -554,7 +560,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         ok = __all_sync(0xffffffffu, mbar_wait(TFULL(buf), (seg >> 1) & 1, kErrWaitTmemFull));
         if (!ok) break;
         tc_fence_after();
-        c = SPLIT ? c + kSegment : x.c1;
+        c += kSeg;
         if constexpr (SPLIT) {
           if (live) {
             auto add = [&](uint32_t from, bool smaller) {
@@ -580,6 +586,18 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
             for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
             tmem_wait_ld();
+            if (x.c1 - x.c0 > kLong) {  // with the segments before
+              float *sum = a.sums + ((int64_t)blockIdx.x * NT + half + i * CW) * BM + q * 32 + lane;
+              if (c - kLong > x.c0) {
+#pragma unroll
+                for (int k = 0; k < CW; ++k) acc[k] += sum[k * BM];
+              }
+              if (c < x.c1) {
+#pragma unroll
+                for (int k = 0; k < CW; ++k) sum[k * BM] = acc[k];
+                continue;
+              }
+            }
             if (MODE == kWeights && x.slot >= 0) write_piece(acc, CW, x, half + i * CW);
             else write(acc, x, half + i * CW);
           }
@@ -848,7 +866,7 @@ int weights_tile(int dtype, int d_in) { return dtype == FGMM_F32 || d_in <= 128 
 
 template <int MODE, int NT, bool SPLIT, typename OUT>
 int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
-           void *pieces, cudaStream_t st) {
+           void *pieces, float *sums, cudaStream_t st) {
   using Sh = Shape<NT, SPLIT>;
   const int bf16 = dtype != FGMM_F16, width = MODE == kForward ? d_out : d_in;
   CUtensorMap ma{}, mb{};
@@ -874,6 +892,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   a.idesc = idesc_f16(BM, NT, MODE == kWeights, MODE != kForward, bf16);
   a.vec32 = (width * sizeof(OUT)) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  a.sums = sums;
   a.failed = failed_word();
   if (!a.failed) return fail(FGMM_ERR_CUDA, "no pinned memory for the products' error word");
   auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
@@ -914,11 +933,11 @@ bool wide_tiles(int64_t R, int K, int width) {
 }
 template <int MODE, typename OUT>
 int launch16(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
-             void *pieces, cudaStream_t st) {
+             void *pieces, float *sums, cudaStream_t st) {
   const int width = MODE == kForward ? d_out : d_in;
   if (MODE == kWeights ? weights_tile(dtype, d_in) == 256 : wide_tiles(p.R, p.K, width))
-    return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
-  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, st);
+    return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
+  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
 }
 
 size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
@@ -962,10 +981,11 @@ int take_failure(cudaStream_t st) {
 }
 
 namespace {
-// The workspace: copies of the operands that TMA cannot read, and DW's pieces.
+// The workspace: copies of the operands that TMA cannot read, DW's pieces, and the blocks' tiles of long 16-bit contractions.
 struct TcSpace {
   uint16_t *x, *weight, *dy;
   char *pieces;
+  float *sums;
   size_t bytes;
 };
 TcSpace tc_space(void *ws, int dtype, int64_t N, int K, int d_in, int d_out, int top_k, const TcParts &parts) {
@@ -975,6 +995,8 @@ TcSpace tc_space(void *ws, int dtype, int64_t N, int K, int d_in, int d_out, int
   s.weight = c.take<uint16_t>(parts.forward || parts.inputs ? copy_elems(dtype, (int64_t)K * d_out, d_in) : 0);
   s.dy = c.take<uint16_t>(parts.inputs || parts.weights ? copy_elems(dtype, N * top_k, d_out) : 0);
   s.pieces = c.take<char>(parts.weights ? piece_bytes(dtype, N * top_k, K, d_in, d_out) : 0);
+  const int64_t longest = std::max<int64_t>({parts.forward ? d_in : 0, parts.inputs ? d_out : 0, parts.weights ? N * top_k : 0});
+  s.sums = c.take<float>(dtype != FGMM_F32 && longest > kLong * KCH ? (size_t)num_sms() * BM * 256 : 0);
   s.bytes = c.bytes() + 256;
   return s;
 }
@@ -991,9 +1013,9 @@ int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_i
   const Operand ox = operand(x, dtype, N, d_in, s.x, copies), ow = operand(weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, copies);
   int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
-  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, st);
-  if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, st);
-  return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, nullptr, st);
+  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, nullptr, st);
+  if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, s.sums, st);
+  return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, nullptr, s.sums, st);
 }
 
 int products_tc_backward(const void *dy, const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out,
@@ -1006,14 +1028,14 @@ int products_tc_backward(const void *dy, const void *x, const void *weight, int 
   int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
   if (parts.inputs) {
-    rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st)
-                           : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, st);
+    rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, nullptr, st)
+                           : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, s.sums, st);
     if (rc) return rc;
   }
   if (!parts.weights) return FGMM_OK;
-  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, st);
-  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, s.pieces, st);
-  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, s.pieces, st);
+  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, nullptr, st);
+  if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, s.pieces, s.sums, st);
+  return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, s.pieces, s.sums, st);
 }
 
 }  // namespace fgmm

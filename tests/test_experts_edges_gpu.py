@@ -201,6 +201,56 @@ def test_weights_gradient_of_slots_that_order_leaves_out(dtype, N, k, d):
         assert ((gy.double().cpu() - dy).abs() <= (2.0 ** -24 + HALF_STEP[dtype]) * dy.abs() * 1.001 + 2.0 ** -24 * (dtype == torch.float16)).all()
 
 
+# ------------------------------------------------------------------------------ products
+HALVES = [torch.float16, torch.bfloat16]
+
+
+def one_sign(*shape, seed, dtype):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.rand(*shape, generator=g, device=DEV) * 0.125 + 0.0625).to(dtype)
+
+
+def check_one_sign(got, want, dtype, segments):
+    """Tensor memory truncates, by less than 2^-23 of the running sum for 8 elements of the contraction: of 8,192 elements of
+    one sign less than 1,024 2^-23 / 2 of their sum.  The segments' sums are added in fp32, and the result rounds once."""
+    off = ((got.double() - want) / want).abs()
+    lim = HALF_STEP[dtype] + 2.0 ** -14 + segments * 2.0 ** -24
+    assert float(off.max()) <= lim * 1.001, (float(off.max()), lim)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("K,d_in,d_out,R", [(64, 256, 896, 1 << 20), (4, 128, 128, 1 << 20), (4, 100, 130, 300001), (64, 512, 1024, 8193), (64, 512, 1024, 70000)])
+def test_weights_gradient_of_very_many_rows_of_one_sign(K, d_in, d_out, R, dtype):
+    x, dy = one_sign(R, d_in, seed=1, dtype=dtype), one_sign(R, d_out, seed=2, dtype=dtype)
+    idx = torch.full((R, 1), 2, dtype=torch.int32, device=DEV)
+    idx[::64] = 3
+    routes = C().group_routes(idx, K)
+    gw = C().expert_products_backward(dy, x, torch.zeros(K, d_out, d_in, device=DEV, dtype=dtype), routes, need_dx=False)[1]
+    for e in (2, 3):
+        of = slice(int(routes.offsets[e]), int(routes.offsets[e + 1]))
+        want = sum(a.double().T @ b.double() for a, b in zip(dy[of].chunk(16), x[routes.order[of].long()].chunk(16)))
+        check_one_sign(gw[e], want, dtype, R // 8192 + 1)
+    assert (gw[:2] == 0).all() and (gw[4:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("d,other", [(8200, 136), (20003, 33), (65536, 520), (1 << 18, 128)])
+def test_products_of_very_wide_rows_of_one_sign(d, other, dtype):
+    N, K = 333, 2
+    idx = torch.arange(N, dtype=torch.int32, device=DEV)[:, None] % K
+    routes = C().group_routes(idx, K)
+    rows = routes.order.long()
+    at = [slice(int(a), int(b)) for a, b in zip(routes.offsets[:-1], routes.offsets[1:])]
+    x, w = one_sign(N, d, seed=1, dtype=dtype), one_sign(K, other, d, seed=2, dtype=dtype) / 16
+    y = C().expert_products(x, w, routes)
+    for e in range(K):
+        check_one_sign(y[at[e]], x[rows[at[e]]].double() @ w[e].double().T, dtype, d // 8192 + 1)
+    dy, w = one_sign(N, d, seed=3, dtype=dtype), one_sign(K, d, other, seed=4, dtype=dtype) / 16
+    dx = C().expert_products_backward(dy, torch.zeros(N, other, device=DEV, dtype=dtype), w, routes, need_dweight=False)[0]
+    for e in range(K):
+        check_one_sign(dx[rows[at[e]]], dy[at[e]].double() @ w[e].double(), dtype, d // 8192 + 1)
+
+
 # --------------------------------------------------------------- waits that have run out
 def a_wait_ran_out():
     """What the products' kernels leave behind: a code in the device's word of host memory."""
