@@ -21,7 +21,8 @@
 //     first is drained into fp32 registers every 256 elements of the contraction.
 //   * 16-bit products are drained every 8,192 elements: truncation takes up to 2^-23 of the sum for every 8, of a sum of one sign
 //     2^-27.3 an element (8,192: 2^-14.3, a tenth of the rounding to fp16; undrained 2^20 rows lost 0.6 %).  The sums of a
-//     longer contraction wait in a tile of fp32 for each block, whose threads read and write their own elements only.
+//     longer contraction wait in a tile of fp32 for each block, whose threads read and write their own elements only (dW of 64
+//     experts of 16,384 rows, 256 -> 896: 645 -> 677 us; y of 32,768 -> 1,024, 4,096 rows: 239 -> 254).
 //   * 16-bit operands whose rows are no multiple of 16 bytes are copied to padded rows first (TMA strides).
 // What bounds it is shared memory at 128 bytes a cycle: a stage of 128 x 256 x 64 16-bit products writes and reads 96 KB, 768
 // cycles, for 512 of tensor time; one of three planes and 128 columns 288 KB, 2,304 for 1,536.  8,192 points with 4 of 64
@@ -197,13 +198,15 @@ __device__ __forceinline__ uint4 pack16(const float *v) {
   }
 }
 
-template <int MODE, int NT, bool SPLIT, typename OUT>
+// LONG: a 16-bit contraction may have more than kLong stages (instances of their own for Y and DX, whose others keep their
+// registers).
+template <int MODE, int NT, bool SPLIT, bool LONG, typename OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                   const __grid_constant__ TcArgs a, OUT *__restrict__ out) {
   using Sh = Shape<NT, SPLIT>;
   constexpr int P = Sh::kPlanes, S = Sh::kStages;
-  constexpr int kSeg = SPLIT ? kSegment : kLong;
+  constexpr int kSeg = SPLIT ? kSegment : LONG ? kLong : 1 << 26;  // (more than any contraction has)
   constexpr int kCols = SPLIT ? 4 * NT : 2 * NT;  // tensor-memory columns
   static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0, "TMEM budget");
   extern __shared__ uint8_t smem_raw[];
@@ -341,7 +344,7 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       for (; ok && tiles.next(x); ++count) {
         const uint32_t low = tmem + (2 + (count & 1)) * NT;  // the smaller products of a float32 tile
         int c = x.c0;
-        do {  // a segment: kSeg stages
+        do {  // a segment: kSeg stages at most
           const int buf = seg & 1;
           if (!mbar_wait(TEMPTY(buf), ((seg >> 1) & 1) ^ 1, kErrWaitTmemEmpty)) { ok = false; break; }
           tc_fence_after();
@@ -546,6 +549,37 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       float4 *to = reinterpret_cast<float4 *>(a.pieces.tiles + ((int64_t)x.slot * BM + q * 32 + lane) * NT + c0);
       for (int k = 0; k < n / 4; ++k) to[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
     };
+    // a segment of a long contraction: a row a lane, 32 columns at a time, added to the segments before in the block's tile of sums
+    // and, with the last one, written
+    auto add_segment = [&](const Tile &x, uint32_t from, bool first, bool last) {
+      const int row = q * 32 + lane;
+      float *sum = a.sums + ((int64_t)blockIdx.x * NT + half) * BM + row;
+      OUT *to = out + ((MODE == kWeights ? (int64_t)x.e * a.d_out + x.m0 : x.r0) + row) * width + x.n0 + half;
+#pragma unroll 1
+      for (int i = 0; i < HC; i += 32, from += 32, sum += 32 * BM) {
+        float v[32];
+        tmem_ld32(from, v);
+        tmem_wait_ld();
+        if (!first) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] += sum[k * BM];
+        }
+        if (!last) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) sum[k * BM] = v[k];
+        } else if (MODE == kWeights && x.slot >= 0) {
+          write_piece(v, 32, x, half + i);
+        } else if (row < x.rows && a.vec) {  // (the width is a multiple of EPV)
+#pragma unroll
+          for (int k = 0; k < 32; k += EPV)
+            if (x.n0 + half + i + k < width) *reinterpret_cast<uint4 *>(to + i + k) = pack16<OUT>(v + k);
+        } else if (row < x.rows) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (x.n0 + half + i + k < width) to[i + k] = from_f32<OUT>(v[k]);
+        }
+      }
+    };
     Tile x;
     for (; ok && tiles.next(x); ++count) {
       const bool live = q * 32 < x.rows && x.n0 + half < width;
@@ -580,24 +614,14 @@ experts_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             // an infinite operand's products with lower planes (of either sign, or zero) say nothing
             if (c >= x.c1) add(lane_tmem + (2 + (count & 1)) * NT, true);
           }
+        } else if (LONG && live && x.c1 - x.c0 > kSeg) {
+          add_segment(x, lane_tmem + buf * NT, c - kSeg == x.c0, c >= x.c1);
         } else if (live) {
           for (int i = 0; i < HC / CW; ++i) {
             if (x.n0 + half + i * CW >= width) break;
 #pragma unroll
             for (int k = 0; k < CW / 32; ++k) tmem_ld32(lane_tmem + buf * NT + i * CW + k * 32, *reinterpret_cast<float(*)[32]>(acc + k * 32));
             tmem_wait_ld();
-            if (x.c1 - x.c0 > kLong) {  // with the segments before
-              float *sum = a.sums + ((int64_t)blockIdx.x * NT + half + i * CW) * BM + q * 32 + lane;
-              if (c - kLong > x.c0) {
-#pragma unroll
-                for (int k = 0; k < CW; ++k) acc[k] += sum[k * BM];
-              }
-              if (c < x.c1) {
-#pragma unroll
-                for (int k = 0; k < CW; ++k) sum[k * BM] = acc[k];
-                continue;
-              }
-            }
             if (MODE == kWeights && x.slot >= 0) write_piece(acc, CW, x, half + i * CW);
             else write(acc, x, half + i * CW);
           }
@@ -864,7 +888,7 @@ PieceSizes piece_sizes(int dtype, int64_t R, int K, int d_in, int d_out, int NT)
 // Columns of a tile of DW.
 int weights_tile(int dtype, int d_in) { return dtype == FGMM_F32 || d_in <= 128 ? 128 : 256; }
 
-template <int MODE, int NT, bool SPLIT, typename OUT>
+template <int MODE, int NT, bool SPLIT, bool LONG, typename OUT>
 int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
            void *pieces, float *sums, cudaStream_t st) {
   using Sh = Shape<NT, SPLIT>;
@@ -895,7 +919,7 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   a.sums = sums;
   a.failed = failed_word();
   if (!a.failed) return fail(FGMM_ERR_CUDA, "no pinned memory for the products' error word");
-  auto kernel = experts_tc_kernel<MODE, NT, SPLIT, OUT>;
+  auto kernel = experts_tc_kernel<MODE, NT, SPLIT, LONG, OUT>;
   static std::atomic<bool> done[64];  // per device
   int dev = 0;
   FGMM_CUDA_TRY(cudaGetDevice(&dev));
@@ -935,9 +959,12 @@ template <int MODE, typename OUT>
 int launch16(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, OUT *out,
              void *pieces, float *sums, cudaStream_t st) {
   const int width = MODE == kForward ? d_out : d_in;
-  if (MODE == kWeights ? weights_tile(dtype, d_in) == 256 : wide_tiles(p.R, p.K, width))
-    return launch<MODE, 256, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
-  return launch<MODE, 128, false>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
+  constexpr bool kRows = MODE == kWeights;  // any of the experts may have a long contraction
+  if (!kRows && (MODE == kForward ? d_in : d_out) > kLong * KCH)
+    return launch<MODE, 256, false, true>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
+  if (kRows ? weights_tile(dtype, d_in) == 256 : wide_tiles(p.R, p.K, width))
+    return launch<MODE, 256, false, kRows>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
+  return launch<MODE, 128, false, kRows>(oa, ob, dtype, N, d_in, d_out, p, out, pieces, sums, st);
 }
 
 size_t piece_bytes(int dtype, int64_t R, int K, int d_in, int d_out) {
@@ -1013,7 +1040,7 @@ int products_tc(const void *x, const void *weight, int dtype, int64_t N, int d_i
   const Operand ox = operand(x, dtype, N, d_in, s.x, copies), ow = operand(weight, dtype, (int64_t)p.K * d_out, d_in, s.weight, copies);
   int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
-  if (dtype == FGMM_F32) return launch<kForward, 128, true>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, nullptr, st);
+  if (dtype == FGMM_F32) return launch<kForward, 128, true, false>(ox, ow, dtype, N, d_in, d_out, p, (float *)y, nullptr, nullptr, st);
   if (dtype == FGMM_BF16) return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)y, nullptr, s.sums, st);
   return launch16<kForward>(ox, ow, dtype, N, d_in, d_out, p, (__half *)y, nullptr, s.sums, st);
 }
@@ -1028,12 +1055,12 @@ int products_tc_backward(const void *dy, const void *x, const void *weight, int 
   int rc = run_copies(copies, dtype, st);
   if (rc) return rc;
   if (parts.inputs) {
-    rc = dtype == FGMM_F32 ? launch<kInputs, 128, true>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, nullptr, st)
+    rc = dtype == FGMM_F32 ? launch<kInputs, 128, true, false>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, nullptr, st)
                            : launch16<kInputs>(og, ow, dtype, N, d_in, d_out, p, dx_rows, nullptr, s.sums, st);
     if (rc) return rc;
   }
   if (!parts.weights) return FGMM_OK;
-  if (dtype == FGMM_F32) return launch<kWeights, 128, true>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, nullptr, st);
+  if (dtype == FGMM_F32) return launch<kWeights, 128, true, false>(og, ox, dtype, N, d_in, d_out, p, (float *)d_weight, s.pieces, nullptr, st);
   if (dtype == FGMM_BF16) return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__nv_bfloat16 *)d_weight, s.pieces, s.sums, st);
   return launch16<kWeights>(og, ox, dtype, N, d_in, d_out, p, (__half *)d_weight, s.pieces, s.sums, st);
 }
