@@ -18,7 +18,8 @@
 //   * float32 operands are three bf16 planes (x = b0 + b1 + b2, 24 bits together), laid out by
 //     split_planes_kernel, and the six products that matter (b0 b0 into one accumulator; b0 b1, b1 b0, b1 b1,
 //     b0 b2 and b2 b0, 2^-8 and less of it, into another).  Tensor-memory accumulation truncates, so the
-//     first is drained into fp32 registers every 256 elements of the contraction.
+//     first is drained into fp32 registers every 256 elements of the contraction (the second with the tile: where every factor is the
+//     same, so that its products have one sign, it loses 2^-21.6 of the result over 65,536 elements, 2^-17 over 2^20).
 //   * 16-bit products are drained every 8,192 elements: truncation takes up to 2^-23 of the sum for every 8, of a sum of one sign
 //     2^-27.3 an element (8,192: 2^-14.3, a tenth of the rounding to fp16; undrained 2^20 rows lost 0.6 %).  The sums of a
 //     longer contraction wait in a tile of fp32 for each block, whose threads read and write their own elements only (dW of 64
