@@ -202,6 +202,39 @@ def test_weights_gradient_of_slots_that_order_leaves_out(dtype, N, k, d):
 
 
 # ------------------------------------------------------------------------------ products
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,k,K,d_in,d_out", [(300, 2, 4, 64, 16), (40, 2, 32, 64, 16), (30, 2, 64, 63, 9), (2100, 3, 3, 128, 8), (700, 4, 16, 100, 40)])
+def test_dx_rounds_once(N, k, K, d_in, d_out, dtype):
+    """A point's rows cancel almost: one rounding of their sum is far below a rounding of each row."""
+    g = gen(N + K)
+    w = torch.randn(1, d_out, d_in, generator=g).expand(K, -1, -1) + torch.randn(K, d_out, d_in, generator=g) * 2.0 ** -6
+    w, x = w.to(dtype), torch.randn(N, d_in, generator=g).to(dtype)
+    idx = plan(N, k, K, N + K, dropped=False)
+    routes = C().group_routes(idx.to(DEV), K)
+    order = routes.order.cpu().long()
+    sign = torch.tensor([1.0, -1.0])[order % k % 2]
+    dy = (torch.randn(N, d_out, generator=g)[order // k] * sign[:, None] * 16).to(dtype)
+    _, _, dx, dxa, _, _ = ref.products(x, w, routes.order.cpu(), routes.offsets.cpu(), k, dy)
+    gx = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes, need_dweight=False)[0]
+    close(gx, dx, dxa, d_out + k, dtype, "dx")
+
+
+@pytest.mark.parametrize("dtype,N,k,K,d_in,d_out", [(torch.float32, 300, 1, 64, 40, 72), (torch.float32, 190, 2, 64, 1030, 33), (torch.bfloat16, 250, 1, 64, 63, 40)])
+def test_few_rows_of_one_popular_expert(dtype, N, k, K, d_in, d_out):
+    """Few rows an expert on average, and one of them has most."""
+    idx = torch.full((N, k), 7, dtype=torch.int32)
+    idx[::5, 0] = torch.randint(0, K, (len(idx[::5]),), generator=gen(1), dtype=torch.int32)
+    idx[:, 1:] = (idx[:, :1] + 1) % K
+    x, w = torch.randn(N, d_in, generator=gen(2)).to(dtype), (torch.randn(K, d_out, d_in, generator=gen(3)) / d_in ** 0.5).to(dtype)
+    dy = torch.randn(N * k, d_out, generator=gen(4)).to(dtype)
+    routes = C().group_routes(idx.to(DEV), K)
+    y, ya, dx, dxa, dw, dwa = ref.products(x, w, routes.order.cpu(), routes.offsets.cpu(), k, dy)
+    close(C().expert_products(x.to(DEV), w.to(DEV), routes), y, ya, d_in, dtype, "y")
+    gx, gw = C().expert_products_backward(dy.to(DEV), x.to(DEV), w.to(DEV), routes)
+    close(gx, dx, dxa, d_out + k, dtype, "dx")
+    close(gw, dw, dwa, N * k, dtype, "dw")
+
+
 HALVES = [torch.float16, torch.bfloat16]
 
 
