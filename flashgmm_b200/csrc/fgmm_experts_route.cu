@@ -235,9 +235,21 @@ template <int VPT, int L> __device__ __forceinline__ float softmax_terms(float (
   return seg_sum<L>(total);
 }
 
+// Given values whose sum leaves fp32 on the way: at 2^-6 of their size 32 of them do not.
+template <int L> __device__ __forceinline__ float large_share(float t, float &sum) {
+  const bool large = !(fabsf(sum) < INFINITY);
+  const float less = seg_sum<L>(0x1p-6f * t);
+  if (large) sum = 0x1p6f * less;
+  const float share = large ? 0x1p-6f * t / less : t / sum;
+  return (large ? less : sum) == 0.0f ? 0.0f : share;
+}
+template <int L> __device__ __noinline__ float call_large_share(float t, float *sum) { return large_share<L>(t, *sum); }
+
 // The chosen scores' shares of their sum (lane j: slot j), from the scores themselves, so that a ratio
 // of values that both underflow is still their ratio; `sum` is the sum before the division.
-template <int L> __device__ __forceinline__ float chosen_share(float z, bool live, int func, float &sum) {
+// CALL: the rare case is a call, for the registers (16,384 x 256 with bias and groups 27.0 -> 25.7 us; 65,536 x 1,024 of
+// the scores alone, where it is not, 63.2 against 64.3).
+template <int L, bool CALL> __device__ __forceinline__ float chosen_share(float z, bool live, int func, float &sum) {
   float t = 0.0f;
   if (func == FGMM_SCORE_GIVEN) {
     t = live ? z : 0.0f;
@@ -248,14 +260,9 @@ template <int L> __device__ __forceinline__ float chosen_share(float z, bool liv
     else t = live ? __fdividef(expf(fminf(z, 0.0f) - fminf(m, 0.0f)), 1.0f + expf(-fabsf(z))) : 0.0f;
   }
   sum = seg_sum<L>(t);
-  // given values whose sum leaves fp32 on the way: at 2^-6 of their size 32 of them do not
   if (func == FGMM_SCORE_GIVEN && __any_sync(kFull, !(fabsf(sum) < INFINITY))) {
-    const bool large = !(fabsf(sum) < INFINITY);
-    const float less = seg_sum<L>(0x1p-6f * t);
-    if (large) {
-      sum = 0x1p6f * less;
-      return less == 0.0f ? 0.0f : 0x1p-6f * t / less;
-    }
+    if constexpr (CALL) return call_large_share<L>(t, &sum);
+    else return large_share<L>(t, sum);
   }
   return sum == 0.0f ? 0.0f : t / sum;
 }
@@ -265,10 +272,9 @@ __device__ __forceinline__ void top_two(float &b1, float &b2, float v1, float v2
   b1 = fmaxf(b1, v1);
 }
 
-// Masks all but the top_groups groups of a warp's row.  tol: the relative error of a c near the row's largest (|z - m| 2^-24 of an s
-// farther off is 0.4 2^-24 of the largest s at most, which tol's spare covers).
+// Masks all but the top_groups groups of a warp's row.  tol: the largest error of an s in fp32.
 template <typename T, int VPT, int V>
-__device__ __forceinline__ void keep_groups(float (&c)[VPT], const T *row, const RouteArgs &a, int lane, float m, float bmax, float tol,
+__device__ __forceinline__ void keep_groups(float (&c)[VPT], const T *row, const RouteArgs &a, int lane, float m, float tol,
                                             float2 *s_group) {
   const int per = a.per, span = per / V;
   // a group is `span` neighbouring lanes of one pack of V: all groups' best two meet in log2 span steps
@@ -318,7 +324,8 @@ __device__ __forceinline__ void keep_groups(float (&c)[VPT], const T *row, const
     if (lane == g) key = 0u;
   }
   const uint32_t high = __reduce_max_sync(kFull, key);  // the largest that goes
-  const float lo = of_key(low), hi = of_key(high), cut = 2.0f * tol * (most + 2.0f * bmax) + 1e-36f;
+  // a group's sum is off by tol for each of its two, and by their roundings and its own
+  const float lo = of_key(low), hi = of_key(high), cut = 4.0f * tol + 0x6p-24f * most + 1e-36f;
   if (high != 0u && !(lo - hi > cut)) {
     // those that could be on either side of the border
     const bool in = mine.x - hi > cut, out = !(mine.x > -INFINITY) || lo - mine.x > cut, near = !in && !out;
@@ -406,7 +413,6 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
     left = left == best ? 0u : left;
   }
   const float bar = best != 0u ? of_key(best) : -FLT_MAX;  // (masked values are below it)
-  const float top = bar == FLT_MAX ? INFINITY : bar;       // (+inf counts as the largest finite value)
   constexpr int kWords = (VPT + 31) / 32;
   uint32_t some[kWords], equal[kWords];
   int n = 0;
@@ -420,12 +426,13 @@ __device__ __forceinline__ bool pick_few(const float (&c)[VPT], int rounds, int 
   }
   int count = (int)__reduce_add_sync(kFull, (unsigned)n);
   if (count > 32) {
+    if (bar == FLT_MAX) return false;  // (+inf, which c may hold, equals it)
     n = 0;
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
 #pragma unroll
       for (int i = w * 32; i < VPT && i < w * 32 + 32; ++i)
-        if (c[i] >= bar && c[i] <= top) equal[w] |= 1u << (i & 31);
+        if (c[i] == bar) equal[w] |= 1u << (i & 31);
       some[w] &= ~equal[w];
       n += __popc(some[w]);
     }
@@ -495,14 +502,14 @@ constexpr int kRouteWarps = 4;
 // BY_VALUE: with a bias or groups, where the values c decide; else the scores do.
 template <typename T, int VPT, int V, int L, bool BY_VALUE>
 __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T, VPT> &raw, const RouteArgs &a, int l, const float *s_bias,
-                                          float bmax, uint64_t *s_cand, float *weights, int32_t *indices) {
-  // fp32 values of c are off by at most 16 2^-24 of |s| and |bias| (exp, the quotient, the bias, a few steps of the softmax's
-  // sum), and those of a softmax by VPT 2^-24 (a lane's part of the sum) and |z - m| 2^-24 (the exponent's rounding) more:
-  // two that differ by more than this (times their sizes) are in the right order
-  constexpr float kTol = 0x1p-20f;
+                                          uint64_t *s_cand, float *weights, int32_t *indices) {
   float c[VPT], m = 0.0f, total = 1.0f, inv = 1.0f;
-  const auto tolerance = [&](float z1, float z2) {
-    return a.func == FGMM_SCORE_SOFTMAX ? fmaf(m - fminf(z1, z2) + (float)VPT, 0x1p-24f, kTol) : kTol;
+  // How far fp32 values are off, in 2^-24 of s: a softmax's by the exponent's rounding (|z - m|, of the terms of its sum 7 on average
+  // at most), the sum's length in a lane and over the lanes, exp and the quotient; a sigmoid's by exp and the reciprocal.  c = s + bias
+  // adds half a step of c (taken as 2^-23).  Two values that differ by more than both errors are in the right order.
+  const auto error = [&](float z, float s, float c) {
+    const float steps = a.func == FGMM_SCORE_SOFTMAX ? m - z + (VPT + 20.0f) : a.func == FGMM_SCORE_SIGMOID ? 8.0f : 0.0f;
+    return fmaf(0x1p-24f * steps, fabsf(s), 0x1p-23f * fabsf(c));
   };
 #pragma unroll
   for (int i = 0; i < VPT; ++i) c[i] = to_f32(raw.v[i]);
@@ -536,7 +543,8 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
       for (int i = 0; i < VPT; ++i) c[i] = fmaxf(c[i] + s_bias[column<V, L>(i, l)], -INFINITY);  // -inf for NaN
     }
     if constexpr (L == 32)
-      if (a.n_groups > 1) keep_groups<T, VPT, V>(c, row, a, l, m, bmax, tolerance(m, m), reinterpret_cast<float2 *>(s_cand));
+      if (a.n_groups > 1)  // (the largest s is 1 / total or 1, and |z - m| s 0.4 of it at most)
+        keep_groups<T, VPT, V>(c, row, a, l, m, error(m, inv, 0.0f), reinterpret_cast<float2 *>(s_cand));
   }
   const bool rounded = BY_VALUE && (a.func != FGMM_SCORE_GIVEN || a.bias);  // c is not exact
   const int rounds = min(L, rounded ? a.top_k + 2 : a.top_k);
@@ -562,9 +570,10 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
   if (rounded) {
     const bool have = chosen >= 0;
     const float z = have ? score_at(row, chosen) : 0.0f, b = have && a.bias ? s_bias[chosen] : 0.0f;
+    const float off = error(z, fminf(fabsf(value) + fabsf(b), inv), value);  // (s by its bounds: the largest is 1 / total or 1)
     const int prev = __shfl_up_sync(kFull, chosen, 1, L);
     const float pv = __shfl_up_sync(kFull, value, 1, L), pz = __shfl_up_sync(kFull, z, 1, L), pb = __shfl_up_sync(kFull, b, 1, L);
-    const bool apart = pv - value > tolerance(pz, z) * (fabsf(pv) + fabsf(value) + 2.0f * bmax) + 1e-36f;  // (of the value before)
+    const bool apart = pv - value > __shfl_up_sync(kFull, off, 1, L) + off + 1e-36f;  // (of the value before)
     const bool near = l > 0 && l <= a.top_k && have && prev >= 0 && !apart && !(pz == z && pb == b);
     const bool border = l < rounds && (have ? l >= a.top_k && prev >= 0 && apart : l >= a.top_k || l == rounds - 1);
     // (all lanes take part in what follows, whatever their rows need)
@@ -572,7 +581,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
     bool whole = false;
     if (__any_sync(kFull, open)) {
       // no gap behind the slots: whether all that is near the last value is the same score and bias (then its order is known)
-      const float lv = seg_get<L>(value, rounds - 1), lz = seg_get<L>(z, rounds - 1), lb = seg_get<L>(b, rounds - 1);
+      const float lv = seg_get<L>(value, rounds - 1), lz = seg_get<L>(z, rounds - 1), lb = seg_get<L>(b, rounds - 1), lo = seg_get<L>(off, rounds - 1);
       bool other = false;
 #pragma unroll 1
       for (int q = 0; q < VPT * L; q += L) {
@@ -580,11 +589,11 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
         if (col >= a.K) break;
         const float u = score_at(row, col), v = a.bias ? s_bias[col] : 0.0f;
         // (a group's masks are in c only: its experts count as near ones here)
-        float x = u;
-        if (a.func == FGMM_SCORE_SOFTMAX) x = expf(u - m) * inv;
-        else if (a.func == FGMM_SCORE_SIGMOID) x = sigmoid(u);
-        x += v;
-        if (u > -INFINITY && x > -INFINITY && !(fabsf(lv - x) > tolerance(lz, u) * (fabsf(lv) + fabsf(x) + 2.0f * bmax) + 1e-36f)) other |= !(u == lz && v == lb);
+        float t = u;
+        if (a.func == FGMM_SCORE_SOFTMAX) t = expf(u - m) * inv;
+        else if (a.func == FGMM_SCORE_SIGMOID) t = sigmoid(u);
+        const float x = t + v;
+        if (u > -INFINITY && x > -INFINITY && !(fabsf(lv - x) > lo + error(u, t, x) + 1e-36f)) other |= !(u == lz && v == lb);
       }
       whole = seg_ballot<L>(other) != 0 && open;
     }
@@ -619,7 +628,7 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
   float w;
   if (a.renorm) {
     float sum;
-    w = chosen_share<L>(z, live, a.func, sum);
+    w = chosen_share<L, BY_VALUE>(z, live, a.func, sum);
   } else if (a.func == FGMM_SCORE_SOFTMAX) {
     w = expf(z - m) / total;
   } else {
@@ -651,15 +660,9 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
   griddep_launch();
   Row<T, VPT> raw;
   if (n - seg < a.N) load_row<T, VPT, V, L>(at(n), a.K, l, raw);
-  float bmax = 0.0f;  // the largest finite |bias|
   if (BY_VALUE && a.bias) {
     for (int c = threadIdx.x; c < VPT * L; c += blockDim.x) s_bias[c] = c < a.K ? __ldg(a.bias + c) : 0.0f;
     __syncthreads();
-    for (int c = lane; c < VPT * L; c += 32) {
-      const float b = fabsf(s_bias[c]);
-      if (b < INFINITY) bmax = fmaxf(bmax, b);
-    }
-    bmax = seg_max<32>(bmax);
   }
   if (n - seg >= a.N) return;
   for (;;) {
@@ -670,7 +673,7 @@ route_kernel(const T *__restrict__ scores, const RouteArgs a, float *__restrict_
     if constexpr (kAhead)
       if (more) load_row<T, VPT, V, L>(at(next), a.K, l, ahead);
     const bool exists = n < a.N;
-    route_row<T, VPT, V, L, BY_VALUE>(at(n), exists, raw, a, l, s_bias, bmax, s_cand[warp], weights + n * a.top_k, indices + n * a.top_k);
+    route_row<T, VPT, V, L, BY_VALUE>(at(n), exists, raw, a, l, s_bias, s_cand[warp], weights + n * a.top_k, indices + n * a.top_k);
     if (!more) break;
     n = next;
     if constexpr (kAhead) raw = ahead;
@@ -718,7 +721,7 @@ __global__ void __launch_bounds__(128, DENSE ? (VPT <= 16 ? 8 : 1) : 12) route_b
     } else {
       if (a.renorm) {
         float sum;
-        const float p = chosen_share<L>(z, live, a.func, sum);
+        const float p = chosen_share<L, false>(z, live, a.func, sum);
         d = g - seg_sum<L>(p * g);
         if (a.func == FGMM_SCORE_GIVEN) d = sum == 0.0f ? 0.0f : d / sum;
         else d *= a.func == FGMM_SCORE_SIGMOID ? p / (1.0f + expf(z)) : p;
