@@ -33,6 +33,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "fgmm_experts.cuh"
@@ -96,7 +97,6 @@ struct Pieces {
 
 struct TcArgs {
   RoutePlan plan;
-  int64_t N;
   int d_in, d_out;
   int a_plane, b_plane;  // columns between the planes of A's and B's rows (float32)
   const uint16_t *a_rows, *b_rows;  // the same matrices for the gathering warps
@@ -791,24 +791,28 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant
 
 // A word of pinned host memory for each device, which a product whose wait ran out sets: the next product on that device fails
 // with it.  Allocated with the first product (also where that is being captured: nothing of it goes into the graph).
-int *failed_word() {
+constexpr int kDevices = 16;  // (one cache line, which every call reads)
+std::atomic<int *> g_failed{nullptr};
+int *failed_words() {
+  if (int *words = g_failed.load(std::memory_order_acquire)) return words;
   static std::mutex mutex;
-  static int *words = nullptr;
-  constexpr int kDevices = 64;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
   std::lock_guard<std::mutex> lock(mutex);
-  if (!words) {
-    void *p = nullptr;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    if (e != cudaSuccess) return nullptr;
-    words = static_cast<int *>(p);
-    std::fill(words, words + kDevices, 0);
-  }
-  return words + dev % kDevices;
+  if (int *words = g_failed.load(std::memory_order_acquire)) return words;
+  void *p = nullptr;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const cudaError_t e = cudaHostAlloc(&p, kDevices * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return nullptr;
+  std::fill(static_cast<int *>(p), static_cast<int *>(p) + kDevices, 0);
+  g_failed.store(static_cast<int *>(p), std::memory_order_release);
+  return static_cast<int *>(p);
+}
+// The current device's.
+int *failed_word() {
+  int dev = 0;
+  int *words = cudaGetDevice(&dev) == cudaSuccess ? failed_words() : nullptr;
+  return words ? words + dev % kDevices : nullptr;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -901,7 +905,6 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   if (rc) return rc;
   TcArgs a{};
   a.plan = p;
-  a.N = N;
   a.d_in = d_in;
   a.d_out = d_out;
   a.a_plane = oa.plane;
@@ -918,12 +921,13 @@ int launch(const Operand &oa, const Operand &ob, int dtype, int64_t N, int d_in,
   a.vec32 = (width * sizeof(OUT)) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   a.vec = (width * sizeof(OUT)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   a.sums = sums;
-  a.failed = failed_word();
-  if (!a.failed) return fail(FGMM_ERR_CUDA, "no pinned memory for the products' error word");
   auto kernel = experts_tc_kernel<MODE, NT, SPLIT, LONG, OUT>;
   static std::atomic<bool> done[64];  // per device
   int dev = 0;
   FGMM_CUDA_TRY(cudaGetDevice(&dev));
+  a.failed = failed_words();
+  if (!a.failed) return fail(FGMM_ERR_CUDA, "no pinned memory for the products' error words");
+  a.failed += dev % kDevices;
   if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
     FGMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::smem(kMaxExperts)));
     if (dev < 64) done[dev].store(true, std::memory_order_release);
@@ -991,6 +995,10 @@ int *experts_error_word() { return failed_word(); }
 // Takes an earlier product's failure.  The device's word is cleared in the stream's order, so that later waits do not give up
 // for it; a capture leaves both words as they are.
 int take_failure(cudaStream_t st) {
+  const volatile int *words = g_failed.load(std::memory_order_acquire);
+  int any = 0;
+  for (int i = 0; words && i < kDevices; ++i) any |= words[i];
+  if (any == 0) return FGMM_OK;  // (asking for the current device would cost a small call more)
   volatile int *word = failed_word();
   const int code = word ? *word : 0;
   if (code == 0) return FGMM_OK;
