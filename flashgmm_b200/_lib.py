@@ -68,6 +68,8 @@ SIGNATURES = {
     "fgmm_expert_products_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp,
                                                      _i32, _vp, _vp, _vp, _sz, _vp]),
     "fgmm_combine_experts": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "fgmm_combine_experts_backward_placed": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i32,
+                                                            _vp, _vp, _vp]),
     "fgmm_combine_experts_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp,
                                                      _vp, _vp]),
 }

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, 
   }
 }
 
-// d_weights of the slots that `order` leaves out (a plan of a part of the experts) stay 0.
+// d_weights of the slots that `order` leaves out (a plan of a part of the experts) stay 0; not needed where position is at hand.
 __global__ void __launch_bounds__(256) zero_weights_kernel(float *__restrict__ d_weights, int64_t R) {
   griddep_wait();
   griddep_launch();
@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(256) zero_weights_kernel(float *__restrict__ d
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restrict__ d_out, const T *__restrict__ y, int d,
                                                                const float *__restrict__ weights, RoutePlan p,
-                                                               T *__restrict__ dy, float *__restrict__ d_weights) {
+                                                               const int32_t *__restrict__ position, T *__restrict__ dy,
+                                                               float *__restrict__ d_weights) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
@@ -262,6 +263,11 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
   if (r >= p.R) return;
   const int id = __ldg(p.order + r);
   const bool known = id >= 0 && id < p.R, live = known && r < __ldg(p.offsets + p.K);
+  if (position && lane == 1) {  // slot r: 0 where its place does not lead back to it
+    const int at = __ldg(position + r);
+    if (at < 0 || at >= p.R || __ldg(p.order + at) != r) d_weights[r] = 0.0f;
+  }
+  const bool placed = known && (!position || __ldg(position + id) == r);
   T *to = dy + r * d;
   float dot = 0.0f;
   if (live) {
@@ -295,7 +301,7 @@ __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restri
     const float zeros[V] = {};
     for (int c = lane * V; c < d; c += 32 * V) store_pack<T, V>(to + c, zeros);
   }
-  if (lane == 0 && known) d_weights[id] = dot;
+  if (lane == 0 && placed) d_weights[id] = dot;
 }
 
 template <bool ENDS, typename TY, typename T>
@@ -326,16 +332,17 @@ int combine_forward_t(const TY *y, int64_t R, int d, const float *w, const int32
 }
 
 template <typename T>
-int combine_backward_t(const T *g, const T *y, int d, const float *w, const RoutePlan &p, T *dy, float *dw, cudaStream_t st) {
+int combine_backward_t(const T *g, const T *y, int d, const float *w, const RoutePlan &p, const int32_t *position, T *dy, float *dw, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = d % V == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(dy) % 16 == 0;
   const unsigned grid = (unsigned)cdiv(p.R, 4);
-  FGMM_CUDA_TRY(launch_pdl(zero_weights_kernel, dim3((unsigned)std::min<int64_t>(cdiv(p.R, 256), 8 * num_sms())), dim3(256), 0, st, dw, p.R));
+  if (!position)
+    FGMM_CUDA_TRY(launch_pdl(zero_weights_kernel, dim3((unsigned)std::min<int64_t>(cdiv(p.R, 256), 8 * num_sms())), dim3(256), 0, st, dw, p.R));
   auto *kernel = !vec ? combine_backward_kernel<T, 1, 4>
                  : d <= 32 * V ? combine_backward_kernel<T, V, 1>
                  : d <= 64 * V ? combine_backward_kernel<T, V, 2> : combine_backward_kernel<T, V, 4>;
-  FGMM_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(128), 0, st, g, y, d, w, p, dy, dw));
+  FGMM_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(128), 0, st, g, y, d, w, p, position, dy, dw));
   return FGMM_OK;
 }
 
@@ -394,10 +401,10 @@ int sum_rows(const float *rows, int parts, int dtype, int d, const RoutePlan &p,
 }
 
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,
-                     const RoutePlan &plan, void *dy, float *d_weights, cudaStream_t st) {
-  if (dtype == FGMM_F32) return combine_backward_t((const float *)d_out, (const float *)y, d, weights, plan, (float *)dy, d_weights, st);
-  if (dtype == FGMM_BF16) return combine_backward_t((const __nv_bfloat16 *)d_out, (const __nv_bfloat16 *)y, d, weights, plan, (__nv_bfloat16 *)dy, d_weights, st);
-  return combine_backward_t((const __half *)d_out, (const __half *)y, d, weights, plan, (__half *)dy, d_weights, st);
+                     const RoutePlan &plan, const int32_t *position, void *dy, float *d_weights, cudaStream_t st) {
+  if (dtype == FGMM_F32) return combine_backward_t((const float *)d_out, (const float *)y, d, weights, plan, position, (float *)dy, d_weights, st);
+  if (dtype == FGMM_BF16) return combine_backward_t((const __nv_bfloat16 *)d_out, (const __nv_bfloat16 *)y, d, weights, plan, position, (__nv_bfloat16 *)dy, d_weights, st);
+  return combine_backward_t((const __half *)d_out, (const __half *)y, d, weights, plan, position, (__half *)dy, d_weights, st);
 }
 
 }  // namespace fgmm

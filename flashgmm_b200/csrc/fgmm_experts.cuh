@@ -63,8 +63,9 @@ int combine_forward(const void *y, int dtype, int64_t R, int d, const float *wei
 // skipped whatever position says.
 int sum_rows(const float *rows, int parts, int dtype, int d, const RoutePlan &plan, const int32_t *position, int64_t N, void *out,
              cudaStream_t st);
+// Without position (which may be null) a launch more sets the gradients of slots that order leaves out.
 int combine_backward(const void *d_out, const void *y, int dtype, int d, const float *weights,
-                     const RoutePlan &plan, void *dy, float *d_weights, cudaStream_t st);
+                     const RoutePlan &plan, const int32_t *position, void *dy, float *d_weights, cudaStream_t st);
 
 // ---- fgmm_experts_few.cu: CUDA-core products for a few rows an expert ----
 int products_few(const void *x, const void *weight, int dtype, int64_t N, int d_in, int d_out, const RoutePlan &p, void *y, cudaStream_t st);

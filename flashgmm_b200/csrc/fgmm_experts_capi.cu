@@ -205,6 +205,13 @@ int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, con
 int fgmm_combine_experts_backward(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
                                   const float *weights, const int32_t *order, const int32_t *offsets,
                                   int32_t K, int32_t top_k, void *dy, float *d_weights, void *stream) {
+  return fgmm_combine_experts_backward_placed(d_out, y, dtype, N, d, weights, order, offsets, nullptr, K, top_k, dy, d_weights, stream);
+}
+
+int fgmm_combine_experts_backward_placed(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
+                                         const float *weights, const int32_t *order, const int32_t *offsets,
+                                         const int32_t *position, int32_t K, int32_t top_k, void *dy,
+                                         float *d_weights, void *stream) {
   int rc = check_experts(dtype, N, K, top_k);
   if (!rc) rc = check_widths(d, d);
   if (rc || N == 0) return rc;
@@ -213,7 +220,7 @@ int fgmm_combine_experts_backward(const void *d_out, const void *y, int32_t dtyp
   if (!aligned(d_out, elem_size(dtype)) || !aligned(y, elem_size(dtype)) || !aligned(dy, elem_size(dtype)))
     return fail(FGMM_ERR_INVALID, "d_out, y and dy must be aligned to their elements");
   const RoutePlan plan{order, offsets, N * top_k, K, top_k};
-  return combine_backward(d_out, y, dtype, d, weights, plan, dy, d_weights, (cudaStream_t)stream);
+  return combine_backward(d_out, y, dtype, d, weights, plan, position, dy, d_weights, (cudaStream_t)stream);
 }
 
 }  // extern "C"

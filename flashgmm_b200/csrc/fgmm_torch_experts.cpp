@@ -51,7 +51,7 @@ void check_shape(const Tensor &t, const char *name, std::initializer_list<int64_
 }
 
 // Contiguous, with the values in memory (a view may hold them negated).
-Tensor dense(const Tensor &t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+Tensor dense(const Tensor &t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
 
 // Rows contiguous; the row stride stays (an expanded or sliced matrix is not copied).
 Tensor with_rows(const Tensor &t) {
@@ -275,9 +275,10 @@ std::tuple<Tensor, Tensor> combine_experts_backward(const Tensor &d_out, const T
   TORCH_CHECK(d >= 1, "y must have at least one column");
   const Tensor yc = dense(y), gc = dense(d_out), w = dense(weights);
   Tensor dy = fresh({p.R, d}, y.scalar_type(), dev), dw = fresh({p.N, p.top_k}, torch::kFloat32, dev);
-  check_rc(fgmm_combine_experts_backward(gc.data_ptr(), yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(),
-                                         p.order.data_ptr<int32_t>(), p.offsets.data_ptr<int32_t>(), p.K, p.top_k,
-                                         dy.data_ptr(), dw.data_ptr<float>(), stream()),
+  check_rc(fgmm_combine_experts_backward_placed(gc.data_ptr(), yc.data_ptr(), dtype, p.N, narrow(d, "d"), w.data_ptr<float>(),
+                                                p.order.data_ptr<int32_t>(), p.offsets.data_ptr<int32_t>(),
+                                                p.position.data_ptr<int32_t>(), p.K, p.top_k, dy.data_ptr(),
+                                                dw.data_ptr<float>(), stream()),
            "combine_experts_backward");
   return {dy, dw};
 }

@@ -282,6 +282,12 @@ int fgmm_combine_experts(const void *y, int32_t dtype, int64_t N, int32_t d, con
 int fgmm_combine_experts_backward(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
                                   const float *weights, const int32_t *order, const int32_t *offsets,
                                   int32_t K, int32_t top_k, void *dy, float *d_weights, void *stream);
+/* The same with the plan's position (which may be NULL), which spares a launch: a slot's gradient comes from the row that its
+ * position leads to, where `order` leads back to the slot, and is 0 elsewhere. */
+int fgmm_combine_experts_backward_placed(const void *d_out, const void *y, int32_t dtype, int64_t N, int32_t d,
+                                         const float *weights, const int32_t *order, const int32_t *offsets,
+                                         const int32_t *position, int32_t K, int32_t top_k, void *dy,
+                                         float *d_weights, void *stream);
 
 /* Size of the fixed device scratch array behind fgmm_em_fused_static. */
 #define FGMM_STATIC_SCRATCH_BYTES (16u << 20)
