@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) zero_weights_kernel(float *__restrict__ d
 }
 
 // A warp per grouped row r of route order[r]: dy[r] = w dout[point], dw = <dout[point], y[r]>; U packs of both rows
-// are on their way at once.  16,411 points of 2 rows of 1,000 fp32 (328 MB) 54 us, 6.1 TB/s.
+// are on their way at once.  16,411 points of 2 rows of 1,000 fp32 (328 MB) 56 us, 5.9 TB/s.
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(128) combine_backward_kernel(const T *__restrict__ d_out, const T *__restrict__ y, int d,
                                                                const float *__restrict__ weights, RoutePlan p,

@@ -35,6 +35,12 @@ int check_widths(int d_in, int d_out) {
 //   dW float32    25 / 51   29 / 53   35 / 54    44 / 60    66 / 62
 //   dW bf16       15 / 26   19 / 27   27 / 27    28 / 27
 // and at 16 rows of 509 x 1,024 bf16: y 154 / 55, dx 196 / 54, dW 112 / 101.
+// The host knows the mean only.  dW gives an expert's rows to one column of blocks there, one row after the other, and a popular
+// expert is slow; us with the rows spread evenly / half of them on one expert / all on one:
+//   24,576 rows, 4,096 experts of 64 x 64 float32   55 / 6,010 / 11,560
+//   384 rows, 64 experts of 512 x 1,024 float32     63 / 402 / 846
+//   4,096 rows, 4,096 experts of 64 x 64 bf16       27 / 820 / 1,640
+// y and dx give windows of rows to the blocks and gain by it (108 / 92 / 79 and 91 / 64 / 50 at the first).
 TcParts on_tensor_cores(int dtype, int64_t R, int K, int d_in, int d_out) {
   const bool f32 = dtype == FGMM_F32, in_copied = f32 || d_in % 8 != 0, out_copied = in_copied || d_out % 8 != 0;
   const auto few = [&](int rows) { return R <= (int64_t)rows * K; };

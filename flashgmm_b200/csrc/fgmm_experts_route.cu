@@ -641,10 +641,11 @@ __device__ __forceinline__ void route_row(const T *row, bool exists, const Row<T
 }
 
 // Instructions bound it where a row is short: at 16,384 bf16 rows of 256 (8 MB, 1.3 us) it takes 10.4 us for 8 of the scores
-// and 25 us with a bias and groups (680 and 1,300 instructions a row; with near values decided by a warp a row, whose one
-// row of 64-bit work others waited for, 37 us); 65,536 rows of 1,024 fp32 responsibilities take 61 us, 4.4 TB/s.
+// and 25 us with a bias and groups (680 and 1,240 instructions a row, a warp a row; with near values decided by a warp a row, whose
+// one row of 64-bit work others waited for, 37 us); 65,536 rows of 1,024 fp32 responsibilities take 62 us, 4.3 TB/s.
 // Resident blocks an SM: where c decides, fewer than the plain rows' (16,384 x 256 10 -> 9: 28.8 -> 25.2 us; 16,384 x 512
-// 7 -> 6: 40.1 -> 38.8; x 1,024 6 -> 5: 61.6 -> 59.9, but the responsibilities 61 -> 69).
+// 7 -> 6: 40.1 -> 38.8; x 1,024 6 -> 5: 61.6 -> 59.9, but the responsibilities 61 -> 69).  At 9 blocks the instance with a bias and
+// groups has 56 registers and spills 150 bytes.
 // The next row is fetched while this one is decided for up to 16 values a lane (more would cost occupancy).
 template <typename T, int VPT, int V, int L, bool BY_VALUE>
 __global__ void __launch_bounds__(32 * kRouteWarps, VPT <= 8 ? (BY_VALUE ? 9 : 10) : VPT <= 16 ? (BY_VALUE ? 6 : 8) : VPT <= 32 ? (BY_VALUE ? 5 : 6) : 2)
