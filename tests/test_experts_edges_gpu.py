@@ -262,7 +262,8 @@ def check_one_sign(got, want, dtype, segments):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("K,d_in,d_out,R", [(64, 256, 896, 1 << 20), (4, 128, 128, 1 << 20), (4, 100, 130, 300001), (64, 512, 1024, 8193), (64, 512, 1024, 70000)])
+@pytest.mark.parametrize("K,d_in,d_out,R", [(64, 256, 896, 1 << 20), (4, 128, 128, 1 << 20), (4, 100, 130, 300001), (64, 512, 1024, 8193), (64, 512, 1024, 70000),
+                                               (4, 2560, 1280, 65613)])
 def test_weights_gradient_of_very_many_rows_of_one_sign(K, d_in, d_out, R, dtype):
     x, dy = one_sign(R, d_in, seed=1, dtype=dtype), one_sign(R, d_out, seed=2, dtype=dtype)
     idx = torch.full((R, 1), 2, dtype=torch.int32, device=DEV)
@@ -292,6 +293,23 @@ def test_products_of_very_wide_rows_of_one_sign(d, other, dtype):
     dx = C().expert_products_backward(dy, torch.zeros(N, other, device=DEV, dtype=dtype), w, routes, need_dweight=False)[0]
     for e in range(K):
         check_one_sign(dx[rows[at[e]]], dy[at[e]].double() @ w[e].double(), dtype, d // 8192 + 1)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+def test_infinities_in_wide_rows_stay_where_they_belong(dtype):
+    N, K, d, d_out = 300, 3, 20000, 72
+    x, w = torch.randn(N, d, generator=gen(1)), torch.randn(K, d_out, d, generator=gen(2)) / 128
+    x[5, 3], x[6, 9000], x[7, 3], x[7, 19999], x[8, 12000] = math.inf, -math.inf, math.inf, math.inf, math.nan
+    x, w = x.to(dtype).to(DEV), w.to(dtype).to(DEV)
+    routes = C().group_routes(torch.arange(N, dtype=torch.int32, device=DEV)[:, None] % K, K)
+    y = C().expert_products(x, w, routes)
+    place = routes.position[:, 0].long()
+    want = torch.stack([(x[n].double() * w[n % K].double()).sum(1) for n in range(5, 9)])
+    got = y[place[5:9]].double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    rest = [n for n in range(N) if not 5 <= n < 9]
+    assert torch.isfinite(y[place[rest]]).all()
 
 
 # --------------------------------------------------------------- waits that have run out
